@@ -1,0 +1,107 @@
+/*
+ * Block-scaled FP8 (e4m3) linear: row quantizer, weight quantizer and matrix
+ * product, device pointers, asynchronous on the context stream. No counterpart
+ * in the reference, whose quantized linear is int8 with one scale per row; this
+ * is the same linear for weights published as e4m3 with one fp32 scale per
+ * 128 x 128 block.
+ *
+ *   scale of a group   s = max(RN(max|x| / 448), 2^-60)
+ *   value              q = e4m3(RN(x / s)), round to nearest even, at most 448
+ *   product            y[m, n] = sum_k (qx[m, k] sx[m, k / 128]) (qw[n, k] sw[n / 128, k / 128]) + bias[n]
+ *
+ * A group of rows with a NaN or an infinity dequantizes to NaN, and so do the
+ * outputs of that row; no other row is affected. Every call allocates nothing
+ * and may be captured into a CUDA graph.
+ */
+#ifndef QPUCUDA_FP8_H
+#define QPUCUDA_FP8_H
+
+#include "qpucuda_runtime.h"
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+#if defined(__GNUC__)
+#pragma GCC visibility push(default)
+#endif
+
+/* Columns (and weight rows) that share one scale. */
+#define QPUCUDA_FP8_GROUP 128u
+
+/* Element types of activations and outputs. */
+typedef enum qpucuda_dtype {
+    QPUCUDA_DTYPE_F32 = 0,
+    QPUCUDA_DTYPE_BF16 = 1,
+    QPUCUDA_DTYPE_F16 = 2
+} qpucuda_dtype;
+
+typedef struct qpucuda_fp8_quantize_desc {
+    const void *x;           /* [source rows][cols], or [..][2 * cols] = gate | up when gated */
+    int x_type;              /* qpucuda_dtype */
+    size_t x_stride;         /* elements */
+    uint32_t rows;           /* quantized rows */
+    uint32_t cols;
+    int gated;               /* nonzero: quantize silu(gate) * up, computed in fp32 */
+    /* Row r is made from source row row_source[r] / row_divisor; a negative entry gives a zero
+     * row. NULL: row r from source row r. Entries are below source_rows * row_divisor. */
+    const int32_t *row_source;
+    uint32_t row_divisor;
+    uint32_t source_rows;
+    uint8_t *q;              /* [rows] rows of q_stride bytes, 16-byte aligned */
+    size_t q_stride;         /* a multiple of 16, at least cols; bytes past cols may be zeroed */
+    float *scales;           /* group g of row r at r * scale_row_stride + g * scale_group_stride */
+    size_t scale_row_stride;
+    size_t scale_group_stride;
+} qpucuda_fp8_quantize_desc;
+
+/* Rows to e4m3 with one scale per 128 columns (the last group may be shorter). */
+qpucuda_status qpucuda_fp8_quantize_rows(qpucuda_context *context, const qpucuda_fp8_quantize_desc *desc);
+
+/* Matrices [batch][rows][cols] (row stride x_stride, matrices rows * x_stride apart) to e4m3
+ * values [batch][rows] of q_stride bytes and scales [batch][ceil(rows/128)][ceil(cols/128)]. */
+qpucuda_status qpucuda_fp8_quantize_blocks(
+    qpucuda_context *context,
+    const void *x, int x_type, size_t x_stride,
+    uint32_t batch, uint32_t rows, uint32_t cols,
+    uint8_t *q, size_t q_stride,
+    float *scales);
+
+typedef struct qpucuda_fp8_gemm_desc {
+    const uint8_t *a;        /* e4m3 [rows] of a_stride bytes */
+    size_t a_stride;         /* multiples of 16, bases 16-byte aligned (as w) */
+    const float *a_scales;   /* strided as in qpucuda_fp8_quantize_desc */
+    size_t a_scale_row_stride;
+    size_t a_scale_group_stride;
+    const uint8_t *w;        /* e4m3 [max(experts, 1)][n] of w_stride bytes */
+    size_t w_stride;
+    const float *w_scales;   /* [max(experts, 1)][ceil(n/128)][ceil(k/128)] */
+    const float *bias;       /* [n] or NULL; NULL with experts */
+    uint32_t rows, n, k;
+    /* 0: one matrix. Otherwise rows [offsets[e], offsets[e + 1]) meet matrix e (offsets: device
+     * int32 [experts + 1], ascending from 0 to at most rows; clamped to that), and rows from
+     * offsets[experts] on become zero. At most QPUCUDA_MAX_EXPERTS. */
+    uint32_t experts;
+    const int32_t *offsets;
+    void *out;               /* [rows][n] */
+    int out_type;            /* qpucuda_dtype */
+    size_t out_stride;       /* elements */
+    /* Nonzero: no kernel that is still unfinished when the one launched just before this call
+     * starts writes w, w_scales or offsets, nor does that one, so they may be read early. */
+    int weights_settled;
+} qpucuda_fp8_gemm_desc;
+
+#define QPUCUDA_MAX_EXPERTS 1024u
+
+qpucuda_status qpucuda_fp8_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc);
+
+#if defined(__GNUC__)
+#pragma GCC visibility pop
+#endif
+#ifdef __cplusplus
+}
+#endif
+
+#endif

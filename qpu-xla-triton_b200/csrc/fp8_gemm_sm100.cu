@@ -1,0 +1,492 @@
+// Block-scaled FP8 product for sm_100a: y[m, n] = sum_b sx[m, b] sw[n / 128, b] p[m, n, b] (+ bias[n]),
+// p[m, n, b] the e4m3 dot product over the 128 columns of block b, accumulated in fp32 by
+// tcgen05.mma (kind::f8f6f4). The scales are arbitrary fp32, so p leaves tensor memory after every
+// block and is added to fp32 registers as fma(p, sx * sw, acc): two roundings of a factor and one of
+// the sum per block.
+//
+// With experts, the rows [offsets[e], offsets[e + 1]) meet matrix e. Tiles are cut inside an
+// expert's rows; the rows of the next expert that a tile's copy also brings in are computed and
+// not stored, the rows no expert owns are zeroed.
+//
+// Rows (tokens) are the narrow side here: the weight is the M = 128 operand and NT rows are the N
+// operand, so a few tokens cost a tile of NT = 16 and not 128. Tensor memory lane = output column,
+// tensor memory column = row.
+#include <cstring>
+
+#include "element.cuh"
+#include "qpucuda_fp8_internal.h"
+#include "qpucuda_internal.h"
+#include "sm100_fp8.cuh"
+
+namespace qpucuda {
+namespace {
+
+using namespace sm100;
+
+constexpr int kBlockN = 128;  // output columns (weight rows) per tile = one row of weight scales
+constexpr int kBlockK = 128;  // columns per stage = one scale group = one swizzle row
+constexpr int kMmaK = 32;     // columns per tcgen05.mma kind::f8f6f4
+constexpr uint32_t kMaxSplit = 8;
+
+struct GemmParams {
+    uint32_t rows, n, k;
+    uint32_t k_blocks, n_blocks;
+    uint32_t experts;  // 0: one matrix
+    const int32_t *offsets;
+    const float *a_scales;
+    size_t a_scale_row_stride, a_scale_group_stride;
+    const float *w_scales;
+    const float *bias;
+    void *out;
+    size_t out_stride;
+    uint32_t weights_settled;
+    unsigned int *error_word;
+};
+
+// The rows of one tile: [row0, row_end) of matrix `expert`, at most the tile's height of them.
+struct Tile {
+    uint32_t expert, row0, row_end;
+    bool valid;
+};
+
+// Whole warp. Tile number `slot` among the tiles of `height` rows cut inside every expert's rows.
+// Offsets that do not ascend within [0, rows] are clamped, so every tile stays inside the rows.
+__device__ __forceinline__ Tile find_tile(const GemmParams &params, uint32_t height, uint32_t slot, uint32_t lane) {
+    Tile tile{0, 0, 0, false};
+    if (params.experts == 0) {
+        tile.row0 = slot * height;
+        tile.row_end = min(params.rows, tile.row0 + height);
+        tile.valid = tile.row0 < params.rows;
+        return tile;
+    }
+    const int32_t rows = static_cast<int32_t>(params.rows);
+    for (uint32_t e0 = 0; e0 < params.experts; e0 += 32) {
+        const uint32_t e = e0 + lane;
+        int32_t begin = 0, end = 0;
+        if (e < params.experts) {
+            begin = min(max(params.offsets[e], 0), rows);
+            end = min(max(params.offsets[e + 1], begin), rows);
+        }
+        const uint32_t tiles = (static_cast<uint32_t>(end - begin) + height - 1) / height;
+        uint32_t through = tiles;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, through, offset);
+            if (lane >= static_cast<uint32_t>(offset)) through += other;
+        }
+        const uint32_t holders = __ballot_sync(0xFFFFFFFFu, slot < through);
+        if (holders != 0) {
+            const int holder = __ffs(static_cast<int>(holders)) - 1;
+            const uint32_t inside = slot - (__shfl_sync(0xFFFFFFFFu, through, holder) - __shfl_sync(0xFFFFFFFFu, tiles, holder));
+            tile.expert = e0 + holder;
+            tile.row0 = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, begin, holder)) + inside * height;
+            tile.row_end = min(static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, end, holder)), tile.row0 + height);
+            tile.valid = true;
+            return tile;
+        }
+        slot -= __shfl_sync(0xFFFFFFFFu, through, 31);
+    }
+    return tile;
+}
+
+// First row that no expert owns.
+__device__ __forceinline__ uint32_t owned_rows(const GemmParams &params) {
+    if (params.experts == 0) return params.rows;
+    return static_cast<uint32_t>(min(max(params.offsets[params.experts], 0), static_cast<int32_t>(params.rows)));
+}
+
+// ---- the narrow kernel ------------------------------------------------------------------------
+
+template <int NT>
+struct Narrow {
+    static constexpr int kWarps = NT >= 128 ? 8 : 4;        // epilogue warps: lane quarters x column halves
+    static constexpr int kColumns = NT / (kWarps / 4);      // accumulators of one epilogue thread
+    static constexpr int kThreads = 64 + 32 * kWarps;
+    static constexpr int kCtasPerSm = NT >= 128 ? 1 : 2;
+    static constexpr int kWBytes = kBlockN * kBlockK;
+    static constexpr int kXBytes = NT * kBlockK;
+    static constexpr int kStageBytes = kWBytes + kXBytes;
+    static constexpr int kStages = NT >= 128 ? 6 : (NT >= 64 ? 4 : 5);
+    static constexpr int kBuffers = NT >= 64 ? (NT >= 128 ? 4 : 4) : 4;  // tensor memory accumulators
+    static constexpr int kTmemColumns = kBuffers * NT;      // a power of two, 64 to 512
+    static constexpr int kScaleFloats = 2 * kColumns;       // per warp: this block's and the next's
+    static constexpr size_t kSharedBytes = static_cast<size_t>(kStages) * kStageBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
+    static_assert(kTmemColumns * kCtasPerSm <= 512, "tensor memory");
+    static_assert(kSharedBytes * kCtasPerSm + 2048 <= 227 * 1024, "shared memory");
+    static_assert(static_cast<size_t>(NT) * kBlockN * 4 <= static_cast<size_t>(kStages) * kStageBytes, "split sums");
+};
+
+template <int STAGES, int BUFFERS>
+struct Control {
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t tmem_full[BUFFERS];
+    uint64_t tmem_empty[BUFFERS];
+    uint64_t drain;
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+
+// Grid: x = column block * split + rank in the cluster, y = tile of rows. The CTAs of a cluster
+// share a tile and split its K blocks; their sums meet in distributed shared memory in rank order,
+// so the result does not depend on timing.
+//   warp 0   copies: a weight and a row box per stage
+//   warp 1   tensor memory and MMA: 4 MMAs per stage into the next of kBuffers accumulators
+//   others   each block's accumulator into registers, scaled; then the sums over the cluster, the store
+template <int NT, typename Out>
+__global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
+    fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                           const GemmParams params) {
+    using Shape = Narrow<NT>;
+    using Ctl = Control<Shape::kStages, Shape::kBuffers>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *stage_w = smem;
+    uint8_t *stage_x = smem + Shape::kStages * Shape::kWBytes;
+    float *scale_rows = reinterpret_cast<float *>(smem + Shape::kStages * Shape::kStageBytes);
+    Ctl *control = reinterpret_cast<Ctl *>(scale_rows + Shape::kWarps * Shape::kScaleFloats);
+    static_assert(sizeof(Ctl) <= 256, "control block");
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t split = cluster_size();
+    const uint32_t rank = cluster_rank();
+    const uint32_t n_block = blockIdx.x / split;
+    const uint32_t n0 = n_block * kBlockN;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Shape::kStages; ++s) {
+            mbar_init(smem_u32(&control->full[s]), 1);
+            mbar_init(smem_u32(&control->empty[s]), 1);
+        }
+        for (int b = 0; b < Shape::kBuffers; ++b) {
+            mbar_init(smem_u32(&control->tmem_full[b]), 1);
+            mbar_init(smem_u32(&control->tmem_empty[b]), Shape::kWarps);
+        }
+        mbar_init(smem_u32(&control->drain), 1);
+        control->abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&control->tmem_base)),
+                     "r"(Shape::kTmemColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = control->tmem_base;
+    const bool early = params.weights_settled != 0;
+    // Weights and offsets that the previous kernel does not write are read before it has finished;
+    // the rows, and every store, wait for it.
+    if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Tile tile = find_tile(params, NT, blockIdx.y, lane);
+    const uint32_t kb_begin = static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * rank / split);
+    const uint32_t kb_end = static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * (rank + 1) / split);
+    const int row0 = static_cast<int>(tile.row0);
+
+    if (!tile.valid) {
+        if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    } else if (warp == 0) {
+        if (lane == 0) {
+            prefetch_tensor_map(&map_w);
+            prefetch_tensor_map(&map_a);
+            const int w_row = static_cast<int>(tile.expert * params.n + n0);
+            auto load_w = [&](uint32_t kb, uint32_t stage) {
+                const uint32_t full = smem_u32(&control->full[stage]);
+                mbar_expect_tx(full, Shape::kStageBytes);
+                tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes), &map_w, full, static_cast<int>(kb * kBlockK), w_row);
+            };
+            auto load_x = [&](uint32_t kb, uint32_t stage) {
+                tma_load_2d(smem_u32(stage_x + stage * Shape::kXBytes), &map_a, smem_u32(&control->full[stage]),
+                            static_cast<int>(kb * kBlockK), row0);
+            };
+            const uint32_t count = kb_end - kb_begin;
+            const uint32_t ahead = min(count, static_cast<uint32_t>(Shape::kStages));
+            for (uint32_t s = 0; s < ahead; ++s) load_w(kb_begin + s, s);
+            if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            for (uint32_t s = 0; s < ahead; ++s) load_x(kb_begin + s, s);
+            uint32_t stage = 0, phase = 1, issued = ahead;
+            bool ok = true;
+            if (ahead == Shape::kStages) {
+                for (uint32_t i = ahead; i < count; ++i) {
+                    ok = wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word);
+                    if (!ok) break;
+                    load_w(kb_begin + i, stage);
+                    load_x(kb_begin + i, stage);
+                    ++issued;
+                    if (++stage == Shape::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                // Let every copy in flight land before the CTA exits: the last use of each stage.
+                for (uint32_t s = 0; s < ahead; ++s) {
+                    const uint32_t uses = (issued - s + Shape::kStages - 1) / Shape::kStages;
+                    wait_drain(smem_u32(&control->full[s]), (uses - 1) & 1u);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            constexpr uint32_t instr = fp8_instr_desc(kBlockN, NT);
+            uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 1;
+            bool ok = true, any = false;
+            for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
+                ok = wait_bounded(smem_u32(&control->tmem_empty[buffer]), buffer_phase, &control->abort_flag, params.error_word) &&
+                     wait_bounded(smem_u32(&control->full[stage]), phase, &control->abort_flag, params.error_word);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t w = smem_desc_sw128(smem_u32(stage_w + stage * Shape::kWBytes));
+                const uint64_t x = smem_desc_sw128(smem_u32(stage_x + stage * Shape::kXBytes));
+#pragma unroll
+                for (int kk = 0; kk < kBlockK / kMmaK; ++kk)
+                    mma_fp8(tmem_base + buffer * NT, w + static_cast<uint64_t>(kk * (kMmaK >> 4)),
+                            x + static_cast<uint64_t>(kk * (kMmaK >> 4)), instr, kk != 0 ? 1u : 0u);
+                mma_commit(smem_u32(&control->empty[stage]));
+                mma_commit(smem_u32(&control->tmem_full[buffer]));
+                any = true;
+                if (++stage == Shape::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                if (++buffer == Shape::kBuffers) {
+                    buffer = 0;
+                    buffer_phase ^= 1u;
+                }
+            }
+            if (!ok && any) {
+                mma_commit(smem_u32(&control->drain));
+                wait_drain(smem_u32(&control->drain), 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        constexpr int kColumns = Shape::kColumns;
+        constexpr int kPerLane = (kColumns + 31) / 32;  // row scales one lane stages per block
+        const uint32_t worker = warp - 2u;
+        const uint32_t quarter = warp & 3u;  // tensor memory lanes this warp may read
+        const uint32_t column0 = (worker / 4u) * kColumns;
+        float *scales = scale_rows + worker * Shape::kScaleFloats;
+        const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n_block) * params.k_blocks;
+        const float *a_scales = params.a_scales + static_cast<size_t>(tile.row0 + column0) * params.a_scale_row_stride;
+        auto fetch = [&](uint32_t kb, float (&row_scale)[kPerLane], float &w_scale) {
+            const bool inside = kb < kb_end;
+            w_scale = inside ? __ldg(w_scales + kb) : 0.0f;
+#pragma unroll
+            for (int p = 0; p < kPerLane; ++p) {
+                const uint32_t j = lane + 32u * p;
+                // rows past the tile hold zeros or another expert's values and are not stored
+                row_scale[p] = inside && j < kColumns && tile.row0 + column0 + j < params.rows
+                                   ? a_scales[static_cast<size_t>(j) * params.a_scale_row_stride + static_cast<size_t>(kb) * params.a_scale_group_stride]
+                                   : 0.0f;
+            }
+        };
+        float row_now[kPerLane], row_next[kPerLane], w_now, w_next;
+        fetch(kb_begin, row_now, w_now);
+        fetch(kb_begin + 1, row_next, w_next);
+        uint64_t acc[kColumns / 2];
+#pragma unroll
+        for (int i = 0; i < kColumns / 2; ++i) acc[i] = 0;
+        const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + column0;
+        uint32_t buffer = 0, buffer_phase = 0;
+        bool ok = true;
+        for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
+            float *products = scales + (kb & 1u) * kColumns;
+#pragma unroll
+            for (int p = 0; p < kPerLane; ++p)
+                if (lane + 32u * p < kColumns) products[lane + 32u * p] = row_now[p] * w_now;
+#pragma unroll
+            for (int p = 0; p < kPerLane; ++p) row_now[p] = row_next[p];
+            w_now = w_next;
+            fetch(kb + 2, row_next, w_next);
+            if (lane == 0) ok = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;  // also orders the products' stores before their loads
+            __syncwarp();
+            if (!ok) break;
+            tc_fence_after();
+            constexpr int kChunk = kColumns < 32 ? kColumns : 32;
+#pragma unroll
+            for (int c = 0; c < kColumns; c += kChunk) {
+                uint32_t r[kChunk];
+                if constexpr (kChunk == 16) {
+                    tmem_load_x16(taddr + buffer * NT + c, r);
+                } else {
+                    tmem_load_x32(taddr + buffer * NT + c, r);
+                }
+                tmem_wait_load(r);
+                if (c + kChunk == kColumns) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
+                }
+#pragma unroll
+                for (int i = 0; i < kChunk; i += 4) {
+                    const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(products + c + i);
+                    acc[(c + i) / 2] = fma2(pack2(r[i], r[i + 1]), s.x, acc[(c + i) / 2]);
+                    acc[(c + i) / 2 + 1] = fma2(pack2(r[i + 2], r[i + 3]), s.y, acc[(c + i) / 2 + 1]);
+                }
+            }
+            if (++buffer == Shape::kBuffers) {
+                buffer = 0;
+                buffer_phase ^= 1u;
+            }
+        }
+        const uint32_t column = quarter * 32u + lane;  // output column inside the block
+        if (split > 1) {
+            // Every MMA of this CTA has completed, so its stages are free: partial[row][column].
+            float *partial = reinterpret_cast<float *>(smem);
+#pragma unroll
+            for (int i = 0; i < kColumns / 2; ++i) {
+                partial[(column0 + 2 * i) * kBlockN + column] = low(acc[i]);
+                partial[(column0 + 2 * i + 1) * kBlockN + column] = high(acc[i]);
+            }
+        } else if (ok && n0 + column < params.n) {
+            const float bias = params.bias != nullptr ? __ldg(params.bias + n0 + column) : 0.0f;
+            Out *out = static_cast<Out *>(params.out) + static_cast<size_t>(tile.row0 + column0) * params.out_stride + n0 + column;
+            const uint32_t rows = tile.row_end - tile.row0 > column0 ? tile.row_end - tile.row0 - column0 : 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < kColumns; ++i) {
+                const float v = (i & 1u) ? high(acc[i / 2]) : low(acc[i / 2]);
+                if (i < rows) out[i * params.out_stride] = from_float<Out>(v + bias);
+            }
+        }
+    }
+    if (split > 1) {
+        __syncwarp();
+        cluster_sync();  // every CTA's partial sums are in place
+        if (tile.valid && warp >= 2) {
+            const uint32_t rows = tile.row_end - tile.row0;
+            const float *partial = reinterpret_cast<const float *>(smem);
+            // the tile's rows in turn over the ranks and the warp groups, 128 columns across
+            const uint32_t worker = threadIdx.x - 64u;
+            const uint32_t column = worker % kBlockN;
+            const bool inside = n0 + column < params.n;
+            const float bias = params.bias != nullptr && inside ? __ldg(params.bias + n0 + column) : 0.0f;
+            constexpr uint32_t kGroups = Shape::kWarps / 4;
+            for (uint32_t row = rank * kGroups + worker / kBlockN; row < rows; row += split * kGroups) {
+                const uint32_t address = smem_u32(partial + row * kBlockN + column);
+                float sum = 0.0f;
+                for (uint32_t r = 0; r < split; ++r) sum += load_cluster(map_to_rank(address, r));
+                if (inside)
+                    static_cast<Out *>(params.out)[static_cast<size_t>(tile.row0 + row) * params.out_stride + n0 + column] =
+                        from_float<Out>(sum + bias);
+            }
+        }
+    }
+    if (params.experts != 0 && rank == 0 && warp >= 2) {
+        const uint32_t worker = threadIdx.x - 64u;
+        const uint32_t column = n0 + worker % kBlockN;
+        if (column < params.n)
+            for (uint32_t row = owned_rows(params) + blockIdx.y * (Shape::kWarps / 4) + worker / kBlockN; row < params.rows;
+                 row += gridDim.y * (Shape::kWarps / 4))
+                static_cast<Out *>(params.out)[static_cast<size_t>(row) * params.out_stride + column] = from_float<Out>(0.0f);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Shape::kTmemColumns)
+                     : "memory");
+    }
+}
+
+template <int NT, typename Out>
+cudaError_t launch_narrow(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, uint32_t tiles,
+                          uint32_t split, cudaStream_t stream) {
+    using Shape = Narrow<NT>;
+    static PerDeviceOnce configured;
+    const cudaError_t error = configured.run([] {
+        return cudaFuncSetAttribute(fp8_gemm_narrow_kernel<NT, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(Shape::kSharedBytes));
+    });
+    if (error != cudaSuccess) return error;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = split;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(params.n_blocks * split, tiles, 1);
+    config.blockDim = dim3(Shape::kThreads);
+    config.dynamicSmemBytes = Shape::kSharedBytes;
+    config.stream = stream;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, fp8_gemm_narrow_kernel<NT, Out>, map_w, map_a, params);
+}
+
+template <typename Out>
+cudaError_t launch_narrow_rows(int nt, const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
+                               uint32_t tiles, uint32_t split, cudaStream_t stream) {
+    switch (nt) {
+        case 16: return launch_narrow<16, Out>(map_w, map_a, params, tiles, split, stream);
+        case 32: return launch_narrow<32, Out>(map_w, map_a, params, tiles, split, stream);
+        case 64: return launch_narrow<64, Out>(map_w, map_a, params, tiles, split, stream);
+        default: return launch_narrow<128, Out>(map_w, map_a, params, tiles, split, stream);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word, int sm_count,
+                            cudaStream_t stream) {
+    GemmParams params{};
+    params.rows = desc.rows;
+    params.n = desc.n;
+    params.k = desc.k;
+    params.k_blocks = (desc.k + kBlockK - 1) / kBlockK;
+    params.n_blocks = (desc.n + kBlockN - 1) / kBlockN;
+    params.experts = desc.experts;
+    params.offsets = desc.offsets;
+    params.a_scales = desc.a_scales;
+    params.a_scale_row_stride = desc.a_scale_row_stride;
+    params.a_scale_group_stride = desc.a_scale_group_stride;
+    params.w_scales = desc.w_scales;
+    params.bias = desc.bias;
+    params.out = desc.out;
+    params.out_stride = desc.out_stride;
+    params.weights_settled = desc.weights_settled != 0 ? 1u : 0u;
+    params.error_word = error_word;
+    const uint64_t matrices = desc.experts != 0 ? desc.experts : 1u;
+    // The tile's height: the smallest that holds an expert's even share of the rows.
+    const uint64_t share = (desc.rows + matrices - 1) / matrices;
+    const int nt = share <= 16 ? 16 : (share <= 32 ? 32 : (share <= 64 ? 64 : 128));
+    CUtensorMap map_w, map_a;
+    if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
+        !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, static_cast<uint32_t>(nt))) {
+        return cudaErrorInvalidValue;
+    }
+    // At most this many tiles of rows, whatever the offsets: one partly filled tile per matrix.
+    const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;
+    const uint64_t tiles = (static_cast<uint64_t>(desc.rows) + filled * (nt - 1)) / nt;
+    if (tiles > 65535u) return cudaErrorInvalidValue;
+    // K is split over a cluster while the tiles leave SMs idle, two CTAs each.
+    uint32_t split = 1;
+    while (split < kMaxSplit && tiles * params.n_blocks * split * 2 <= static_cast<uint64_t>(sm_count) * 2 &&
+           split * 2 <= params.k_blocks) {
+        split *= 2;
+    }
+    const uint32_t grid_tiles = static_cast<uint32_t>(tiles);
+    switch (desc.out_type) {
+        case QPUCUDA_DTYPE_F32: return launch_narrow_rows<float>(nt, map_w, map_a, params, grid_tiles, split, stream);
+        case QPUCUDA_DTYPE_BF16: return launch_narrow_rows<__nv_bfloat16>(nt, map_w, map_a, params, grid_tiles, split, stream);
+        case QPUCUDA_DTYPE_F16: return launch_narrow_rows<__half>(nt, map_w, map_a, params, grid_tiles, split, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace qpucuda

@@ -1,0 +1,35 @@
+// Launchers of the block-scaled FP8 linear and of the expert routing (arguments already checked).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "qpucuda_experts.h"
+#include "qpucuda_fp8.h"
+
+namespace qpucuda {
+
+cudaError_t launch_fp8_quantize_rows(const qpucuda_fp8_quantize_desc &desc, int sm_count, cudaStream_t stream);
+cudaError_t launch_fp8_quantize_blocks(const void *x, int x_type, size_t x_stride, uint32_t batch, uint32_t rows,
+                                       uint32_t cols, uint8_t *q, size_t q_stride, float *scales, cudaStream_t stream);
+// error_word: the context's, for the kernel's bounded waits. cudaErrorInvalidValue when an operand
+// cannot be described to the copy engine.
+cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word, int sm_count,
+                            cudaStream_t stream);
+
+size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts);
+cudaError_t launch_expert_sort(const void *ids, bool ids_64, uint32_t tokens, uint32_t choices, uint32_t experts,
+                               int32_t *offsets, int32_t *source, int32_t *position, void *workspace, int sm_count,
+                               cudaStream_t stream);
+cudaError_t launch_expert_gather(const void *x, int type, size_t x_stride, uint32_t tokens, uint32_t choices,
+                                 uint32_t width, const int32_t *position, const int32_t *offsets, uint32_t experts,
+                                 void *rows, size_t rows_stride, int sm_count, cudaStream_t stream);
+cudaError_t launch_expert_combine(const void *rows, int type, size_t rows_stride, uint32_t tokens, uint32_t choices,
+                                  uint32_t width, const int32_t *position, const float *weights, void *out,
+                                  size_t out_stride, int sm_count, cudaStream_t stream);
+cudaError_t launch_expert_combine_backward(const void *rows, int type, size_t rows_stride, const void *grad,
+                                           size_t grad_stride, uint32_t tokens, uint32_t choices, uint32_t width,
+                                           const int32_t *position, const int32_t *offsets, uint32_t experts,
+                                           const float *weights, void *grad_rows, size_t grad_rows_stride,
+                                           float *grad_weights, int sm_count, cudaStream_t stream);
+
+}  // namespace qpucuda

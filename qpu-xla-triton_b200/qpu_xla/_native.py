@@ -175,6 +175,57 @@ class GgmlStats(Structure):
     ]
 
 
+class Fp8QuantizeDesc(Structure):
+    """``qpucuda_fp8_quantize_desc``."""
+
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_type", c_int),
+        ("x_stride", c_size_t),
+        ("rows", c_uint32),
+        ("cols", c_uint32),
+        ("gated", c_int),
+        ("row_source", c_void_p),
+        ("row_divisor", c_uint32),
+        ("source_rows", c_uint32),
+        ("q", c_void_p),
+        ("q_stride", c_size_t),
+        ("scales", c_void_p),
+        ("scale_row_stride", c_size_t),
+        ("scale_group_stride", c_size_t),
+    ]
+
+
+class Fp8GemmDesc(Structure):
+    """``qpucuda_fp8_gemm_desc``."""
+
+    _fields_ = [
+        ("a", c_void_p),
+        ("a_stride", c_size_t),
+        ("a_scales", c_void_p),
+        ("a_scale_row_stride", c_size_t),
+        ("a_scale_group_stride", c_size_t),
+        ("w", c_void_p),
+        ("w_stride", c_size_t),
+        ("w_scales", c_void_p),
+        ("bias", c_void_p),
+        ("rows", c_uint32),
+        ("n", c_uint32),
+        ("k", c_uint32),
+        ("experts", c_uint32),
+        ("offsets", c_void_p),
+        ("out", c_void_p),
+        ("out_type", c_int),
+        ("out_stride", c_size_t),
+        ("weights_settled", c_int),
+    ]
+
+
+# qpucuda_dtype
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+DTYPE_F16 = 2
+
 GGML_TYPE_F32 = 0
 GGML_TYPE_Q4_0 = 2
 
@@ -258,6 +309,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _P, c_size_t, c_uint32, _P, c_size_t, c_uint32, c_uint32, c_uint32],
     ),
     "qpucuda_q4_0_kernel_source_hash": (c_char_p, []),
+    # qpucuda_fp8.h
+    "qpucuda_fp8_quantize_rows": (_S, [_P, POINTER(Fp8QuantizeDesc)]),
+    "qpucuda_fp8_quantize_blocks": (_S, [_P, _P, c_int, c_size_t, c_uint32, c_uint32, c_uint32, _P, c_size_t, _P]),
+    "qpucuda_fp8_gemm": (_S, [_P, POINTER(Fp8GemmDesc)]),
+    # qpucuda_experts.h
+    "qpucuda_expert_sort_workspace": (c_size_t, [c_uint32, c_uint32, c_uint32]),
+    "qpucuda_expert_sort": (_S, [_P, _P, c_int, c_uint32, c_uint32, c_uint32, _P, _P, _P, _P, c_size_t]),
+    "qpucuda_expert_gather": (
+        _S,
+        [_P, _P, c_int, c_size_t, c_uint32, c_uint32, c_uint32, _P, _P, c_uint32, _P, c_size_t],
+    ),
+    "qpucuda_expert_combine": (_S, [_P, _P, c_int, c_size_t, c_uint32, c_uint32, c_uint32, _P, _P, _P, c_size_t]),
+    "qpucuda_expert_combine_backward": (
+        _S,
+        [_P, _P, c_int, c_size_t, _P, c_size_t, c_uint32, c_uint32, c_uint32, _P, _P, c_uint32, _P, _P, c_size_t, _P],
+    ),
     # qpucuda_ggml.h
     "qpucuda_ggml_supports_mul_mat": (
         c_int,
@@ -406,6 +473,8 @@ __all__ = [
     "Capabilities",
     "ContextConfig",
     "FailurePoint",
+    "Fp8GemmDesc",
+    "Fp8QuantizeDesc",
     "NativeContext",
     "Q40Execution",
     "Q40LinearDesc",

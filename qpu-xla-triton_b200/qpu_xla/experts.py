@@ -1,0 +1,263 @@
+"""Tokens sorted by expert and back, and an FFN of FP8 experts, on CUDA.
+
+Each token t makes ``choices`` choices of an expert; choice (t, j) has the flat
+index ``t * choices + j``. Rows are ordered by expert, then by flat index; an id
+outside ``[0, experts)`` drops the choice (a padding token). No counterpart in
+the reference. The order and the sums never depend on timing: the sort counts
+integers, a token's choices are added in their order, there are no atomics on
+floating-point values.
+
+The functions run on the current stream of their device. There is no autograd:
+each step's gradient is a function of its own (``gather_tokens_backward``,
+``combine_tokens_backward``).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Any, Self
+
+from qpu_xla import _native
+from qpu_xla.device import Device
+from qpu_xla.fp8 import (
+    MAX_EXPERTS,
+    PreparedFP8Experts,
+    QuantizedBlocksFP8,
+    check_matrix,
+    dtype_code,
+    launch,
+    require_cuda,
+)
+
+
+@dataclass(frozen=True, slots=True)
+class ExpertOrder:
+    """int32 CUDA tensors of one sort: ``offsets [experts + 1]`` (rows of expert e are ``offsets[e] ..
+    offsets[e + 1]``), ``source [tokens * choices]`` (the flat index at each row, -1 from
+    ``offsets[experts]`` on) and ``position [tokens, choices]`` (the row of each choice, -1 when
+    dropped)."""
+
+    offsets: Any
+    source: Any
+    position: Any
+
+    def __post_init__(self: Self) -> None:
+        import torch
+
+        fields = (self.offsets, self.source, self.position)
+        if any(t.dtype != torch.int32 or not t.is_contiguous() for t in fields):
+            raise ValueError("expert order tensors must be contiguous int32")
+        if self.offsets.dim() != 1 or self.source.dim() != 1 or self.position.dim() != 2 or self.offsets.shape[0] < 2:
+            raise ValueError("expert order needs offsets [experts + 1], source [rows] and position [tokens, choices]")
+        if self.source.shape[0] != self.position.numel() or self.position.shape[1] == 0:
+            raise ValueError("expert order needs one row per choice")
+        if any(t.device != self.offsets.device for t in fields):
+            raise ValueError("expert order tensors must be on one device")
+
+    @property
+    def experts(self: Self) -> int:
+        return int(self.offsets.shape[0]) - 1
+
+    @property
+    def tokens(self: Self) -> int:
+        return int(self.position.shape[0])
+
+    @property
+    def choices(self: Self) -> int:
+        return int(self.position.shape[1])
+
+    @property
+    def rows(self: Self) -> int:
+        return int(self.source.shape[0])
+
+    def check(self: Self, torch_device: Any, *, tokens: int | None = None) -> None:
+        if self.offsets.device != torch_device:
+            raise ValueError(f"expert order must be on {torch_device}, the device it is used with")
+        if tokens is not None and tokens != self.tokens:
+            raise ValueError(f"expert order is of {self.tokens} tokens, not {tokens}")
+
+
+def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
+    """Sort the choices ``[tokens, choices]`` (int32 or int64 expert ids) by expert, stably."""
+    import torch
+
+    torch_device = require_cuda(device, "sort_tokens")
+    if expert_ids.dtype not in (torch.int32, torch.int64) or expert_ids.dim() != 2 or expert_ids.shape[1] == 0:
+        raise ValueError("sort_tokens requires int32 or int64 expert ids [tokens, choices]")
+    if expert_ids.device != torch_device:
+        raise ValueError(f"sort_tokens expert ids must be on {torch_device}")
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"sort_tokens takes 1 to {MAX_EXPERTS} experts")
+    if expert_ids.numel() >= 2**31:
+        raise ValueError("sort_tokens takes fewer than 2**31 choices")
+    ids = expert_ids.contiguous()
+    tokens, choices = (int(extent) for extent in ids.shape)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=torch_device)
+    source = torch.empty(tokens * choices, dtype=torch.int32, device=torch_device)
+    position = torch.empty((tokens, choices), dtype=torch.int32, device=torch_device)
+    needed = int(_native.load().qpucuda_expert_sort_workspace(tokens, choices, experts))
+    workspace = torch.empty(needed, dtype=torch.uint8, device=torch_device) if needed else None
+    launch(
+        device, "qpucuda_expert_sort", ids.data_ptr(), int(ids.dtype == torch.int64), tokens, choices, experts, offsets.data_ptr(),
+        source.data_ptr(), position.data_ptr(), None if workspace is None else workspace.data_ptr(), needed,
+    )
+    return ExpertOrder(offsets, source, position)
+
+
+def _destination(out: Any, shape: tuple[int, int], dtype: Any, torch_device: Any, what: str) -> tuple[Any, int]:
+    import torch
+
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=torch_device), shape[1]
+    if out.dtype != dtype:
+        raise ValueError(f"{what} must have the type of its source")
+    return out, check_matrix(out, torch_device, what, shape)
+
+
+def _refuse_overlap(written: Any, read: Any, what: str) -> None:
+    """The kernels read and write in no particular order."""
+    def span(t: Any) -> tuple[int, int]:
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+
+    if written.numel() and read.numel():
+        (a, a_end), (b, b_end) = span(written), span(read)
+        if a < b_end and b < a_end:
+            raise ValueError(f"{what} must not overlap its source")
+
+
+def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = None) -> Any:
+    """Tokens ``[T, H]`` (float32, bfloat16 or float16) copied into expert order, ``[T * choices, H]``:
+    row ``order.position[t, j]`` is token t. Rows from ``offsets[experts]`` on become zero."""
+    torch_device = require_cuda(device, "gather_tokens")
+    code = dtype_code(source.dtype, "gather_tokens source")
+    stride = check_matrix(source, torch_device, "gather_tokens source", (order.tokens, None))
+    order.check(torch_device)
+    width = int(source.shape[1])
+    out, out_stride = _destination(out, (order.rows, width), source.dtype, torch_device, "gather_tokens out")
+    _refuse_overlap(out, source, "gather_tokens out")
+    if out.numel():
+        launch(
+            device, "qpucuda_expert_gather", source.data_ptr(), code, stride, order.tokens, order.choices, width,
+            order.position.data_ptr(), order.offsets.data_ptr(), order.experts, out.data_ptr(), out_stride,
+        )
+    return out
+
+
+def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: Any, name: str) -> Any:
+    torch_device = require_cuda(device, name)
+    code = dtype_code(rows.dtype, f"{name} rows")
+    stride = check_matrix(rows, torch_device, f"{name} rows", (order.rows, None))
+    order.check(torch_device)
+    width = int(rows.shape[1])
+    out, out_stride = _destination(out, (order.tokens, width), rows.dtype, torch_device, f"{name} out")
+    _refuse_overlap(out, rows, f"{name} out")
+    if out.numel():
+        launch(
+            device, "qpucuda_expert_combine", rows.data_ptr(), code, stride, order.tokens, order.choices, width,
+            order.position.data_ptr(), None if weights is None else weights.data_ptr(), out.data_ptr(), out_stride,
+        )
+    return out
+
+
+def _check_weights(weights: Any, order: ExpertOrder, torch_device: Any, name: str) -> None:
+    import torch
+
+    if weights.dtype != torch.float32 or tuple(weights.shape) != (order.tokens, order.choices) or not weights.is_contiguous():
+        raise ValueError(f"{name} requires contiguous float32 weights [tokens, choices]")
+    if weights.device != torch_device:
+        raise ValueError(f"{name} weights must be on {torch_device}")
+
+
+def gather_tokens_backward(device: Device, grad_rows: Any, order: ExpertOrder, out: Any = None) -> Any:
+    """The tokens' gradient ``[T, H]`` from the sorted rows' ``[T * choices, H]``: the sum over a
+    token's choices in fp32, rounded once. Dropped choices add nothing."""
+    return _combine(device, grad_rows, None, order, out, "gather_tokens_backward")
+
+
+def combine_tokens(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: Any = None) -> Any:
+    """Sorted rows ``[T * choices, H]`` back to tokens: ``out[t] = sum_j weights[t, j] *
+    rows[position[t, j]]`` in fp32, in the order of j, rounded once. A dropped choice adds nothing,
+    whatever its weight."""
+    _check_weights(weights, order, require_cuda(device, "combine_tokens"), "combine_tokens")
+    return _combine(device, rows, weights, order, out, "combine_tokens")
+
+
+def combine_tokens_backward(device: Device, rows: Any, weights: Any, grad: Any, order: ExpertOrder) -> tuple[Any, Any]:
+    """The gradients of :func:`combine_tokens` from that of its result, ``grad [T, H]``: of the rows
+    (``weights[t, j] * grad[t]`` at ``position[t, j]``, zero where no choice is) and of the weights
+    (``<rows[position[t, j]], grad[t]>`` in fp32, zero where dropped)."""
+    import torch
+
+    name = "combine_tokens_backward"
+    torch_device = require_cuda(device, name)
+    code = dtype_code(rows.dtype, f"{name} rows")
+    if grad.dtype != rows.dtype:
+        raise ValueError(f"{name} grad must have the type of the rows")
+    stride = check_matrix(rows, torch_device, f"{name} rows", (order.rows, None))
+    width = int(rows.shape[1])
+    grad_stride = check_matrix(grad, torch_device, f"{name} grad", (order.tokens, width))
+    order.check(torch_device)
+    _check_weights(weights, order, torch_device, name)
+    grad_rows = torch.empty((order.rows, width), dtype=rows.dtype, device=torch_device)
+    grad_weights = torch.empty((order.tokens, order.choices), dtype=torch.float32, device=torch_device)
+    if grad_rows.numel():
+        launch(
+            device, "qpucuda_expert_combine_backward", rows.data_ptr(), code, stride, grad.data_ptr(), grad_stride, order.tokens,
+            order.choices, width, order.position.data_ptr(), order.offsets.data_ptr(), order.experts, weights.data_ptr(),
+            grad_rows.data_ptr(), width, grad_weights.data_ptr(),
+        )
+    else:
+        grad_weights.zero_()
+    return grad_rows, grad_weights
+
+
+class FP8ExpertsFFN:
+    """A layer of experts: ``sum_j w[t, j] down_e(silu(gate_e(x_t)) * up_e(x_t))``, e = ids[t, j].
+
+    ``gate_up`` ``[E, 2 I, H]`` stacks each expert's gate rows on its up rows, ``down`` is
+    ``[E, H_out, I]``; both block-scaled e4m3. Per call: one sort, one quantization of the tokens in
+    expert order, the gate/up product (kept in fp32), one gated quantization, the down product, the
+    weighted sum.
+    """
+
+    def __init__(self: Self, device: Device, gate_up: QuantizedBlocksFP8, down: QuantizedBlocksFP8) -> None:
+        if len(gate_up.shape) != 3 or len(down.shape) != 3 or gate_up.shape[0] != down.shape[0] or gate_up.shape[1] != 2 * down.shape[2]:
+            raise ValueError("FP8ExpertsFFN requires gate_up [E, 2 * inner, inputs] and down [E, outputs, inner]")
+        self.device = device
+        self.gate_up = PreparedFP8Experts(device, gate_up)
+        self.down = PreparedFP8Experts(device, down, gated=True)
+
+    @property
+    def experts(self: Self) -> int:
+        return self.gate_up.experts
+
+    def forward(self: Self, source: Any, expert_ids: Any, weights: Any) -> Any:
+        """Tokens ``[T, H]``, their expert ids ``[T, choices]`` and float32 weights, to ``[T, H_out]``
+        of the source's type."""
+        import torch
+
+        order = sort_tokens(self.device, expert_ids, self.experts)
+        hidden = self.gate_up.forward_tokens(source, order, dtype=torch.float32)
+        rows = self.down.forward(hidden, order.offsets, dtype=source.dtype)
+        return combine_tokens(self.device, rows, weights, order)
+
+    def close(self: Self) -> None:
+        self.gate_up.close()
+        self.down.close()
+
+    def __enter__(self: Self) -> Self:
+        return self
+
+    def __exit__(self: Self, exc_type: object, exc_value: object, traceback: object) -> None:
+        self.close()
+
+
+__all__ = [
+    "ExpertOrder",
+    "FP8ExpertsFFN",
+    "combine_tokens",
+    "combine_tokens_backward",
+    "gather_tokens",
+    "gather_tokens_backward",
+    "sort_tokens",
+]

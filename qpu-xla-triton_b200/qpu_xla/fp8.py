@@ -1,0 +1,452 @@
+"""Block-scaled FP8 (e4m3) linear plans on CUDA.
+
+The W8A8 linear of :mod:`qpu_xla.quantization` for weights published as e4m3
+values with one fp32 scale per 128 x 128 block; no counterpart in the reference.
+Activation rows are quantized on the fly with one scale per 128 columns::
+
+    s = max(RN(max|x| / 448), 2**-60)      q = e4m3(RN(x / s)), round to nearest even
+    y[m, n] = sum_k (qx[m, k] sx[m, k // 128]) (qw[n, k] sw[n // 128, k // 128]) (+ bias[n])
+
+summed in fp32 and rounded once to the output's type. A group of 128 columns
+that holds a NaN or an infinity dequantizes to NaN, and so do that row's outputs.
+
+Everything here runs on the current stream of the plan's device, allocates its
+scratch from PyTorch per call (so calls on several streams, and several captured
+CUDA graphs, share no workspace) and has no CPU path. There is no autograd:
+results carry no gradient.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Iterable
+from dataclasses import dataclass
+from typing import Any, Self
+
+import numpy as np
+
+from qpu_xla import _native
+from qpu_xla.device import Device
+from qpu_xla.errors import DependencyError
+from qpu_xla.kernel import Kernel
+from qpu_xla.memory import AccessMode, Tensor
+from qpu_xla.queue import Event, Queue
+
+FP8_GROUP = 128
+MAX_EXPERTS = 1024
+
+
+def _dtype_codes() -> dict[Any, int]:
+    import torch
+
+    return {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
+
+
+def dtype_code(dtype: Any, what: str) -> int:
+    """``qpucuda_dtype`` of an activation or output type."""
+    code = _dtype_codes().get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16")
+    return code
+
+
+def groups_of(size: int) -> int:
+    return (size + FP8_GROUP - 1) // FP8_GROUP
+
+
+def require_cuda(device: Device, what: str) -> Any:
+    """The torch device behind a CUDA ``Device``."""
+    if not device.is_cuda:
+        raise ValueError(f"{what} requires the CUDA backend (this build has no CPU path)")
+    return device.backend.torch_device  # type: ignore[attr-defined]
+
+
+def check_matrix(tensor: Any, torch_device: Any, what: str, shape: tuple[int | None, int | None] = (None, None)) -> int:
+    """A rank-2 tensor on ``torch_device`` with unit inner stride and the given extents; its row stride."""
+    if tensor.dim() != 2 or any(want is not None and have != want for have, want in zip(tensor.shape, shape)):
+        raise ValueError(f"{what} must be rank-2 {list(shape)}, not {list(tensor.shape)}")
+    if tensor.device != torch_device:
+        raise ValueError(f"{what} must be on {torch_device}, the device it is used with")
+    if tensor.shape[1] > 1 and tensor.stride(1) != 1:
+        raise ValueError(f"{what} must be row-major (unit inner stride)")
+    if tensor.shape[0] <= 1:
+        return int(max(tensor.shape[1], 1))
+    if tensor.stride(0) < tensor.shape[1]:
+        raise ValueError(f"{what} must not have overlapping rows")
+    return int(tensor.stride(0))
+
+
+def launch(device: Device, name: str, *args: Any, stream: Any = None) -> None:
+    """Call one libqpucuda entry point on ``stream`` (default: the device's current stream)."""
+    import torch
+
+    backend = device.backend
+    stream = torch.cuda.current_stream(backend.torch_device) if stream is None else stream  # type: ignore[attr-defined]
+    backend.launch(stream, lambda native: native.check(getattr(native.library, name)(native.handle, *args), name))  # type: ignore[attr-defined]
+
+
+@dataclass(frozen=True, slots=True)
+class QuantizedRowsFP8:
+    """e4m3 rows ``[M, K]`` and their fp32 scales ``[M, ceil(K / 128)]`` (any strides)."""
+
+    values: Any
+    scales: Any
+
+    def __post_init__(self: Self) -> None:
+        import torch
+
+        if self.values.dim() != 2 or self.values.dtype != torch.float8_e4m3fn:
+            raise ValueError("quantized rows must be rank-2 float8_e4m3fn")
+        if tuple(self.scales.shape) != (self.values.shape[0], groups_of(self.values.shape[1])) or self.scales.dtype != torch.float32:
+            raise ValueError("quantized rows need one float32 scale per row and 128 columns")
+        if self.scales.device != self.values.device:
+            raise ValueError("quantized rows and their scales must be on one device")
+
+    @property
+    def shape(self: Self) -> tuple[int, int]:
+        return (int(self.values.shape[0]), int(self.values.shape[1]))
+
+    def dequantize(self: Self) -> Any:
+        """fp32 reconstruction ``[M, K]``."""
+        spread = self.scales.repeat_interleave(FP8_GROUP, dim=1)[:, : self.values.shape[1]]
+        return self.values.float() * spread
+
+
+@dataclass(frozen=True, slots=True)
+class QuantizedBlocksFP8:
+    """e4m3 weights ``[N, K]`` with fp32 scales ``[ceil(N / 128), ceil(K / 128)]``, or one such matrix
+    per expert (``[E, N, K]`` and ``[E, ceil(N / 128), ceil(K / 128)]``)."""
+
+    values: Any
+    scales: Any
+
+    def __post_init__(self: Self) -> None:
+        import torch
+
+        if self.values.dim() not in (2, 3) or self.values.dtype != torch.float8_e4m3fn or 0 in self.values.shape:
+            raise ValueError("quantized weights must be non-empty rank-2 or rank-3 float8_e4m3fn")
+        *batch, rows, cols = self.values.shape
+        if tuple(self.scales.shape) != (*batch, groups_of(rows), groups_of(cols)) or self.scales.dtype != torch.float32:
+            raise ValueError("quantized weights need one float32 scale per 128 x 128 block")
+        if self.scales.device != self.values.device:
+            raise ValueError("quantized weights and their scales must be on one device")
+
+    @property
+    def shape(self: Self) -> tuple[int, ...]:
+        return tuple(int(extent) for extent in self.values.shape)
+
+    def dequantize(self: Self) -> Any:
+        """fp32 reconstruction, shaped as the values."""
+        rows, cols = self.values.shape[-2:]
+        spread = self.scales.repeat_interleave(FP8_GROUP, dim=-2)[..., :rows, :].repeat_interleave(FP8_GROUP, dim=-1)
+        return self.values.float() * spread[..., :cols]
+
+
+def quantize_blocks_fp8(device: Device, weight: Any) -> QuantizedBlocksFP8:
+    """Quantize weights ``[N, K]`` or ``[E, N, K]`` (float32, bfloat16 or float16 CUDA tensor) per 128 x 128 block."""
+    import torch
+
+    torch_device = require_cuda(device, "quantize_blocks_fp8")
+    code = dtype_code(weight.dtype, "quantize_blocks_fp8 weight")
+    if weight.dim() not in (2, 3) or 0 in weight.shape:
+        raise ValueError("quantize_blocks_fp8 requires a non-empty rank-2 or rank-3 weight")
+    if weight.device != torch_device:
+        raise ValueError(f"quantize_blocks_fp8 weight must be on {torch_device}")
+    weight = weight.contiguous()
+    *batch, rows, cols = weight.shape
+    values = torch.empty(weight.shape, dtype=torch.float8_e4m3fn, device=torch_device)
+    scales = torch.empty((*batch, groups_of(rows), groups_of(cols)), dtype=torch.float32, device=torch_device)
+    launch(
+        device, "qpucuda_fp8_quantize_blocks", weight.data_ptr(), code, cols, batch[0] if batch else 1, rows, cols,
+        values.data_ptr(), cols, scales.data_ptr(),
+    )
+    return QuantizedBlocksFP8(values, scales)
+
+
+def _quantize_desc(
+    source: Any, stride: int, cols: int, gated: bool, rows: int, q: int, q_stride: int, scales: int, scale_strides: tuple[int, int],
+    row_source: Any = None, row_divisor: int = 1,
+) -> Any:
+    return _native.Fp8QuantizeDesc(
+        source.data_ptr(), dtype_code(source.dtype, "quantizer source"), stride, rows, cols, int(gated),
+        None if row_source is None else row_source.data_ptr(), row_divisor, source.shape[0], q, q_stride, scales, *scale_strides,
+    )
+
+
+def _columns(source: Any, gated: bool, what: str) -> int:
+    if source.dim() != 2 or source.shape[1] == 0 or (gated and source.shape[1] % 2):
+        raise ValueError(f"{what} must be rank-2 [rows, {'2 * ' if gated else ''}columns]")
+    return int(source.shape[1]) // (2 if gated else 1)
+
+
+def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> QuantizedRowsFP8:
+    """Quantize rows ``[M, K]`` (float32, bfloat16 or float16) with one scale per 128 columns.
+
+    ``gated``: the source is ``[M, 2 K]``, gate then up, and ``silu(gate) * up`` is quantized,
+    computed in fp32. The values are a view of rows padded to 16 bytes.
+    """
+    import torch
+
+    torch_device = require_cuda(device, "quantize_rows_fp8")
+    dtype_code(source.dtype, "quantize_rows_fp8 source")
+    cols = _columns(source, gated, "quantize_rows_fp8 source")
+    stride = check_matrix(source, torch_device, "quantize_rows_fp8 source")
+    rows = int(source.shape[0])
+    q_stride = (cols + 15) // 16 * 16
+    values = torch.empty((rows, q_stride), dtype=torch.float8_e4m3fn, device=torch_device)
+    scales = torch.empty((rows, groups_of(cols)), dtype=torch.float32, device=torch_device)
+    if rows:
+        desc = _quantize_desc(source, stride, cols, gated, rows, values.data_ptr(), q_stride, scales.data_ptr(), (groups_of(cols), 1))
+        launch(device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
+    return QuantizedRowsFP8(values[:, :cols], scales)
+
+
+class _PreparedFP8:
+    """A weight (one matrix, or one per expert) resident on one GPU in the layout the product reads:
+    e4m3 rows padded to 16 bytes, block scales, optional bias. The plan owns copies; calls only
+    read them, so any number may be in flight. Keep the plan open until their work has finished
+    (``close`` waits for the device)."""
+
+    _name = "prepared FP8 linear"
+
+    def __init__(self: Self, device: Device, weight: QuantizedBlocksFP8, bias: Any, gated: bool) -> None:
+        import torch
+
+        self._torch_device = require_cuda(device, type(self).__name__)
+        self.device = device
+        self.gated = bool(gated)
+        *batch, self.output_count, self.input_count = weight.shape
+        self.experts = batch[0] if batch else 0
+        padded = (self.input_count + 15) // 16 * 16
+        self._values = torch.zeros((*batch, self.output_count, padded), dtype=torch.uint8, device=self._torch_device)
+        self._values[..., : self.input_count].copy_(weight.values.view(torch.uint8))
+        self._scales = weight.scales.to(self._torch_device).clone(memory_format=torch.contiguous_format)
+        self._bias = None
+        if bias is not None:
+            bias = torch.as_tensor(bias)
+            if tuple(bias.shape) != (self.output_count,):
+                raise ValueError("bias must have one fp32 value per output feature")
+            self._bias = bias.to(self._torch_device, torch.float32).clone(memory_format=torch.contiguous_format)
+        torch.cuda.current_stream(self._torch_device).synchronize()
+        self._closed = False
+
+    def __enter__(self: Self) -> Self:
+        self._require_open()
+        return self
+
+    def __exit__(self: Self, exc_type: object, exc_value: object, traceback: object) -> None:
+        self.close()
+
+    def _require_open(self: Self) -> None:
+        if self._closed:
+            raise RuntimeError(f"{self._name} plan is closed")
+
+    def close(self: Self) -> None:
+        """Wait for the device and release the weight."""
+        if self._closed:
+            return
+        import torch
+
+        torch.cuda.synchronize(self._torch_device)
+        self._values = self._scales = self._bias = None
+        self._closed = True
+
+    @property
+    def resident_bytes(self: Self) -> int:
+        self._require_open()
+        return sum(t.numel() * t.element_size() for t in (self._values, self._scales, self._bias) if t is not None)
+
+    def _output(self: Self, rows: int, out: Any, dtype: Any, default: Any) -> tuple[Any, int]:
+        import torch
+
+        if out is None:
+            dtype = default if dtype is None else dtype
+            dtype_code(dtype, f"{self._name} output")
+            return torch.empty((rows, self.output_count), dtype=dtype, device=self._torch_device), self.output_count
+        if dtype is not None and out.dtype != dtype:
+            raise ValueError(f"{self._name} out and dtype differ")
+        dtype_code(out.dtype, f"{self._name} output")
+        return out, check_matrix(out, self._torch_device, f"{self._name} output", (rows, self.output_count))
+
+    def _gemm(
+        self: Self, a: int, a_stride: int, a_scales: int, scale_strides: tuple[int, int], rows: int, out_address: int, out_code: int,
+        out_stride: int, offsets: Any = None, settled: bool = False, stream: Any = None,
+    ) -> None:
+        desc = _native.Fp8GemmDesc(
+            a, a_stride, a_scales, *scale_strides, self._values.data_ptr(), self._values.stride(-2), self._scales.data_ptr(),
+            None if self._bias is None else self._bias.data_ptr(), rows, self.output_count, self.input_count, self.experts,
+            None if offsets is None else offsets.data_ptr(), out_address, out_code, out_stride, int(settled),
+        )
+        launch(self.device, "qpucuda_fp8_gemm", ctypes.byref(desc), stream=stream)
+
+    def _scratch(self: Self, rows: int) -> tuple[Any, int, int, int]:
+        """One allocation for the quantized rows and, behind them, their scales (group-major: a warp
+        of the product reads the scales of neighbouring rows)."""
+        import torch
+
+        stride = (self.input_count + 15) // 16 * 16
+        scratch = torch.empty(rows * stride + 4 * rows * groups_of(self.input_count), dtype=torch.uint8, device=self._torch_device)
+        return scratch, scratch.data_ptr(), stride, scratch.data_ptr() + rows * stride
+
+    def _quantize_and_multiply(
+        self: Self, source: Any, stride: int, rows: int, out: Any, out_stride: int, offsets: Any = None, row_source: Any = None, row_divisor: int = 1
+    ) -> None:
+        scratch, values, q_stride, scales = self._scratch(rows)
+        desc = _quantize_desc(source, stride, self.input_count, self.gated, rows, values, q_stride, scales, (1, rows), row_source, row_divisor)
+        launch(self.device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
+        # The weight and the offsets are older than the quantizer's launch: the product reads them early.
+        self._gemm(
+            values, q_stride, scales, (1, rows), rows, out.data_ptr(), dtype_code(out.dtype, "output"), out_stride,
+            offsets=offsets, settled=True,
+        )
+        del scratch
+
+    def _check_source(self: Self, source: Any) -> int:
+        dtype_code(source.dtype, f"{self._name} source")
+        width = self.input_count * (2 if self.gated else 1)
+        return check_matrix(source, self._torch_device, f"{self._name} source", (None, width))
+
+    def _check_rows(self: Self, rows: QuantizedRowsFP8) -> tuple[int, int, tuple[int, int]]:
+        values = rows.values
+        count = int(values.shape[0])
+        stride = check_matrix(values, self._torch_device, f"{self._name} quantized rows", (None, self.input_count))
+        if count <= 1:
+            stride = (self.input_count + 15) // 16 * 16
+        if stride % 16 or values.data_ptr() % 16:
+            raise ValueError(f"{self._name} quantized rows must start on 16-byte boundaries")
+        if min(rows.scales.stride()) < 0:
+            raise ValueError(f"{self._name} scales must not have negative strides")
+        return count, stride, (int(rows.scales.stride(0)), int(rows.scales.stride(1)))
+
+
+class PreparedFP8Linear(_PreparedFP8):
+    """``y = x W^T (+ bias)`` with a resident block-scaled e4m3 weight ``[N, K]``.
+
+    ``gated``: sources are ``[M, 2 K]``, gate then up (the output of one merged gate/up plan), and
+    ``silu(gate) * up`` is what is quantized: an FFN's down projection.
+    """
+
+    def __init__(self: Self, device: Device, weight: QuantizedBlocksFP8, *, bias: Any = None, gated: bool = False) -> None:
+        if len(weight.shape) != 2:
+            raise ValueError("PreparedFP8Linear requires a rank-2 weight; PreparedFP8Experts takes one per expert")
+        super().__init__(device, weight, bias, gated)
+
+    def forward(self: Self, source: Any, out: Any = None, *, dtype: Any = None) -> Any:
+        """Rows ``[M, K]`` (float32, bfloat16 or float16) to ``[M, N]`` of ``dtype`` (default: the
+        source's type, or ``out``'s)."""
+        self._require_open()
+        stride = self._check_source(source)
+        rows = int(source.shape[0])
+        out, out_stride = self._output(rows, out, dtype, source.dtype)
+        if rows:
+            self._quantize_and_multiply(source, stride, rows, out, out_stride)
+        return out
+
+    def forward_quantized(self: Self, rows: QuantizedRowsFP8, out: Any = None, *, dtype: Any = None) -> Any:
+        """The product alone, over rows quantized before (:func:`quantize_rows_fp8`); ``dtype``
+        defaults to float32."""
+        import torch
+
+        self._require_open()
+        count, stride, scale_strides = self._check_rows(rows)
+        out, out_stride = self._output(count, out, dtype, torch.float32)
+        if count:
+            self._gemm(
+                rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(),
+                dtype_code(out.dtype, "output"), out_stride,
+            )
+        return out
+
+    def execute(self: Self, destination: Tensor, source: Tensor, *, queue: Queue, wait_for: Iterable[Event] = ()) -> Event:
+        """The same on a queue, float32 tensors of the plan's device (as ``PreparedW8A8Linear.execute``)."""
+        import torch
+
+        self._require_open()
+        if queue.device is not self.device or source.buffer.device is not self.device or destination.buffer.device is not self.device:
+            raise DependencyError("prepared FP8 linear queue and tensors must belong to the plan device")
+        if source.dtype != np.dtype(np.float32) or destination.dtype != np.dtype(np.float32):
+            raise ValueError("prepared FP8 linear requires float32 source and destination")
+        width = self.input_count * (2 if self.gated else 1)
+        if len(source.shape) != 2 or source.shape[1] != width or destination.shape != (source.shape[0], self.output_count):
+            raise ValueError("prepared FP8 linear source and destination shapes do not align")
+        if source.strides[1] != 4 or destination.strides[1] != 4:
+            raise ValueError("prepared FP8 linear requires unit inner strides")
+        rows = int(source.shape[0])
+
+        def executor(backend: Any, args: tuple[Any, ...], grid: tuple[int, int, int], stream: Any) -> None:
+            with torch.cuda.stream(stream):
+                scratch, values, q_stride, scales = self._scratch(rows)
+                desc = _native.Fp8QuantizeDesc(
+                    source.address, _native.DTYPE_F32, source.row_stride_elements, rows, self.input_count, int(self.gated), None, 1, rows,
+                    values, q_stride, scales, 1, rows,
+                )
+                launch(self.device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc), stream=stream)
+                self._gemm(
+                    values, q_stride, scales, (1, rows), rows, destination.address, _native.DTYPE_F32, destination.row_stride_elements,
+                    settled=True, stream=stream,
+                )
+                del scratch
+
+        return queue.submit(
+            Kernel("cuda.fp8_linear", executor), (), wait_for=wait_for,
+            buffers=(source.access(AccessMode.READ), destination.access(AccessMode.WRITE)),
+        )
+
+
+class PreparedFP8Experts(_PreparedFP8):
+    """One resident block-scaled e4m3 weight per expert, ``[E, N, K]``: rows sorted by expert (see
+    :func:`qpu_xla.experts.sort_tokens`) meet their expert's matrix in one launch."""
+
+    _name = "prepared FP8 experts"
+
+    def __init__(self: Self, device: Device, weight: QuantizedBlocksFP8, *, gated: bool = False) -> None:
+        if len(weight.shape) != 3:
+            raise ValueError("PreparedFP8Experts requires a rank-3 weight [experts, outputs, inputs]")
+        if weight.shape[0] > MAX_EXPERTS:
+            raise ValueError(f"PreparedFP8Experts takes at most {MAX_EXPERTS} experts")
+        super().__init__(device, weight, None, gated)
+
+    def _check_offsets(self: Self, offsets: Any) -> None:
+        import torch
+
+        if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.experts + 1,) or not offsets.is_contiguous():
+            raise ValueError("prepared FP8 experts need contiguous int32 offsets [experts + 1]")
+        if offsets.device != self._torch_device:
+            raise ValueError(f"prepared FP8 experts offsets must be on {self._torch_device}")
+
+    def forward(self: Self, source: Any, offsets: Any, out: Any = None, *, dtype: Any = None) -> Any:
+        """Rows ``[R, K]``, those of expert e at ``offsets[e] .. offsets[e + 1]`` (ascending int32 on
+        the GPU, clamped to ``[0, R]``), to ``[R, N]``. Rows from ``offsets[E]`` on become zero."""
+        self._require_open()
+        stride = self._check_source(source)
+        self._check_offsets(offsets)
+        rows = int(source.shape[0])
+        out, out_stride = self._output(rows, out, dtype, source.dtype)
+        if rows:
+            self._quantize_and_multiply(source, stride, rows, out, out_stride, offsets)
+        return out
+
+    def forward_tokens(self: Self, tokens: Any, order: Any, out: Any = None, *, dtype: Any = None) -> Any:
+        """:meth:`forward` of the tokens ``[T, K]`` in expert order, without the sorted copy: row r is
+        quantized straight from token ``order.source[r] // choices``. ``[T * choices, N]``."""
+        self._require_open()
+        stride = self._check_source(tokens)
+        self._check_offsets(order.offsets)
+        order.check(self._torch_device, tokens=int(tokens.shape[0]))
+        rows = int(order.source.shape[0])
+        out, out_stride = self._output(rows, out, dtype, tokens.dtype)
+        if rows:
+            self._quantize_and_multiply(tokens, stride, rows, out, out_stride, order.offsets, order.source, order.choices)
+        return out
+
+
+__all__ = [
+    "FP8_GROUP",
+    "MAX_EXPERTS",
+    "PreparedFP8Experts",
+    "PreparedFP8Linear",
+    "QuantizedBlocksFP8",
+    "QuantizedRowsFP8",
+    "quantize_blocks_fp8",
+    "quantize_rows_fp8",
+]

@@ -1,0 +1,100 @@
+"""Host-side rules of the FP8 plans and the expert routing: argument checks that need no GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from qpu_xla import Device, _native
+from qpu_xla.experts import ExpertOrder, FP8ExpertsFFN, gather_tokens, sort_tokens
+from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, QuantizedBlocksFP8, QuantizedRowsFP8, quantize_blocks_fp8, quantize_rows_fp8
+
+E4M3 = torch.float8_e4m3fn
+
+
+def weight(*shape: int) -> QuantizedBlocksFP8:
+    *batch, n, k = shape
+    return QuantizedBlocksFP8(torch.zeros(shape, dtype=E4M3), torch.ones((*batch, -(-n // 128), -(-k // 128))))
+
+
+def test_quantized_containers_check_their_shapes_and_types() -> None:
+    assert weight(130, 300).shape == (130, 300)
+    assert weight(3, 130, 300).dequantize().shape == (3, 130, 300)
+    for values, scales in (
+        (torch.zeros((130, 300), dtype=E4M3), torch.ones((1, 3))),
+        (torch.zeros((130, 300), dtype=E4M3), torch.ones((2, 3), dtype=torch.float64)),
+        (torch.zeros((130, 300), dtype=torch.uint8), torch.ones((2, 3))),
+        (torch.zeros((300,), dtype=E4M3), torch.ones((3,))),
+        (torch.zeros((2, 130, 300), dtype=E4M3), torch.ones((2, 3))),
+        (torch.zeros((0, 300), dtype=E4M3), torch.ones((0, 3))),
+    ):
+        with pytest.raises(ValueError):
+            QuantizedBlocksFP8(values, scales)
+    with pytest.raises(ValueError, match="one float32 scale"):
+        QuantizedRowsFP8(torch.zeros((2, 300), dtype=E4M3), torch.ones((2, 2)))
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        QuantizedRowsFP8(torch.zeros((2, 300)), torch.ones((2, 3)))
+
+
+def test_dequantization_spreads_each_scale_over_its_group() -> None:
+    rows = QuantizedRowsFP8(torch.ones((2, 130)).to(E4M3), torch.tensor([[2.0, 3.0], [4.0, 5.0]]))
+    assert rows.dequantize()[0, 127:130].tolist() == [2.0, 3.0, 3.0]
+    blocks = QuantizedBlocksFP8(torch.ones((129, 129)).to(E4M3), torch.tensor([[2.0, 3.0], [4.0, 5.0]]))
+    assert blocks.dequantize()[127:129, 127:129].tolist() == [[2.0, 3.0], [4.0, 5.0]]
+
+
+def test_calls_need_the_cuda_backend() -> None:
+    with Device.fake() as device:
+        for call in (
+            lambda: quantize_rows_fp8(device, torch.zeros((2, 8))),
+            lambda: quantize_blocks_fp8(device, torch.zeros((2, 8))),
+            lambda: PreparedFP8Linear(device, weight(8, 8)),
+            lambda: PreparedFP8Experts(device, weight(2, 8, 8)),
+            lambda: sort_tokens(device, torch.zeros((2, 2), dtype=torch.int32), 2),
+        ):
+            with pytest.raises(ValueError, match="CUDA backend"):
+                call()
+
+
+def test_plans_check_the_weight_rank_before_the_device() -> None:
+    with Device.fake() as device:
+        with pytest.raises(ValueError, match="rank-2"):
+            PreparedFP8Linear(device, weight(2, 8, 8))
+        with pytest.raises(ValueError, match="rank-3"):
+            PreparedFP8Experts(device, weight(8, 8))
+        with pytest.raises(ValueError, match="at most 1024"):
+            PreparedFP8Experts(device, weight(1025, 1, 1))
+        with pytest.raises(ValueError, match="gate_up"):
+            FP8ExpertsFFN(device, weight(2, 24, 8), weight(2, 8, 10))
+
+
+def test_expert_order_checks_its_tensors() -> None:
+    offsets, source, position = (torch.zeros(s, dtype=torch.int32) for s in (3, 8, (4, 2)))
+    order = ExpertOrder(offsets, source, position)
+    assert (order.experts, order.tokens, order.choices, order.rows) == (2, 4, 2, 8)
+    for fields in ((offsets.long(), source, position), (offsets, source[:7], position), (offsets[:1], source, position), (offsets, source, position.t())):
+        with pytest.raises(ValueError):
+            ExpertOrder(*fields)
+    with pytest.raises(ValueError, match="CUDA backend"), Device.fake() as device:
+        gather_tokens(device, torch.zeros((4, 3)), order)
+
+
+def test_null_arguments_are_rejected_without_a_device() -> None:
+    library = _native.load()
+    assert library.qpucuda_fp8_quantize_rows(None, ctypes.byref(_native.Fp8QuantizeDesc())) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_fp8_gemm(None, ctypes.byref(_native.Fp8GemmDesc())) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_fp8_quantize_blocks(None, None, 0, 0, 0, 0, 0, None, 0, None) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_sort(None, None, 0, 0, 0, 0, None, None, None, None, 0) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_gather(None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_combine(None, None, 0, 0, 0, 0, 0, None, None, None, 0) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_combine_backward(None, None, 0, 0, None, 0, 0, 0, 0, None, None, 0, None, None, 0, None) == _native.Status.INVALID_ARGUMENT
+
+
+def test_sort_workspace_is_only_needed_past_one_chunk() -> None:
+    size = _native.load().qpucuda_expert_sort_workspace
+    assert size(1, 1, 1) == 0 and size(512, 8, 64) == 0
+    assert size(4096, 8, 64) > 0 and size(4096, 8, 64) % (4 * 64) == 0
+    assert size(0, 8, 64) == 0 and size(8, 0, 64) == 0 and size(8, 8, 1025) == 0
+    assert size(2**31, 2, 4) == 0
