@@ -440,6 +440,373 @@ cudaError_t launch_narrow_rows(int nt, const CUtensorMap &map_w, const CUtensorM
     }
 }
 
+// ---- the wide kernel --------------------------------------------------------------------------
+
+// Many rows: 128 rows are the M operand, 256 output columns the N operand, so tensor memory lane =
+// row and the factor sx * sw is one number per thread and block (a row's scale; the two halves of
+// the columns are two rows of weight scales, one for each group of four epilogue warps).
+constexpr int kWideM = 128;
+constexpr int kWideN = 256;
+constexpr uint64_t kGroupBytes = 40ull << 20;  // rows of a group of tiles: part of the 126 MB L2
+constexpr uint64_t kGroupRows = 16;
+constexpr int kWideStages = 4;
+constexpr int kWideWarps = 8;  // epilogue: lane quarters x column halves
+constexpr int kWideThreads = 128 + 32 * kWideWarps;
+// Registers a thread: an epilogue thread holds 128 sums and 32 loaded values, the other four warps
+// hold next to nothing. Launched with 168 each (three warps per scheduler), handed over to
+// 40 + 2 x 232 = 3 x 168.
+constexpr int kWideFewRegisters = 40;
+constexpr int kWideManyRegisters = 232;
+static_assert(128 * kWideFewRegisters + 256 * kWideManyRegisters <= 384 * 168, "register hand-over");
+constexpr int kWideABytes = kWideM * kBlockK;
+constexpr int kWideWBytes = kWideN * kBlockK;
+constexpr int kWideStageBytes = kWideABytes + kWideWBytes;
+constexpr int kWideStoreBytes = 2048;  // per epilogue warp: 32 rows x 64 bytes on their way out
+constexpr size_t kWideTableBytes = (QPUCUDA_MAX_EXPERTS + 1) * sizeof(uint32_t);
+constexpr size_t kWideSharedBytes = kWideStages * kWideStageBytes + kWideWarps * kWideStoreBytes + kWideTableBytes + 256 + 1024;
+static_assert(kWideSharedBytes <= 227 * 1024, "shared memory");
+
+struct WideTile {
+    uint32_t expert, row0, row_end, n0;
+};
+
+// Tile order inside a matrix: groups of group_rows row blocks, the row block fastest inside a group,
+// so the rows of a group stay in L2 while its columns stream past and each weight tile is read from
+// DRAM once per group.
+__device__ __forceinline__ void order_tile(uint32_t tile, uint32_t m_blocks, uint32_t n_tiles, uint32_t group_rows,
+                                           uint32_t &m_block, uint32_t &n_tile) {
+    const uint32_t group_tiles = group_rows * n_tiles;
+    const uint32_t group = tile / group_tiles;
+    const uint32_t first = group * group_rows;
+    const uint32_t height = min(group_rows, m_blocks - first);
+    const uint32_t local = tile - group * group_tiles;
+    m_block = first + local % height;
+    n_tile = local / height;
+}
+
+// first_tile[e]: tiles of the experts before e. The last e with first_tile[e] <= tile holds it.
+__device__ __forceinline__ WideTile locate(const GemmParams &params, const uint32_t *first_tile, uint32_t n_tiles,
+                                           uint32_t group_rows, uint32_t tile) {
+    WideTile result;
+    uint32_t begin = 0, end = params.rows, local = tile;
+    result.expert = 0;
+    if (params.experts != 0) {
+        uint32_t low_e = 0, high_e = params.experts;  // first_tile[low_e] <= tile < first_tile[high_e]
+        while (high_e - low_e > 1) {
+            const uint32_t middle = (low_e + high_e) / 2;
+            if (first_tile[middle] <= tile) {
+                low_e = middle;
+            } else {
+                high_e = middle;
+            }
+        }
+        result.expert = low_e;
+        local = tile - first_tile[low_e];
+        const int32_t rows = static_cast<int32_t>(params.rows);
+        begin = static_cast<uint32_t>(min(max(params.offsets[low_e], 0), rows));
+        end = static_cast<uint32_t>(min(max(params.offsets[low_e + 1], static_cast<int32_t>(begin)), rows));
+    }
+    uint32_t m_block, n_tile;
+    order_tile(local, (end - begin + kWideM - 1) / kWideM, n_tiles, group_rows, m_block, n_tile);
+    result.row0 = begin + m_block * kWideM;
+    result.row_end = min(end, result.row0 + kWideM);
+    result.n0 = n_tile * kWideN;
+    return result;
+}
+
+// 64 bytes of each of a warp's 32 rows, transposed through shared memory so that four lanes write
+// one row's 64 bytes. Slot c of row r lies at slot c ^ ((r >> 1) & 3): no bank conflicts either way.
+template <typename Out>
+__device__ __forceinline__ void store_chunk(uint4 *buffer, const float (&v)[64 / sizeof(Out)], Out *out, size_t out_stride,
+                                            uint32_t rows, uint32_t columns, bool vector, uint32_t lane) {
+    constexpr int kColumns = 64 / sizeof(Out);
+    constexpr int kPerSlot = kColumns / 4;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        Vector<Out> slot;
+#pragma unroll
+        for (int i = 0; i < kPerSlot; ++i) slot.items[i] = from_float<Out>(v[c * kPerSlot + i]);
+        buffer[lane * 4 + (c ^ ((lane >> 1) & 3))] = slot.bits;
+    }
+    __syncwarp();
+    if (vector && columns >= kColumns) {
+        const uint32_t c = lane & 3u;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t r = i * 8u + lane / 4u;
+            const uint4 value = buffer[r * 4 + (c ^ ((r >> 1) & 3))];
+            if (r < rows) *reinterpret_cast<uint4 *>(out + r * out_stride + c * kPerSlot) = value;
+        }
+    } else if (lane < kColumns) {
+        const Out *items = reinterpret_cast<const Out *>(buffer);
+        for (uint32_t r = 0; r < min(rows, 32u); ++r)
+            if (lane < columns)
+                out[r * out_stride + lane] = items[(r * 4 + ((lane / kPerSlot) ^ ((r >> 1) & 3))) * kPerSlot + lane % kPerSlot];
+    }
+}
+
+// Persistent: one CTA per SM walks tiles blockIdx.x, + gridDim.x, ...
+//   warp 0   copies: a row box and two weight boxes per stage
+//   warp 1   tensor memory and MMA: 4 MMAs per stage into one of two accumulators
+//   warp 2   the experts' table of tiles, warp 3 nothing
+//   4 to 11  each block's accumulator into registers, scaled; at the tile's end the store
+template <typename Out>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                         const GemmParams params, uint32_t n_tiles, uint32_t group_rows) {
+    using Ctl = Control<kWideStages, 2>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *stage_w = smem;
+    uint8_t *stage_a = smem + kWideStages * kWideWBytes;
+    uint8_t *store = smem + kWideStages * kWideStageBytes;
+    uint32_t *first_tile = reinterpret_cast<uint32_t *>(store + kWideWarps * kWideStoreBytes);
+    Ctl *control = reinterpret_cast<Ctl *>(store + kWideWarps * kWideStoreBytes + kWideTableBytes + 4);
+    static_assert(sizeof(Ctl) <= 248 && (kWideTableBytes + 4) % 8 == 0, "control block");
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kWideStages; ++s) {
+            mbar_init(smem_u32(&control->full[s]), 1);
+            mbar_init(smem_u32(&control->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&control->tmem_full[b]), 1);
+            mbar_init(smem_u32(&control->tmem_empty[b]), kWideWarps);
+        }
+        mbar_init(smem_u32(&control->drain), 1);
+        control->abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&control->tmem_base)),
+                     "r"(2 * kWideN)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // The rows' copies, the offsets and every store come after the previous kernel. Weights are not
+    // read early here: the tiles are long.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 2 && params.experts != 0) {
+        uint32_t before = 0;
+        const int32_t rows = static_cast<int32_t>(params.rows);
+        for (uint32_t e0 = 0; e0 < params.experts; e0 += 32) {
+            const uint32_t e = e0 + lane;
+            uint32_t tiles = 0;
+            if (e < params.experts) {
+                const int32_t begin = min(max(params.offsets[e], 0), rows);
+                const int32_t end = min(max(params.offsets[e + 1], begin), rows);
+                tiles = (static_cast<uint32_t>(end - begin) + kWideM - 1) / kWideM * n_tiles;
+            }
+            uint32_t through = tiles;
+#pragma unroll
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, through, offset);
+                if (lane >= static_cast<uint32_t>(offset)) through += other;
+            }
+            if (e < params.experts) first_tile[e] = before + through - tiles;
+            before += __shfl_sync(0xFFFFFFFFu, through, 31);
+        }
+        if (lane == 0) first_tile[params.experts] = before;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = control->tmem_base;
+    const uint32_t total = params.experts != 0 ? first_tile[params.experts] : (params.rows + kWideM - 1) / kWideM * n_tiles;
+
+    if (warp == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
+        if (lane == 0) {
+            prefetch_tensor_map(&map_w);
+            prefetch_tensor_map(&map_a);
+            uint32_t stage = 0, phase = 0, issued_mask = 0, issued_phases = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                const WideTile tile = locate(params, first_tile, n_tiles, group_rows, t);
+                const int w_row = static_cast<int>(tile.expert * params.n + tile.n0);
+                for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+                    ok = wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word);
+                    if (!ok) break;
+                    const uint32_t full = smem_u32(&control->full[stage]);
+                    const int x = static_cast<int>(kb * kBlockK);
+                    mbar_expect_tx(full, kWideStageBytes);
+                    tma_load_2d(smem_u32(stage_a + stage * kWideABytes), &map_a, full, x, static_cast<int>(tile.row0));
+                    tma_load_2d(smem_u32(stage_w + stage * kWideWBytes), &map_w, full, x, w_row);
+                    tma_load_2d(smem_u32(stage_w + stage * kWideWBytes + kWideWBytes / 2), &map_w, full, x, w_row + kBlockN);
+                    issued_mask |= 1u << stage;
+                    issued_phases = (issued_phases & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kWideStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {  // let every copy in flight land before the CTA exits
+                for (int s = 0; s < kWideStages; ++s)
+                    if ((issued_mask >> s) & 1u) wait_drain(smem_u32(&control->full[s]), (issued_phases >> s) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
+        if (lane == 0) {
+            constexpr uint32_t instr = fp8_instr_desc(kWideM, kWideN);
+            uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 1;
+            bool ok = true, any = false;
+            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+                    ok = wait_bounded(smem_u32(&control->tmem_empty[buffer]), buffer_phase, &control->abort_flag, params.error_word) &&
+                         wait_bounded(smem_u32(&control->full[stage]), phase, &control->abort_flag, params.error_word);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t a = smem_desc_sw128(smem_u32(stage_a + stage * kWideABytes));
+                    const uint64_t w = smem_desc_sw128(smem_u32(stage_w + stage * kWideWBytes));
+#pragma unroll
+                    for (int kk = 0; kk < kBlockK / kMmaK; ++kk)
+                        mma_fp8(tmem_base + buffer * kWideN, a + static_cast<uint64_t>(kk * (kMmaK >> 4)),
+                                w + static_cast<uint64_t>(kk * (kMmaK >> 4)), instr, kk != 0 ? 1u : 0u);
+                    mma_commit(smem_u32(&control->empty[stage]));
+                    mma_commit(smem_u32(&control->tmem_full[buffer]));
+                    any = true;
+                    if (++stage == kWideStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    if (++buffer == 2) {
+                        buffer = 0;
+                        buffer_phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok && any) {
+                mma_commit(smem_u32(&control->drain));
+                wait_drain(smem_u32(&control->drain), 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideManyRegisters));
+        const uint32_t worker = warp - 4u;
+        const uint32_t quarter = warp & 3u;
+        const uint32_t half = worker / 4u;
+        uint4 *buffer_out = reinterpret_cast<uint4 *>(store + worker * kWideStoreBytes);
+        const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + half * (kWideN / 2);
+        const bool vector = (reinterpret_cast<uintptr_t>(params.out) & 15u) == 0 && params.out_stride * sizeof(Out) % 16 == 0;
+        uint32_t buffer = 0, buffer_phase = 0;
+        for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
+            const WideTile tile = locate(params, first_tile, n_tiles, group_rows, t);
+            const uint32_t n0 = tile.n0 + half * (kWideN / 2);
+            const uint32_t row0 = tile.row0 + quarter * 32u;
+            const bool row_inside = row0 + lane < tile.row_end;
+            const bool block_inside = n0 < params.n;
+            const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n0 / kBlockN) * params.k_blocks;
+            const float *a_scales = params.a_scales + static_cast<size_t>(row0 + lane) * params.a_scale_row_stride;
+            auto fetch = [&](uint32_t kb, float &a, float &w) {
+                const bool inside = kb < params.k_blocks;
+                a = inside && row_inside ? a_scales[static_cast<size_t>(kb) * params.a_scale_group_stride] : 0.0f;
+                w = inside && block_inside ? __ldg(w_scales + kb) : 0.0f;
+            };
+            float a_now, w_now, a_next, w_next;
+            fetch(0, a_now, w_now);
+            fetch(1, a_next, w_next);
+            uint64_t acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0;
+            bool ok = true;
+            for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+                const float factor = a_now * w_now;
+                const uint64_t factors = pack2(factor, factor);
+                a_now = a_next;
+                w_now = w_next;
+                fetch(kb + 2, a_next, w_next);
+                if (lane == 0) ok = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
+                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_load_x32(taddr + buffer * kWideN + c * 32, r);
+                    tmem_wait_load(r);
+                    if (c == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pack2(r[2 * i], r[2 * i + 1]), factors, acc[c * 16 + i]);
+                }
+                if (++buffer == 2) {
+                    buffer = 0;
+                    buffer_phase ^= 1u;
+                }
+            }
+            if (!ok) break;
+            if (row0 >= tile.row_end || !block_inside) continue;
+            constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
+            const uint32_t rows = tile.row_end - row0;
+#pragma unroll
+            for (int c = 0; c < kWideN / 2; c += kChunk) {
+                const uint32_t n = n0 + c;
+                if (n >= params.n) break;
+                float v[kChunk];
+#pragma unroll
+                for (int i = 0; i < kChunk; i += 2) {
+                    v[i] = low(acc[(c + i) / 2]);
+                    v[i + 1] = high(acc[(c + i) / 2]);
+                }
+                if (params.bias != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[i] += n + i < params.n ? __ldg(params.bias + n + i) : 0.0f;
+                }
+                store_chunk<Out>(buffer_out, v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
+                                 params.out_stride, rows, params.n - n, vector, lane);
+            }
+        }
+        if (params.experts != 0) {
+            // rows no expert owns
+            const uint32_t step = gridDim.x * kWideWarps;
+            for (uint32_t row = owned_rows(params) + blockIdx.x * kWideWarps + worker; row < params.rows; row += step)
+                for (uint32_t n = lane; n < params.n; n += 32)
+                    static_cast<Out *>(params.out)[static_cast<size_t>(row) * params.out_stride + n] = from_float<Out>(0.0f);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kWideN) : "memory");
+    }
+}
+
+template <typename Out>
+cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, uint64_t tiles,
+                        uint32_t n_tiles, uint32_t group_rows, int sm_count, cudaStream_t stream) {
+    static PerDeviceOnce configured;
+    const cudaError_t error = configured.run([] {
+        return cudaFuncSetAttribute(fp8_gemm_wide_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(kWideSharedBytes));
+    });
+    if (error != cudaSuccess) return error;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(tiles < static_cast<uint64_t>(sm_count) ? tiles : static_cast<uint64_t>(sm_count)));
+    config.blockDim = dim3(kWideThreads);
+    config.dynamicSmemBytes = kWideSharedBytes;
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out>, map_w, map_a, params, n_tiles, group_rows);
+}
+
 }  // namespace
 
 cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word, int sm_count,
@@ -462,6 +829,28 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
     params.weights_settled = desc.weights_settled != 0 ? 1u : 0u;
     params.error_word = error_word;
     const uint64_t matrices = desc.experts != 0 ? desc.experts : 1u;
+    // Rows of an even share, and tiles of 128 x 256 at most, whatever the offsets.
+    const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;
+    const uint32_t n_tiles = (desc.n + kWideN - 1) / kWideN;
+    const uint64_t wide_tiles = (static_cast<uint64_t>(desc.rows) + filled * (kWideM - 1)) / kWideM * n_tiles;
+    if (wide_tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    if (desc.rows / matrices >= kWideM && wide_tiles >= static_cast<uint64_t>(sm_count)) {
+        CUtensorMap map_w, map_a;
+        if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
+            !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, kWideM)) {
+            return cudaErrorInvalidValue;
+        }
+        uint64_t group = kGroupBytes / (static_cast<uint64_t>(kWideM) * desc.k);
+        group = group < kGroupRows ? kGroupRows : group;
+        const uint32_t group_rows = static_cast<uint32_t>(group < 0x10000u ? group : 0x10000u);
+        switch (desc.out_type) {
+            case QPUCUDA_DTYPE_F32: return launch_wide<float>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
+            case QPUCUDA_DTYPE_BF16:
+                return launch_wide<__nv_bfloat16>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
+            case QPUCUDA_DTYPE_F16: return launch_wide<__half>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
+        }
+        return cudaErrorInvalidValue;
+    }
     // The tile's height: the smallest that holds an expert's even share of the rows.
     const uint64_t share = (desc.rows + matrices - 1) / matrices;
     const int nt = share <= 16 ? 16 : (share <= 32 ? 32 : (share <= 64 ? 64 : 128));
@@ -471,7 +860,6 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
         return cudaErrorInvalidValue;
     }
     // At most this many tiles of rows, whatever the offsets: one partly filled tile per matrix.
-    const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;
     const uint64_t tiles = (static_cast<uint64_t>(desc.rows) + filled * (nt - 1)) / nt;
     if (tiles > 65535u) return cudaErrorInvalidValue;
     // K is split over a cluster while the tiles leave SMs idle, two CTAs each.
