@@ -718,34 +718,51 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            bool ok = true;
-            for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+            // 32 columns at a time through two sets of registers: the next load is under way while
+            // the previous one is added, across the blocks' border as well.
+            uint32_t even[32], odd[32];
+            auto add = [&](int c, const uint32_t (&r)[32], uint64_t factors) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pack2(r[2 * i], r[2 * i + 1]), factors, acc[c * 16 + i]);
+            };
+            auto arrived = [&]() {
+                bool full = true;
+                if (lane == 0) full = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
+                full = __shfl_sync(0xFFFFFFFFu, full ? 1 : 0, 0) != 0;
+                tc_fence_after();
+                return full;
+            };
+            bool ok = arrived();
+            if (ok) tmem_load_x32(taddr + buffer * kWideN, even);
+            for (uint32_t kb = 0; ok && kb < params.k_blocks; ++kb) {
                 const float factor = a_now * w_now;
                 const uint64_t factors = pack2(factor, factor);
                 a_now = a_next;
                 w_now = w_next;
                 fetch(kb + 2, a_next, w_next);
-                if (lane == 0) ok = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
-                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    tmem_load_x32(taddr + buffer * kWideN + c * 32, r);
-                    tmem_wait_load(r);
-                    if (c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pack2(r[2 * i], r[2 * i + 1]), factors, acc[c * 16 + i]);
-                }
+                const uint32_t block = taddr + buffer * kWideN;
+                tmem_wait_load(even);
+                tmem_load_x32(block + 32, odd);
+                add(0, even, factors);
+                tmem_wait_load(odd);
+                tmem_load_x32(block + 64, even);
+                add(1, odd, factors);
+                tmem_wait_load(even);
+                tmem_load_x32(block + 96, odd);
+                add(2, even, factors);
+                tmem_wait_load(odd);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
                 if (++buffer == 2) {
                     buffer = 0;
                     buffer_phase ^= 1u;
                 }
+                if (kb + 1 < params.k_blocks) {
+                    ok = arrived();
+                    if (ok) tmem_load_x32(taddr + buffer * kWideN, even);
+                }
+                add(3, odd, factors);
             }
             if (!ok) break;
             if (row0 >= tile.row_end || !block_inside) continue;

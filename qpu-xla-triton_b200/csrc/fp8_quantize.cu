@@ -25,25 +25,48 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
-__device__ __forceinline__ float group_scale(float amax) { return max_nan(__fdiv_rn(amax, kE4m3Max), kScaleFloor); }
-
-// RN(x / s) up to what the rounding to e4m3 can see, without a division per element. p = x * RN(1/s)
-// lies within 3 * 2^-24 |x/s| (1.5 fp32 steps) of x / s, so within 2 fp32 steps of RN(x / s). e4m3
-// keeps 3 of the 23 fraction bits in its normal range (from 2^-6): its rounding borders there have
-// the low 20 bits 0x80000, and p rounds as RN(x / s) does unless it is within 4 steps of one (9 in
-// 2^20 values). Those, and values below 2^-6 (rare: s makes the group's largest 448), are divided;
-// zero is exact either way.
-__device__ __forceinline__ float quotient(float x, float scale, float inverse) {
-    float p = __fmul_rn(x, inverse);
-    const uint32_t bits = __float_as_uint(p);
-    const bool near_border = ((bits - 0x7FFFCu) & 0xFFFFFu) <= 8u;
-    const bool small = fabsf(p) < 0.015625f && x != 0.0f;
-    if (near_border || small) p = __fdiv_rn(x, scale);
-    return p;
+// max(RN(amax / 448), 2^-60), the quotient by Markstein's correction of a product with the rounded
+// reciprocal: q0 = RN(a y) with y = RN(1 / 448) is within one step of a / 448, the remainder a - 448 q0
+// is exact in an fma, and RN(q0 + remainder * y) is then the rounded quotient (amax above 2^-100;
+// anything smaller ends at the floor). An infinite amax gives NaN, which serves as well.
+__device__ __forceinline__ float group_scale(float amax) {
+    constexpr float kReciprocal = 1.0f / 448.0f;
+    const float q0 = __fmul_rn(amax, kReciprocal);
+    const float remainder = __fmaf_rn(-q0, kE4m3Max, amax);
+    return max_nan(__fmaf_rn(remainder, kReciprocal, q0), kScaleFloor);
 }
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+           (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
+}
+
+// e4m3(RN(x / s)) of N values without a division each. The products with two reciprocals, 2^-20
+// below and above an approximate one (which is within 2^-23; each product rounds by 2^-24), lie on
+// either side of x / s, so of RN(x / s) too. Rounding to e4m3 is monotonic: where both give the same
+// value, so does RN(x / s), in the subnormal range and at zero as well. Otherwise (a border within
+// 2^-20, 1.5e-5 of the values) the quotients of all N are formed.
+template <int N>
+__device__ __forceinline__ void quantize_values(const float (&v)[N], float scale, uint32_t (&packed)[N / 4]) {
+    const float inverse = reciprocal(scale);
+    const float below = inverse * (1.0f - 9.5367431640625e-07f), above = inverse * (1.0f + 9.5367431640625e-07f);
+    bool differ = false;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        packed[i / 4] = e4m3x4(v[i] * below, v[i + 1] * below, v[i + 2] * below, v[i + 3] * below);
+        differ |= packed[i / 4] != e4m3x4(v[i] * above, v[i + 1] * above, v[i + 2] * above, v[i + 3] * above);
+    }
+    if (differ) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            packed[i / 4] = e4m3x4(__fdiv_rn(v[i], scale), __fdiv_rn(v[i + 1], scale), __fdiv_rn(v[i + 2], scale), __fdiv_rn(v[i + 3], scale));
+    }
 }
 
 // silu(g) * u in fp32. exp(-g) overflows to infinity below g = -88.7, where the quotient is then -0
@@ -147,14 +170,8 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
             for (int offset = kLanes / 2; offset > 0; offset >>= 1)
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, offset));
             const float scale = group_scale(amax);
-            const float inverse = __frcp_rn(scale);
             uint32_t packed[kVector<T> / 4];
-#pragma unroll
-            for (int i = 0; i < kVector<T>; i += 4) {
-                packed[i / 4] =
-                    e4m3x2(quotient(v[u][i], scale, inverse), quotient(v[u][i + 1], scale, inverse)) |
-                    (e4m3x2(quotient(v[u][i + 2], scale, inverse), quotient(v[u][i + 3], scale, inverse)) << 16);
-            }
+            quantize_values(v[u], scale, packed);
             const uint32_t column = groups[u] * 128u + inner;
             if (rows[u] < params.rows) {
                 // q rows are padded to 16 bytes, so a vector that starts below cols fits
