@@ -46,7 +46,7 @@ typedef struct qpucuda_fp8_quantize_desc {
     uint32_t cols;
     int gated;               /* nonzero: quantize silu(gate) * up, computed in fp32 */
     /* Row r is made from source row row_source[r] / row_divisor; a negative entry gives a zero
-     * row. NULL: row r from source row r. Entries are below source_rows * row_divisor. */
+     * row, as does one past source_rows. NULL: row r from source row r. */
     const int32_t *row_source;
     uint32_t row_divisor;
     uint32_t source_rows;
@@ -96,6 +96,12 @@ typedef struct qpucuda_fp8_gemm_desc {
 #define QPUCUDA_MAX_EXPERTS 1024u
 
 qpucuda_status qpucuda_fp8_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc);
+
+/* Both in one call: the rows into quantize->q and ->scales, then the product that reads them (its a,
+ * a_stride, a_scales, rows and k must be those; weights_settled may then be set unless the call just
+ * before this one still writes the weight when the rows are quantized). */
+qpucuda_status qpucuda_fp8_linear(qpucuda_context *context, const qpucuda_fp8_quantize_desc *quantize,
+                                  const qpucuda_fp8_gemm_desc *gemm);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

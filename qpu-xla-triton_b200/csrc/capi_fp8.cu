@@ -35,13 +35,8 @@ bool routing_fits(uint32_t tokens, uint32_t choices, uint32_t experts) {
            static_cast<uint64_t>(tokens) * choices <= static_cast<uint64_t>(INT32_MAX);
 }
 
-}  // namespace
-
-extern "C" {
-
-qpucuda_status qpucuda_fp8_quantize_rows(qpucuda_context *context, const qpucuda_fp8_quantize_desc *desc) {
-    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
-    if (desc->rows == 0) return QPUCUDA_OK;
+// Argument checks: QPUCUDA_OK, or the refusal with its message. `rows` is not zero.
+qpucuda_status check_quantize(qpucuda_context *context, const qpucuda_fp8_quantize_desc *desc) {
     const uint64_t width = static_cast<uint64_t>(desc->cols) * (desc->gated != 0 ? 2u : 1u);
     if (!known_type(desc->x_type) || desc->cols == 0 || desc->cols > INT32_MAX || desc->x == nullptr || desc->q == nullptr ||
         desc->scales == nullptr || desc->x_stride < width || desc->q_stride < desc->cols || desc->q_stride % 16 != 0 ||
@@ -50,9 +45,44 @@ qpucuda_status qpucuda_fp8_quantize_rows(qpucuda_context *context, const qpucuda
                     "fp8_quantize_rows: needs fp32, bf16 or fp16 rows, and 16-byte aligned values with row strides "
                     "that are multiples of 16 and hold the columns");
     }
-    if (desc->row_source != nullptr && desc->row_divisor == 0) {
+    if (desc->row_source != nullptr && (desc->row_divisor == 0 || !aligned(desc->row_source, 4))) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT, "fp8_quantize_rows: row_divisor must be positive");
     }
+    return QPUCUDA_OK;
+}
+
+qpucuda_status check_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc) {
+    const uint64_t matrices = desc->experts != 0 ? desc->experts : 1u;
+    if (!known_type(desc->out_type) || desc->n == 0 || desc->k == 0 || desc->k > INT32_MAX || desc->rows > INT32_MAX ||
+        desc->a == nullptr || desc->a_scales == nullptr || desc->w == nullptr || desc->w_scales == nullptr ||
+        desc->out == nullptr || desc->a_stride < desc->k || desc->w_stride < desc->k || desc->a_stride % 16 != 0 ||
+        desc->w_stride % 16 != 0 || !aligned(desc->a, 16) || !aligned(desc->w, 16) || desc->out_stride < desc->n ||
+        !aligned(desc->out, type_bytes(desc->out_type)) || !aligned(desc->a_scales, 4) || !aligned(desc->w_scales, 4) ||
+        !aligned(desc->bias, 4) || !aligned(desc->offsets, 4)) {
+        return fail(context, QPUCUDA_INVALID_ARGUMENT,
+                    "fp8_gemm: operands need 16-byte aligned rows and in-range strides, the output fp32, bf16 or fp16");
+    }
+    if (desc->experts > QPUCUDA_MAX_EXPERTS || (desc->experts != 0 && (desc->offsets == nullptr || desc->bias != nullptr)) ||
+        matrices * desc->n > static_cast<uint64_t>(INT32_MAX)) {
+        return fail(context, QPUCUDA_INVALID_ARGUMENT,
+                    "fp8_gemm: experts need offsets and no bias, at most %u of them and 2^31 weight rows in all",
+                    QPUCUDA_MAX_EXPERTS);
+    }
+    if (!(context->cc_major == 10 && context->cc_minor == 0)) {
+        return fail(context, QPUCUDA_CAPABILITY_MISSING, "fp8_gemm: the tcgen05 FP8 product needs an sm_100 device");
+    }
+    return QPUCUDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+qpucuda_status qpucuda_fp8_quantize_rows(qpucuda_context *context, const qpucuda_fp8_quantize_desc *desc) {
+    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    if (desc->rows == 0) return QPUCUDA_OK;
+    const qpucuda_status checked = check_quantize(context, desc);
+    if (checked != QPUCUDA_OK) return checked;
     return submit(context, "fp8_quantize_rows",
                   [&] { return launch_fp8_quantize_rows(*desc, context->sm_count, context->stream); });
 }
@@ -75,27 +105,28 @@ qpucuda_status qpucuda_fp8_quantize_blocks(qpucuda_context *context, const void 
 qpucuda_status qpucuda_fp8_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc) {
     if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
     if (desc->rows == 0) return QPUCUDA_OK;
-    const uint64_t matrices = desc->experts != 0 ? desc->experts : 1u;
-    if (!known_type(desc->out_type) || desc->n == 0 || desc->k == 0 || desc->k > INT32_MAX || desc->rows > INT32_MAX ||
-        desc->a == nullptr || desc->a_scales == nullptr || desc->w == nullptr || desc->w_scales == nullptr ||
-        desc->out == nullptr || desc->a_stride < desc->k || desc->w_stride < desc->k || desc->a_stride % 16 != 0 ||
-        desc->w_stride % 16 != 0 || !aligned(desc->a, 16) || !aligned(desc->w, 16) || desc->out_stride < desc->n ||
-        !aligned(desc->out, type_bytes(desc->out_type)) || !aligned(desc->a_scales, 4) || !aligned(desc->w_scales, 4) ||
-        !aligned(desc->bias, 4) || !aligned(desc->offsets, 4)) {
-        return fail(context, QPUCUDA_INVALID_ARGUMENT,
-                    "fp8_gemm: operands need 16-byte aligned rows and in-range strides, the output fp32, bf16 or fp16");
-    }
-    if (desc->experts > QPUCUDA_MAX_EXPERTS || (desc->experts != 0 && (desc->offsets == nullptr || desc->bias != nullptr)) ||
-        matrices * desc->n > static_cast<uint64_t>(INT32_MAX)) {
-        return fail(context, QPUCUDA_INVALID_ARGUMENT,
-                    "fp8_gemm: experts need offsets and no bias, at most %u of them and 2^31 weight rows in all",
-                    QPUCUDA_MAX_EXPERTS);
-    }
-    if (!(context->cc_major == 10 && context->cc_minor == 0)) {
-        return fail(context, QPUCUDA_CAPABILITY_MISSING, "fp8_gemm: the tcgen05 FP8 product needs an sm_100 device");
-    }
+    const qpucuda_status checked = check_gemm(context, desc);
+    if (checked != QPUCUDA_OK) return checked;
     return submit(context, "fp8_gemm",
                   [&] { return launch_fp8_gemm(*desc, context->d_error, context->sm_count, context->stream); });
+}
+
+qpucuda_status qpucuda_fp8_linear(qpucuda_context *context, const qpucuda_fp8_quantize_desc *quantize,
+                                  const qpucuda_fp8_gemm_desc *gemm) {
+    if (context == nullptr || quantize == nullptr || gemm == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    if (quantize->rows == 0 && gemm->rows == 0) return QPUCUDA_OK;
+    if (quantize->rows != gemm->rows || quantize->cols != gemm->k || quantize->q != gemm->a ||
+        quantize->q_stride != gemm->a_stride || quantize->scales != gemm->a_scales ||
+        quantize->scale_row_stride != gemm->a_scale_row_stride || quantize->scale_group_stride != gemm->a_scale_group_stride) {
+        return fail(context, QPUCUDA_INVALID_ARGUMENT, "fp8_linear: the product must read the rows that are quantized");
+    }
+    qpucuda_status checked = check_quantize(context, quantize);
+    if (checked == QPUCUDA_OK) checked = check_gemm(context, gemm);
+    if (checked != QPUCUDA_OK) return checked;
+    return submit(context, "fp8_linear", [&] {
+        const cudaError_t error = launch_fp8_quantize_rows(*quantize, context->sm_count, context->stream);
+        return error != cudaSuccess ? error : launch_fp8_gemm(*gemm, context->d_error, context->sm_count, context->stream);
+    });
 }
 
 size_t qpucuda_expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts) {

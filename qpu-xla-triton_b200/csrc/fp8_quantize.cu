@@ -12,6 +12,7 @@
 #include "element.cuh"
 #include "qpucuda_fp8_internal.h"
 #include "qpucuda_internal.h"
+#include "sm100_fp8.cuh"
 
 namespace qpucuda {
 namespace {
@@ -36,37 +37,30 @@ __device__ __forceinline__ float group_scale(float amax) {
     return max_nan(__fmaf_rn(remainder, kReciprocal, q0), kScaleFloor);
 }
 
-__device__ __forceinline__ float reciprocal(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
-           (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
-}
-
-// e4m3(RN(x / s)) of N values without a division each. The products with two reciprocals, 2^-20
-// below and above an approximate one (which is within 2^-23; each product rounds by 2^-24), lie on
-// either side of x / s, so of RN(x / s) too. Rounding to e4m3 is monotonic: where both give the same
-// value, so does RN(x / s), in the subnormal range and at zero as well. Otherwise (a border within
-// 2^-20, 1.5e-5 of the values) the quotients of all N are formed.
+// e4m3(RN(x / s)) of N values, two to an instruction. A hardware division per value, or a branch to
+// one near the borders of e4m3 (bf16 values over a bf16 maximum lie on borders in 1 of 500 cases, so
+// half of the warps took it), costs more than the copy itself. Markstein's correction instead, twice:
+// with y = RN(1 / s), q1 = RN(q0 + (x - q0 s) y) is within one step of x / s, its remainder is exact in
+// an fma, and RN(q1 + (x - q1 s) y) is the rounded quotient (Markstein 1990). That needs remainders
+// above the smallest normal number: true for every quotient above 2^-10, the smallest border of e4m3,
+// as s is at least 2^-60; smaller quotients end as zero whatever their last bits.
 template <int N>
 __device__ __forceinline__ void quantize_values(const float (&v)[N], float scale, uint32_t (&packed)[N / 4]) {
-    const float inverse = reciprocal(scale);
-    const float below = inverse * (1.0f - 9.5367431640625e-07f), above = inverse * (1.0f + 9.5367431640625e-07f);
-    bool differ = false;
+    using sm100::fma2;
+    using sm100::pack2;
+    const float inverse = __frcp_rn(scale);
+    const uint64_t y = pack2(inverse, inverse), minus_s = pack2(-scale, -scale), zero = pack2(-0.0f, -0.0f);
+    uint16_t pairs[N / 2];
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        packed[i / 4] = e4m3x4(v[i] * below, v[i + 1] * below, v[i + 2] * below, v[i + 3] * below);
-        differ |= packed[i / 4] != e4m3x4(v[i] * above, v[i + 1] * above, v[i + 2] * above, v[i + 3] * above);
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t x = pack2(v[i], v[i + 1]);
+        uint64_t q = fma2(x, y, zero);
+        q = fma2(fma2(q, minus_s, x), y, q);
+        q = fma2(fma2(q, minus_s, x), y, q);
+        pairs[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(sm100::low(q), sm100::high(q)), __NV_SATFINITE, __NV_E4M3);
     }
-    if (differ) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4)
-            packed[i / 4] = e4m3x4(__fdiv_rn(v[i], scale), __fdiv_rn(v[i + 1], scale), __fdiv_rn(v[i + 2], scale), __fdiv_rn(v[i + 3], scale));
-    }
+    for (int i = 0; i < N / 4; ++i) packed[i] = pairs[2 * i] | (static_cast<uint32_t>(pairs[2 * i + 1]) << 16);
 }
 
 // silu(g) * u in fp32. exp(-g) overflows to infinity below g = -88.7, where the quotient is then -0
@@ -85,84 +79,81 @@ struct RowsParams {
     size_t scale_row_stride, scale_group_stride;
 };
 
-// Elements [column, column + kVector) of a row as fp32, zero past cols.
+// kVector elements at x as fp32, zero from `remaining` of them on.
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void load_row(const T *row, uint32_t column, uint32_t cols, float (&v)[kVector<T>]) {
-    if (VECTOR && column + kVector<T> <= cols) {
+__device__ __forceinline__ void load_row(const T *x, uint32_t remaining, float (&v)[kVector<T>]) {
+    if (VECTOR) {
         Vector<T> raw;
-        raw.bits = load_stream16(row + column);
+        raw.bits = make_uint4(0, 0, 0, 0);
+        if (remaining >= static_cast<uint32_t>(kVector<T>)) {
+            raw.bits = load_stream16(x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVector<T>; ++i)
+                if (static_cast<uint32_t>(i) < remaining) raw.items[i] = x[i];
+        }
 #pragma unroll
         for (int i = 0; i < kVector<T>; ++i) v[i] = to_float(raw.items[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < kVector<T>; ++i) v[i] = column + i < cols ? to_float(row[column + i]) : 0.0f;
+        for (int i = 0; i < kVector<T>; ++i) v[i] = static_cast<uint32_t>(i) < remaining ? to_float(x[i]) : 0.0f;
     }
 }
 
 // One group is 128 columns of a row: kVector elements on each of 32 (fp32) or 16 (16-bit) lanes, so
 // every lane moves 16 bytes and the maximum is a shuffle reduction inside those lanes. A warp takes
-// kUnroll steps of one or two neighbouring groups and loads them all before it uses the first.
-// Reads each input once and writes each output once: bound by HBM.
+// STEPS steps of one or two neighbouring groups of one row, at fixed distances from one address, and
+// loads them all before it uses the first. Each input is read once, each output written once; what
+// it has to keep below HBM's time is its instructions.
 constexpr int kRowsThreads = 256;
-constexpr int kUnroll = 4;
 
-template <typename T, bool GATED, bool VECTOR>
-__global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const RowsParams params) {
+template <typename T, bool GATED, bool VECTOR, int STEPS>
+__global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const RowsParams params, uint32_t chunks) {
     constexpr int kLanes = 128 / kVector<T>;
     constexpr int kPerStep = 32 / kLanes;
-    constexpr int kPerWarp = kPerStep * kUnroll;
     // The source may be the previous kernel's output. Once it is complete, the product that follows
     // may start and stream its weights while the rows are quantized.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t total = static_cast<uint64_t>(params.rows) * params.groups;
+    const uint32_t inner = lane * kVector<T>;  // column inside a step
+    const uint64_t total = static_cast<uint64_t>(params.rows) * chunks;
     const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kRowsThreads / 32);
-    for (uint64_t item0 = (static_cast<uint64_t>(blockIdx.x) * (kRowsThreads / 32) + threadIdx.x / 32) * kPerWarp;
-         item0 < total; item0 += warps * kPerWarp) {
-        const uint64_t first = item0 + lane / kLanes;
-        uint32_t row, group;
+    for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kRowsThreads / 32) + threadIdx.x / 32; item < total; item += warps) {
+        uint32_t row, chunk;
         if (total <= 0xFFFFFFFFull) {
-            row = static_cast<uint32_t>(first) / params.groups;
-            group = static_cast<uint32_t>(first) - row * params.groups;
+            row = static_cast<uint32_t>(item) / chunks;
+            chunk = static_cast<uint32_t>(item) - row * chunks;
         } else {
-            row = static_cast<uint32_t>(first / params.groups);
-            group = static_cast<uint32_t>(first - static_cast<uint64_t>(row) * params.groups);
+            row = static_cast<uint32_t>(item / chunks);
+            chunk = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * chunks);
         }
-        float v[kUnroll][kVector<T>];
-        uint32_t rows[kUnroll], groups[kUnroll];
-        const uint32_t inner = (lane % kLanes) * kVector<T>;
+        uint32_t source = row;
+        if (params.row_source != nullptr) {
+            const int32_t entry = params.row_source[row];
+            source = entry < 0 ? 0xFFFFFFFFu : static_cast<uint32_t>(entry) / params.row_divisor;
+        }
+        const bool present = source < params.source_rows;
+        const uint32_t column0 = chunk * (STEPS * kPerStep * 128u) + inner;
+        const T *x = static_cast<const T *>(params.x) + (present ? static_cast<size_t>(source) * params.x_stride : 0) + column0;
+        float v[STEPS][kVector<T>];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            rows[u] = row;
-            groups[u] = group;
-            const uint32_t column = group * 128u + inner;
-            int64_t source = row < params.rows ? static_cast<int64_t>(row) : -1;
-            if (source >= 0 && params.row_source != nullptr) {
-                const int32_t entry = params.row_source[row];
-                source = entry < 0 ? -1 : static_cast<int64_t>(static_cast<uint32_t>(entry) / params.row_divisor);
-                if (source >= static_cast<int64_t>(params.source_rows)) source = -1;
-            }
+        for (int u = 0; u < STEPS; ++u) {
+            constexpr int kStep = kPerStep * 128;
+            const uint32_t remaining = present && column0 + u * kStep < params.cols ? params.cols - column0 - u * kStep : 0u;
+            load_row<T, VECTOR>(x + u * kStep, remaining, v[u]);
+            if (GATED) {
+                float up[kVector<T>];
+                load_row<T, VECTOR>(x + params.cols + u * kStep, remaining, up);
 #pragma unroll
-            for (int i = 0; i < kVector<T>; ++i) v[u][i] = 0.0f;
-            if (source >= 0 && column < params.cols) {
-                const T *x = static_cast<const T *>(params.x) + static_cast<size_t>(source) * params.x_stride;
-                load_row<T, VECTOR>(x, column, params.cols, v[u]);
-                if (GATED) {
-                    float up[kVector<T>];
-                    load_row<T, VECTOR>(x + params.cols, column, params.cols, up);
-#pragma unroll
-                    for (int i = 0; i < kVector<T>; ++i) v[u][i] = silu_times(v[u][i], up[i]);
-                }
-            }
-            group += kPerStep;
-            while (group >= params.groups) {
-                group -= params.groups;
-                ++row;
+                for (int i = 0; i < kVector<T>; ++i) v[u][i] = silu_times(v[u][i], up[i]);
             }
         }
+        uint8_t *q = params.q + static_cast<size_t>(row) * params.q_stride + column0;
+        const uint32_t group0 = column0 / 128u;
+        float *scales = params.scales + static_cast<size_t>(row) * params.scale_row_stride + static_cast<size_t>(group0) * params.scale_group_stride;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < STEPS; ++u) {
             float amax = 0.0f;
 #pragma unroll
             for (int i = 0; i < kVector<T>; ++i) amax = max_nan(amax, fabsf(v[u][i]));
@@ -172,20 +163,14 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
             const float scale = group_scale(amax);
             uint32_t packed[kVector<T> / 4];
             quantize_values(v[u], scale, packed);
-            const uint32_t column = groups[u] * 128u + inner;
-            if (rows[u] < params.rows) {
+            if (column0 + u * (kPerStep * 128u) < params.cols) {
                 // q rows are padded to 16 bytes, so a vector that starts below cols fits
-                if (column < params.cols) {
-                    uint8_t *q = params.q + static_cast<size_t>(rows[u]) * params.q_stride + column;
-                    if constexpr (kVector<T> == 8) {
-                        *reinterpret_cast<uint2 *>(q) = make_uint2(packed[0], packed[kVector<T> / 4 - 1]);
-                    } else {
-                        *reinterpret_cast<uint32_t *>(q) = packed[0];
-                    }
+                if constexpr (kVector<T> == 8) {
+                    *reinterpret_cast<uint2 *>(q + u * kPerStep * 128) = make_uint2(packed[0], packed[kVector<T> / 4 - 1]);
+                } else {
+                    *reinterpret_cast<uint32_t *>(q + u * kPerStep * 128) = packed[0];
                 }
-                if (inner == 0)
-                    params.scales[static_cast<size_t>(rows[u]) * params.scale_row_stride +
-                                  static_cast<size_t>(groups[u]) * params.scale_group_stride] = scale;
+                if (lane % kLanes == 0) scales[static_cast<size_t>(u * kPerStep) * params.scale_group_stride] = scale;
             }
         }
     }
@@ -223,11 +208,12 @@ __global__ void __launch_bounds__(256) quantize_blocks_fp8_kernel(const T *__res
         }
 }
 
-template <typename T, bool GATED>
-cudaError_t launch_rows(const RowsParams &params, bool vector, int sm_count, cudaStream_t stream) {
-    constexpr uint64_t kPerBlock = static_cast<uint64_t>(32 / (128 / kVector<T>)) * kUnroll * (kRowsThreads / 32);
-    const uint64_t total = static_cast<uint64_t>(params.rows) * params.groups;
-    uint64_t blocks = (total + kPerBlock - 1) / kPerBlock;
+template <typename T, bool GATED, bool VECTOR, int STEPS>
+cudaError_t launch_rows(const RowsParams &params, int sm_count, cudaStream_t stream) {
+    constexpr uint32_t kGroups = static_cast<uint32_t>(32 / (128 / kVector<T>)) * STEPS;
+    const uint32_t chunks = (params.groups + kGroups - 1) / kGroups;
+    const uint64_t warps = static_cast<uint64_t>(params.rows) * chunks;
+    uint64_t blocks = (warps + kRowsThreads / 32 - 1) / (kRowsThreads / 32);
     const uint64_t most = static_cast<uint64_t>(sm_count) * 64u;
     if (blocks > most) blocks = most;
     cudaLaunchAttribute attribute{};
@@ -239,8 +225,17 @@ cudaError_t launch_rows(const RowsParams &params, bool vector, int sm_count, cud
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    return vector ? cudaLaunchKernelEx(&config, quantize_rows_fp8_kernel<T, GATED, true>, params)
-                  : cudaLaunchKernelEx(&config, quantize_rows_fp8_kernel<T, GATED, false>, params);
+    return cudaLaunchKernelEx(&config, quantize_rows_fp8_kernel<T, GATED, VECTOR, STEPS>, params, chunks);
+}
+
+// Four steps a warp where that still gives every SM several warps' worth of work, one otherwise.
+template <typename T, bool GATED>
+cudaError_t launch_rows_steps(const RowsParams &params, bool vector, int sm_count, cudaStream_t stream) {
+    const bool many = params.groups >= 4 && static_cast<uint64_t>(params.rows) * params.groups >= static_cast<uint64_t>(sm_count) * 64u;
+    if (vector) {
+        return many ? launch_rows<T, GATED, true, 4>(params, sm_count, stream) : launch_rows<T, GATED, true, 1>(params, sm_count, stream);
+    }
+    return many ? launch_rows<T, GATED, false, 4>(params, sm_count, stream) : launch_rows<T, GATED, false, 1>(params, sm_count, stream);
 }
 
 template <typename T>
@@ -253,7 +248,7 @@ cudaError_t launch_rows_type(const qpucuda_fp8_quantize_desc &desc, int sm_count
     params.groups = (desc.cols + 127u) / 128u;
     params.row_source = desc.row_source;
     params.row_divisor = desc.row_divisor;
-    params.source_rows = desc.source_rows;
+    params.source_rows = desc.row_source != nullptr ? desc.source_rows : desc.rows;
     params.q = desc.q;
     params.q_stride = desc.q_stride;
     params.scales = desc.scales;
@@ -262,8 +257,8 @@ cudaError_t launch_rows_type(const qpucuda_fp8_quantize_desc &desc, int sm_count
     // 16-byte loads need aligned rows and, gated, an aligned second half.
     const bool vector = (reinterpret_cast<uintptr_t>(desc.x) & 15u) == 0 && desc.x_stride % kVector<T> == 0 &&
                         (desc.gated == 0 || desc.cols % kVector<T> == 0);
-    return desc.gated != 0 ? launch_rows<T, true>(params, vector, sm_count, stream)
-                           : launch_rows<T, false>(params, vector, sm_count, stream);
+    return desc.gated != 0 ? launch_rows_steps<T, true>(params, vector, sm_count, stream)
+                           : launch_rows_steps<T, false>(params, vector, sm_count, stream);
 }
 
 }  // namespace

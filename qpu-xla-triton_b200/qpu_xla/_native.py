@@ -313,6 +313,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "qpucuda_fp8_quantize_rows": (_S, [_P, POINTER(Fp8QuantizeDesc)]),
     "qpucuda_fp8_quantize_blocks": (_S, [_P, _P, c_int, c_size_t, c_uint32, c_uint32, c_uint32, _P, c_size_t, _P]),
     "qpucuda_fp8_gemm": (_S, [_P, POINTER(Fp8GemmDesc)]),
+    "qpucuda_fp8_linear": (_S, [_P, POINTER(Fp8QuantizeDesc), POINTER(Fp8GemmDesc)]),
     # qpucuda_experts.h
     "qpucuda_expert_sort_workspace": (c_size_t, [c_uint32, c_uint32, c_uint32]),
     "qpucuda_expert_sort": (_S, [_P, _P, c_int, c_uint32, c_uint32, c_uint32, _P, _P, _P, _P, c_size_t]),

@@ -113,7 +113,16 @@ class CudaBackend:
                 self.device_ordinal, timeout_ns=timeout_ns, failure_mask=failure_mask, stream=None
             )
         self.launch_lock = threading.RLock()
+        # The current stream's handle without a Stream object around it (0.1 against 2.2 us a call).
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._closed = False
+
+    @property
+    def current_stream_handle(self: Self) -> int:
+        """The cudaStream_t that is current on this device."""
+        if self._raw_stream is not None:
+            return int(self._raw_stream(self.device_ordinal))
+        return int(self._torch.cuda.current_stream(self.torch_device).cuda_stream)
 
     def allocate(self: Self, nbytes: int, *, alignment: int) -> BackendAllocation:
         _validate_allocation_request(nbytes, alignment)
@@ -133,6 +142,20 @@ class CudaBackend:
         with self.launch_lock:
             self.native.set_stream(int(stream.cuda_stream))
             return fn(self.native)
+
+    def call(self: Self, name: str, args: tuple[Any, ...], stream: int) -> None:
+        """One C entry point ``name(context, *args)`` on ``stream`` (a cudaStream_t): :meth:`launch`
+        for the calls whose time is the host's."""
+        if self._closed:
+            raise DeviceClosedError("backend is closed")
+        native = self.native
+        library, handle = native.library, native.handle
+        with self.launch_lock:
+            status = library.qpucuda_context_set_stream(handle, stream or None)
+            if status == 0:
+                status = getattr(library, name)(handle, *args)
+            if status != 0:
+                native.check(status, name)
 
     def close(self: Self) -> None:
         if not self._closed:

@@ -17,6 +17,8 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Any, Self
 
+import torch
+
 from qpu_xla import _native
 from qpu_xla.device import Device
 from qpu_xla.fp8 import (
@@ -42,8 +44,6 @@ class ExpertOrder:
     position: Any
 
     def __post_init__(self: Self) -> None:
-        import torch
-
         fields = (self.offsets, self.source, self.position)
         if any(t.dtype != torch.int32 or not t.is_contiguous() for t in fields):
             raise ValueError("expert order tensors must be contiguous int32")
@@ -79,8 +79,6 @@ class ExpertOrder:
 
 def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     """Sort the choices ``[tokens, choices]`` (int32 or int64 expert ids) by expert, stably."""
-    import torch
-
     torch_device = require_cuda(device, "sort_tokens")
     if expert_ids.dtype not in (torch.int32, torch.int64) or expert_ids.dim() != 2 or expert_ids.shape[1] == 0:
         raise ValueError("sort_tokens requires int32 or int64 expert ids [tokens, choices]")
@@ -104,25 +102,21 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     return ExpertOrder(offsets, source, position)
 
 
-def _destination(out: Any, shape: tuple[int, int], dtype: Any, torch_device: Any, what: str) -> tuple[Any, int]:
-    import torch
-
+def _destination(out: Any, rows: int, width: int, read: Any, torch_device: Any, what: str) -> tuple[Any, int]:
+    """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride. It may not overlap
+    ``read``: the kernels read and write in no particular order."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=torch_device), shape[1]
-    if out.dtype != dtype:
+        return torch.empty((rows, width), dtype=read.dtype, device=torch_device), max(width, 1)
+    if out.dtype != read.dtype:
         raise ValueError(f"{what} must have the type of its source")
-    return out, check_matrix(out, torch_device, what, shape)
-
-
-def _refuse_overlap(written: Any, read: Any, what: str) -> None:
-    """The kernels read and write in no particular order."""
-    def span(t: Any) -> tuple[int, int]:
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-
-    if written.numel() and read.numel():
-        (a, a_end), (b, b_end) = span(written), span(read)
-        if a < b_end and b < a_end:
+    stride = check_matrix(out, torch_device, what, rows, width)[2]
+    if out.numel() and read.numel():
+        (begin, end), (read_begin, read_end) = (
+            (t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()) for t in (out, read)
+        )
+        if begin < read_end and read_begin < end:
             raise ValueError(f"{what} must not overlap its source")
+    return out, stride
 
 
 def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = None) -> Any:
@@ -130,39 +124,34 @@ def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = No
     row ``order.position[t, j]`` is token t. Rows from ``offsets[experts]`` on become zero."""
     torch_device = require_cuda(device, "gather_tokens")
     code = dtype_code(source.dtype, "gather_tokens source")
-    stride = check_matrix(source, torch_device, "gather_tokens source", (order.tokens, None))
     order.check(torch_device)
-    width = int(source.shape[1])
-    out, out_stride = _destination(out, (order.rows, width), source.dtype, torch_device, "gather_tokens out")
-    _refuse_overlap(out, source, "gather_tokens out")
-    if out.numel():
+    tokens, choices = order.position.shape
+    _, width, stride = check_matrix(source, torch_device, "gather_tokens source", tokens)
+    out, out_stride = _destination(out, tokens * choices, width, source, torch_device, "gather_tokens out")
+    if tokens and width:
         launch(
-            device, "qpucuda_expert_gather", source.data_ptr(), code, stride, order.tokens, order.choices, width,
-            order.position.data_ptr(), order.offsets.data_ptr(), order.experts, out.data_ptr(), out_stride,
+            device, "qpucuda_expert_gather", source.data_ptr(), code, stride, tokens, choices, width, order.position.data_ptr(),
+            order.offsets.data_ptr(), order.experts, out.data_ptr(), out_stride,
         )
     return out
 
 
-def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: Any, name: str) -> Any:
-    torch_device = require_cuda(device, name)
-    code = dtype_code(rows.dtype, f"{name} rows")
-    stride = check_matrix(rows, torch_device, f"{name} rows", (order.rows, None))
+def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: Any, torch_device: Any, name: str) -> Any:
+    code = dtype_code(rows.dtype, name)
     order.check(torch_device)
-    width = int(rows.shape[1])
-    out, out_stride = _destination(out, (order.tokens, width), rows.dtype, torch_device, f"{name} out")
-    _refuse_overlap(out, rows, f"{name} out")
-    if out.numel():
+    tokens, choices = order.position.shape
+    _, width, stride = check_matrix(rows, torch_device, name, tokens * choices)
+    out, out_stride = _destination(out, tokens, width, rows, torch_device, name)
+    if tokens and width:
         launch(
-            device, "qpucuda_expert_combine", rows.data_ptr(), code, stride, order.tokens, order.choices, width,
-            order.position.data_ptr(), None if weights is None else weights.data_ptr(), out.data_ptr(), out_stride,
+            device, "qpucuda_expert_combine", rows.data_ptr(), code, stride, tokens, choices, width, order.position.data_ptr(),
+            None if weights is None else weights.data_ptr(), out.data_ptr(), out_stride,
         )
     return out
 
 
 def _check_weights(weights: Any, order: ExpertOrder, torch_device: Any, name: str) -> None:
-    import torch
-
-    if weights.dtype != torch.float32 or tuple(weights.shape) != (order.tokens, order.choices) or not weights.is_contiguous():
+    if weights.dtype != torch.float32 or weights.shape != order.position.shape or not weights.is_contiguous():
         raise ValueError(f"{name} requires contiguous float32 weights [tokens, choices]")
     if weights.device != torch_device:
         raise ValueError(f"{name} weights must be on {torch_device}")
@@ -171,40 +160,39 @@ def _check_weights(weights: Any, order: ExpertOrder, torch_device: Any, name: st
 def gather_tokens_backward(device: Device, grad_rows: Any, order: ExpertOrder, out: Any = None) -> Any:
     """The tokens' gradient ``[T, H]`` from the sorted rows' ``[T * choices, H]``: the sum over a
     token's choices in fp32, rounded once. Dropped choices add nothing."""
-    return _combine(device, grad_rows, None, order, out, "gather_tokens_backward")
+    return _combine(device, grad_rows, None, order, out, require_cuda(device, "gather_tokens_backward"), "gather_tokens_backward")
 
 
 def combine_tokens(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: Any = None) -> Any:
     """Sorted rows ``[T * choices, H]`` back to tokens: ``out[t] = sum_j weights[t, j] *
     rows[position[t, j]]`` in fp32, in the order of j, rounded once. A dropped choice adds nothing,
     whatever its weight."""
-    _check_weights(weights, order, require_cuda(device, "combine_tokens"), "combine_tokens")
-    return _combine(device, rows, weights, order, out, "combine_tokens")
+    torch_device = require_cuda(device, "combine_tokens")
+    _check_weights(weights, order, torch_device, "combine_tokens")
+    return _combine(device, rows, weights, order, out, torch_device, "combine_tokens")
 
 
 def combine_tokens_backward(device: Device, rows: Any, weights: Any, grad: Any, order: ExpertOrder) -> tuple[Any, Any]:
     """The gradients of :func:`combine_tokens` from that of its result, ``grad [T, H]``: of the rows
     (``weights[t, j] * grad[t]`` at ``position[t, j]``, zero where no choice is) and of the weights
     (``<rows[position[t, j]], grad[t]>`` in fp32, zero where dropped)."""
-    import torch
-
     name = "combine_tokens_backward"
     torch_device = require_cuda(device, name)
-    code = dtype_code(rows.dtype, f"{name} rows")
+    code = dtype_code(rows.dtype, name)
     if grad.dtype != rows.dtype:
         raise ValueError(f"{name} grad must have the type of the rows")
-    stride = check_matrix(rows, torch_device, f"{name} rows", (order.rows, None))
-    width = int(rows.shape[1])
-    grad_stride = check_matrix(grad, torch_device, f"{name} grad", (order.tokens, width))
     order.check(torch_device)
+    tokens, choices = order.position.shape
+    _, width, stride = check_matrix(rows, torch_device, f"{name} rows", tokens * choices)
+    grad_stride = check_matrix(grad, torch_device, f"{name} grad", tokens, width)[2]
     _check_weights(weights, order, torch_device, name)
-    grad_rows = torch.empty((order.rows, width), dtype=rows.dtype, device=torch_device)
-    grad_weights = torch.empty((order.tokens, order.choices), dtype=torch.float32, device=torch_device)
-    if grad_rows.numel():
+    grad_rows = torch.empty((tokens * choices, width), dtype=rows.dtype, device=torch_device)
+    grad_weights = torch.empty((tokens, choices), dtype=torch.float32, device=torch_device)
+    if tokens and width:
         launch(
-            device, "qpucuda_expert_combine_backward", rows.data_ptr(), code, stride, grad.data_ptr(), grad_stride, order.tokens,
-            order.choices, width, order.position.data_ptr(), order.offsets.data_ptr(), order.experts, weights.data_ptr(),
-            grad_rows.data_ptr(), width, grad_weights.data_ptr(),
+            device, "qpucuda_expert_combine_backward", rows.data_ptr(), code, stride, grad.data_ptr(), grad_stride, tokens, choices, width,
+            order.position.data_ptr(), order.offsets.data_ptr(), order.experts, weights.data_ptr(), grad_rows.data_ptr(), width,
+            grad_weights.data_ptr(),
         )
     else:
         grad_weights.zero_()
@@ -234,8 +222,6 @@ class FP8ExpertsFFN:
     def forward(self: Self, source: Any, expert_ids: Any, weights: Any) -> Any:
         """Tokens ``[T, H]``, their expert ids ``[T, choices]`` and float32 weights, to ``[T, H_out]``
         of the source's type."""
-        import torch
-
         order = sort_tokens(self.device, expert_ids, self.experts)
         hidden = self.gate_up.forward_tokens(source, order, dtype=torch.float32)
         rows = self.down.forward(hidden, order.offsets, dtype=source.dtype)

@@ -24,6 +24,7 @@ from dataclasses import dataclass
 from typing import Any, Self
 
 import numpy as np
+import torch
 
 from qpu_xla import _native
 from qpu_xla.device import Device
@@ -36,15 +37,12 @@ FP8_GROUP = 128
 MAX_EXPERTS = 1024
 
 
-def _dtype_codes() -> dict[Any, int]:
-    import torch
-
-    return {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
+_DTYPE_CODES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 
 
 def dtype_code(dtype: Any, what: str) -> int:
     """``qpucuda_dtype`` of an activation or output type."""
-    code = _dtype_codes().get(dtype)
+    code = _DTYPE_CODES.get(dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, bfloat16 or float16")
     return code
@@ -61,28 +59,29 @@ def require_cuda(device: Device, what: str) -> Any:
     return device.backend.torch_device  # type: ignore[attr-defined]
 
 
-def check_matrix(tensor: Any, torch_device: Any, what: str, shape: tuple[int | None, int | None] = (None, None)) -> int:
-    """A rank-2 tensor on ``torch_device`` with unit inner stride and the given extents; its row stride."""
-    if tensor.dim() != 2 or any(want is not None and have != want for have, want in zip(tensor.shape, shape)):
-        raise ValueError(f"{what} must be rank-2 {list(shape)}, not {list(tensor.shape)}")
+def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = None, cols: int | None = None) -> tuple[int, int, int]:
+    """A rank-2 tensor on ``torch_device`` with unit inner stride and the given extents: its rows,
+    columns and row stride (a single row's stride is its width, whatever the tensor says)."""
+    shape = tensor.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}], not {list(shape)}")
     if tensor.device != torch_device:
         raise ValueError(f"{what} must be on {torch_device}, the device it is used with")
-    if tensor.shape[1] > 1 and tensor.stride(1) != 1:
+    have_rows, have_cols = shape
+    stride, inner = tensor.stride()
+    if inner != 1 and have_cols > 1:
         raise ValueError(f"{what} must be row-major (unit inner stride)")
-    if tensor.shape[0] <= 1:
-        return int(max(tensor.shape[1], 1))
-    if tensor.stride(0) < tensor.shape[1]:
+    if have_rows <= 1:
+        return have_rows, have_cols, max(have_cols, 1)
+    if stride < have_cols:
         raise ValueError(f"{what} must not have overlapping rows")
-    return int(tensor.stride(0))
+    return have_rows, have_cols, stride
 
 
-def launch(device: Device, name: str, *args: Any, stream: Any = None) -> None:
-    """Call one libqpucuda entry point on ``stream`` (default: the device's current stream)."""
-    import torch
-
+def launch(device: Device, name: str, *args: Any, stream: int | None = None) -> None:
+    """Call one libqpucuda entry point on ``stream`` (a cudaStream_t; default: the device's current stream)."""
     backend = device.backend
-    stream = torch.cuda.current_stream(backend.torch_device) if stream is None else stream  # type: ignore[attr-defined]
-    backend.launch(stream, lambda native: native.check(getattr(native.library, name)(native.handle, *args), name))  # type: ignore[attr-defined]
+    backend.call(name, args, backend.current_stream_handle if stream is None else stream)  # type: ignore[attr-defined]
 
 
 @dataclass(frozen=True, slots=True)
@@ -93,8 +92,6 @@ class QuantizedRowsFP8:
     scales: Any
 
     def __post_init__(self: Self) -> None:
-        import torch
-
         if self.values.dim() != 2 or self.values.dtype != torch.float8_e4m3fn:
             raise ValueError("quantized rows must be rank-2 float8_e4m3fn")
         if tuple(self.scales.shape) != (self.values.shape[0], groups_of(self.values.shape[1])) or self.scales.dtype != torch.float32:
@@ -121,8 +118,6 @@ class QuantizedBlocksFP8:
     scales: Any
 
     def __post_init__(self: Self) -> None:
-        import torch
-
         if self.values.dim() not in (2, 3) or self.values.dtype != torch.float8_e4m3fn or 0 in self.values.shape:
             raise ValueError("quantized weights must be non-empty rank-2 or rank-3 float8_e4m3fn")
         *batch, rows, cols = self.values.shape
@@ -144,8 +139,6 @@ class QuantizedBlocksFP8:
 
 def quantize_blocks_fp8(device: Device, weight: Any) -> QuantizedBlocksFP8:
     """Quantize weights ``[N, K]`` or ``[E, N, K]`` (float32, bfloat16 or float16 CUDA tensor) per 128 x 128 block."""
-    import torch
-
     torch_device = require_cuda(device, "quantize_blocks_fp8")
     code = dtype_code(weight.dtype, "quantize_blocks_fp8 weight")
     if weight.dim() not in (2, 3) or 0 in weight.shape:
@@ -173,32 +166,25 @@ def _quantize_desc(
     )
 
 
-def _columns(source: Any, gated: bool, what: str) -> int:
-    if source.dim() != 2 or source.shape[1] == 0 or (gated and source.shape[1] % 2):
-        raise ValueError(f"{what} must be rank-2 [rows, {'2 * ' if gated else ''}columns]")
-    return int(source.shape[1]) // (2 if gated else 1)
-
-
 def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> QuantizedRowsFP8:
     """Quantize rows ``[M, K]`` (float32, bfloat16 or float16) with one scale per 128 columns.
 
     ``gated``: the source is ``[M, 2 K]``, gate then up, and ``silu(gate) * up`` is quantized,
     computed in fp32. The values are a view of rows padded to 16 bytes.
     """
-    import torch
-
     torch_device = require_cuda(device, "quantize_rows_fp8")
     dtype_code(source.dtype, "quantize_rows_fp8 source")
-    cols = _columns(source, gated, "quantize_rows_fp8 source")
-    stride = check_matrix(source, torch_device, "quantize_rows_fp8 source")
-    rows = int(source.shape[0])
+    rows, cols, stride = check_matrix(source, torch_device, "quantize_rows_fp8 source")
+    if cols == 0 or (gated and cols % 2):
+        raise ValueError("quantize_rows_fp8 source must have columns, an even number of them when gated")
+    cols = cols // 2 if gated else cols
     q_stride = (cols + 15) // 16 * 16
     values = torch.empty((rows, q_stride), dtype=torch.float8_e4m3fn, device=torch_device)
     scales = torch.empty((rows, groups_of(cols)), dtype=torch.float32, device=torch_device)
     if rows:
         desc = _quantize_desc(source, stride, cols, gated, rows, values.data_ptr(), q_stride, scales.data_ptr(), (groups_of(cols), 1))
         launch(device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
-    return QuantizedRowsFP8(values[:, :cols], scales)
+    return QuantizedRowsFP8(values if q_stride == cols else values[:, :cols], scales)
 
 
 class _PreparedFP8:
@@ -210,14 +196,14 @@ class _PreparedFP8:
     _name = "prepared FP8 linear"
 
     def __init__(self: Self, device: Device, weight: QuantizedBlocksFP8, bias: Any, gated: bool) -> None:
-        import torch
-
         self._torch_device = require_cuda(device, type(self).__name__)
         self.device = device
         self.gated = bool(gated)
         *batch, self.output_count, self.input_count = weight.shape
         self.experts = batch[0] if batch else 0
-        padded = (self.input_count + 15) // 16 * 16
+        self._source_columns = self.input_count * (2 if gated else 1)
+        self._groups = groups_of(self.input_count)
+        self._padded = padded = (self.input_count + 15) // 16 * 16
         self._values = torch.zeros((*batch, self.output_count, padded), dtype=torch.uint8, device=self._torch_device)
         self._values[..., : self.input_count].copy_(weight.values.view(torch.uint8))
         self._scales = weight.scales.to(self._torch_device).clone(memory_format=torch.contiguous_format)
@@ -227,6 +213,9 @@ class _PreparedFP8:
             if tuple(bias.shape) != (self.output_count,):
                 raise ValueError("bias must have one fp32 value per output feature")
             self._bias = bias.to(self._torch_device, torch.float32).clone(memory_format=torch.contiguous_format)
+        self._values_address = self._values.data_ptr()
+        self._scales_address = self._scales.data_ptr()
+        self._bias_address = None if self._bias is None else self._bias.data_ptr()
         torch.cuda.current_stream(self._torch_device).synchronize()
         self._closed = False
 
@@ -245,8 +234,6 @@ class _PreparedFP8:
         """Wait for the device and release the weight."""
         if self._closed:
             return
-        import torch
-
         torch.cuda.synchronize(self._torch_device)
         self._values = self._scales = self._bias = None
         self._closed = True
@@ -257,8 +244,6 @@ class _PreparedFP8:
         return sum(t.numel() * t.element_size() for t in (self._values, self._scales, self._bias) if t is not None)
 
     def _output(self: Self, rows: int, out: Any, dtype: Any, default: Any) -> tuple[Any, int]:
-        import torch
-
         if out is None:
             dtype = default if dtype is None else dtype
             dtype_code(dtype, f"{self._name} output")
@@ -266,56 +251,48 @@ class _PreparedFP8:
         if dtype is not None and out.dtype != dtype:
             raise ValueError(f"{self._name} out and dtype differ")
         dtype_code(out.dtype, f"{self._name} output")
-        return out, check_matrix(out, self._torch_device, f"{self._name} output", (rows, self.output_count))
+        return out, check_matrix(out, self._torch_device, f"{self._name} output", rows, self.output_count)[2]
 
-    def _gemm(
+    def _gemm_desc(
         self: Self, a: int, a_stride: int, a_scales: int, scale_strides: tuple[int, int], rows: int, out_address: int, out_code: int,
-        out_stride: int, offsets: Any = None, settled: bool = False, stream: Any = None,
-    ) -> None:
-        desc = _native.Fp8GemmDesc(
-            a, a_stride, a_scales, *scale_strides, self._values.data_ptr(), self._values.stride(-2), self._scales.data_ptr(),
-            None if self._bias is None else self._bias.data_ptr(), rows, self.output_count, self.input_count, self.experts,
-            None if offsets is None else offsets.data_ptr(), out_address, out_code, out_stride, int(settled),
+        out_stride: int, offsets: int | None = None, settled: bool = False,
+    ) -> Any:
+        return _native.Fp8GemmDesc(
+            a, a_stride, a_scales, *scale_strides, self._values_address, self._padded, self._scales_address, self._bias_address, rows,
+            self.output_count, self.input_count, self.experts, offsets, out_address, out_code, out_stride, settled,
         )
-        launch(self.device, "qpucuda_fp8_gemm", ctypes.byref(desc), stream=stream)
 
-    def _scratch(self: Self, rows: int) -> tuple[Any, int, int, int]:
-        """One allocation for the quantized rows and, behind them, their scales (group-major: a warp
-        of the product reads the scales of neighbouring rows)."""
-        import torch
-
-        stride = (self.input_count + 15) // 16 * 16
-        scratch = torch.empty(rows * stride + 4 * rows * groups_of(self.input_count), dtype=torch.uint8, device=self._torch_device)
-        return scratch, scratch.data_ptr(), stride, scratch.data_ptr() + rows * stride
-
-    def _quantize_and_multiply(
-        self: Self, source: Any, stride: int, rows: int, out: Any, out_stride: int, offsets: Any = None, row_source: Any = None, row_divisor: int = 1
+    def _linear(
+        self: Self, source: int, source_code: int, source_rows: int, stride: int, rows: int, out: int, out_code: int, out_stride: int,
+        offsets: int | None = None, row_source: int | None = None, row_divisor: int = 1, stream: int | None = None,
     ) -> None:
-        scratch, values, q_stride, scales = self._scratch(rows)
-        desc = _quantize_desc(source, stride, self.input_count, self.gated, rows, values, q_stride, scales, (1, rows), row_source, row_divisor)
-        launch(self.device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
-        # The weight and the offsets are older than the quantizer's launch: the product reads them early.
-        self._gemm(
-            values, q_stride, scales, (1, rows), rows, out.data_ptr(), dtype_code(out.dtype, "output"), out_stride,
-            offsets=offsets, settled=True,
+        """Quantize and multiply. One scratch allocation, for this call alone: the quantized rows and,
+        behind them, their scales, group-major (a warp of the product reads neighbouring rows' scales).
+        The weight is older than the quantizer's launch, so the product may read it early; so are the
+        offsets."""
+        padded = self._padded
+        scratch = torch.empty(rows * (padded + 4 * self._groups), dtype=torch.uint8, device=self._torch_device)
+        values = scratch.data_ptr()
+        scales = values + rows * padded
+        quantize = _native.Fp8QuantizeDesc(
+            source, source_code, stride, rows, self.input_count, self.gated, row_source, row_divisor, source_rows, values, padded, scales, 1, rows
         )
-        del scratch
+        gemm = self._gemm_desc(values, padded, scales, (1, rows), rows, out, out_code, out_stride, offsets, True)
+        launch(self.device, "qpucuda_fp8_linear", ctypes.byref(quantize), ctypes.byref(gemm), stream=stream)
 
-    def _check_source(self: Self, source: Any) -> int:
-        dtype_code(source.dtype, f"{self._name} source")
-        width = self.input_count * (2 if self.gated else 1)
-        return check_matrix(source, self._torch_device, f"{self._name} source", (None, width))
+    def _check_source(self: Self, source: Any) -> tuple[int, int, int]:
+        """Rows, row stride and type code."""
+        code = dtype_code(source.dtype, f"{self._name} source")
+        rows, _, stride = check_matrix(source, self._torch_device, f"{self._name} source", None, self._source_columns)
+        return rows, stride, code
 
     def _check_rows(self: Self, rows: QuantizedRowsFP8) -> tuple[int, int, tuple[int, int]]:
         values = rows.values
-        count = int(values.shape[0])
-        stride = check_matrix(values, self._torch_device, f"{self._name} quantized rows", (None, self.input_count))
+        count, _, stride = check_matrix(values, self._torch_device, f"{self._name} quantized rows", None, self.input_count)
         if count <= 1:
-            stride = (self.input_count + 15) // 16 * 16
+            stride = self._padded
         if stride % 16 or values.data_ptr() % 16:
             raise ValueError(f"{self._name} quantized rows must start on 16-byte boundaries")
-        if min(rows.scales.stride()) < 0:
-            raise ValueError(f"{self._name} scales must not have negative strides")
         return count, stride, (int(rows.scales.stride(0)), int(rows.scales.stride(1)))
 
 
@@ -335,57 +312,44 @@ class PreparedFP8Linear(_PreparedFP8):
         """Rows ``[M, K]`` (float32, bfloat16 or float16) to ``[M, N]`` of ``dtype`` (default: the
         source's type, or ``out``'s)."""
         self._require_open()
-        stride = self._check_source(source)
-        rows = int(source.shape[0])
+        rows, stride, code = self._check_source(source)
         out, out_stride = self._output(rows, out, dtype, source.dtype)
         if rows:
-            self._quantize_and_multiply(source, stride, rows, out, out_stride)
+            self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride)
         return out
 
     def forward_quantized(self: Self, rows: QuantizedRowsFP8, out: Any = None, *, dtype: Any = None) -> Any:
         """The product alone, over rows quantized before (:func:`quantize_rows_fp8`); ``dtype``
         defaults to float32."""
-        import torch
-
         self._require_open()
         count, stride, scale_strides = self._check_rows(rows)
         out, out_stride = self._output(count, out, dtype, torch.float32)
         if count:
-            self._gemm(
-                rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(),
-                dtype_code(out.dtype, "output"), out_stride,
+            gemm = self._gemm_desc(
+                rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride
             )
+            launch(self.device, "qpucuda_fp8_gemm", ctypes.byref(gemm))
         return out
 
     def execute(self: Self, destination: Tensor, source: Tensor, *, queue: Queue, wait_for: Iterable[Event] = ()) -> Event:
         """The same on a queue, float32 tensors of the plan's device (as ``PreparedW8A8Linear.execute``)."""
-        import torch
-
         self._require_open()
         if queue.device is not self.device or source.buffer.device is not self.device or destination.buffer.device is not self.device:
             raise DependencyError("prepared FP8 linear queue and tensors must belong to the plan device")
         if source.dtype != np.dtype(np.float32) or destination.dtype != np.dtype(np.float32):
             raise ValueError("prepared FP8 linear requires float32 source and destination")
-        width = self.input_count * (2 if self.gated else 1)
-        if len(source.shape) != 2 or source.shape[1] != width or destination.shape != (source.shape[0], self.output_count):
+        if len(source.shape) != 2 or source.shape[1] != self._source_columns or destination.shape != (source.shape[0], self.output_count):
             raise ValueError("prepared FP8 linear source and destination shapes do not align")
         if source.strides[1] != 4 or destination.strides[1] != 4:
             raise ValueError("prepared FP8 linear requires unit inner strides")
         rows = int(source.shape[0])
 
         def executor(backend: Any, args: tuple[Any, ...], grid: tuple[int, int, int], stream: Any) -> None:
-            with torch.cuda.stream(stream):
-                scratch, values, q_stride, scales = self._scratch(rows)
-                desc = _native.Fp8QuantizeDesc(
-                    source.address, _native.DTYPE_F32, source.row_stride_elements, rows, self.input_count, int(self.gated), None, 1, rows,
-                    values, q_stride, scales, 1, rows,
+            with torch.cuda.stream(stream):  # the scratch belongs to the queue's stream
+                self._linear(
+                    source.address, _native.DTYPE_F32, rows, source.row_stride_elements, rows, destination.address, _native.DTYPE_F32,
+                    destination.row_stride_elements, stream=stream.cuda_stream,
                 )
-                launch(self.device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc), stream=stream)
-                self._gemm(
-                    values, q_stride, scales, (1, rows), rows, destination.address, _native.DTYPE_F32, destination.row_stride_elements,
-                    settled=True, stream=stream,
-                )
-                del scratch
 
         return queue.submit(
             Kernel("cuda.fp8_linear", executor), (), wait_for=wait_for,
@@ -407,8 +371,6 @@ class PreparedFP8Experts(_PreparedFP8):
         super().__init__(device, weight, None, gated)
 
     def _check_offsets(self: Self, offsets: Any) -> None:
-        import torch
-
         if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.experts + 1,) or not offsets.is_contiguous():
             raise ValueError("prepared FP8 experts need contiguous int32 offsets [experts + 1]")
         if offsets.device != self._torch_device:
@@ -418,25 +380,27 @@ class PreparedFP8Experts(_PreparedFP8):
         """Rows ``[R, K]``, those of expert e at ``offsets[e] .. offsets[e + 1]`` (ascending int32 on
         the GPU, clamped to ``[0, R]``), to ``[R, N]``. Rows from ``offsets[E]`` on become zero."""
         self._require_open()
-        stride = self._check_source(source)
+        rows, stride, code = self._check_source(source)
         self._check_offsets(offsets)
-        rows = int(source.shape[0])
         out, out_stride = self._output(rows, out, dtype, source.dtype)
         if rows:
-            self._quantize_and_multiply(source, stride, rows, out, out_stride, offsets)
+            self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, offsets.data_ptr())
         return out
 
     def forward_tokens(self: Self, tokens: Any, order: Any, out: Any = None, *, dtype: Any = None) -> Any:
         """:meth:`forward` of the tokens ``[T, K]`` in expert order, without the sorted copy: row r is
         quantized straight from token ``order.source[r] // choices``. ``[T * choices, N]``."""
         self._require_open()
-        stride = self._check_source(tokens)
+        tokens_count, stride, code = self._check_source(tokens)
         self._check_offsets(order.offsets)
-        order.check(self._torch_device, tokens=int(tokens.shape[0]))
-        rows = int(order.source.shape[0])
+        order.check(self._torch_device, tokens=tokens_count)
+        rows = order.rows
         out, out_stride = self._output(rows, out, dtype, tokens.dtype)
         if rows:
-            self._quantize_and_multiply(tokens, stride, rows, out, out_stride, order.offsets, order.source, order.choices)
+            self._linear(
+                tokens.data_ptr(), code, tokens_count, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, order.offsets.data_ptr(),
+                order.source.data_ptr(), order.choices,
+            )
         return out
 
 
