@@ -79,24 +79,33 @@ struct RowsParams {
     size_t scale_row_stride, scale_group_stride;
 };
 
-// kVector elements at x as fp32, zero from `remaining` of them on.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void load_row(const T *x, uint32_t remaining, float (&v)[kVector<T>]) {
-    if (VECTOR) {
-        Vector<T> raw;
-        raw.bits = make_uint4(0, 0, 0, 0);
-        if (remaining >= static_cast<uint32_t>(kVector<T>)) {
-            raw.bits = load_stream16(x);
+// kVector elements at x, zero from `remaining` of them on. Full vectors first and the ragged end of a
+// row in a pass of its own, so that nothing stands between the loads of several steps.
+template <typename T, bool VECTOR, int STEPS>
+__device__ __forceinline__ void load_steps(const T *x, uint32_t remaining, uint32_t step, Vector<T> (&raw)[STEPS]) {
+    constexpr uint32_t kItems = kVector<T>;
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const uint32_t left = remaining > u * step ? remaining - u * step : 0u;
+        raw[u].bits = make_uint4(0, 0, 0, 0);
+        if (VECTOR) {
+            if (left >= kItems) raw[u].bits = load_stream16(x + u * step);
         } else {
 #pragma unroll
-            for (int i = 0; i < kVector<T>; ++i)
-                if (static_cast<uint32_t>(i) < remaining) raw.items[i] = x[i];
+            for (uint32_t i = 0; i < kItems; ++i)
+                if (i < left) raw[u].items[i] = x[u * step + i];
         }
+    }
+    if (VECTOR && remaining % step != 0 && remaining % step < kItems) {
 #pragma unroll
-        for (int i = 0; i < kVector<T>; ++i) v[i] = to_float(raw.items[i]);
-    } else {
+        for (int u = 0; u < STEPS; ++u) {
+            const uint32_t left = remaining > u * step ? remaining - u * step : 0u;
+            if (left < kItems) {
 #pragma unroll
-        for (int i = 0; i < kVector<T>; ++i) v[i] = static_cast<uint32_t>(i) < remaining ? to_float(x[i]) : 0.0f;
+                for (uint32_t i = 0; i < kItems; ++i)
+                    if (i < left) raw[u].items[i] = x[u * step + i];
+            }
+        }
     }
 }
 
@@ -136,33 +145,29 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
         const bool present = source < params.source_rows;
         const uint32_t column0 = chunk * (STEPS * kPerStep * 128u) + inner;
         const T *x = static_cast<const T *>(params.x) + (present ? static_cast<size_t>(source) * params.x_stride : 0) + column0;
-        float v[STEPS][kVector<T>];
-#pragma unroll
-        for (int u = 0; u < STEPS; ++u) {
-            constexpr int kStep = kPerStep * 128;
-            const uint32_t remaining = present && column0 + u * kStep < params.cols ? params.cols - column0 - u * kStep : 0u;
-            load_row<T, VECTOR>(x + u * kStep, remaining, v[u]);
-            if (GATED) {
-                float up[kVector<T>];
-                load_row<T, VECTOR>(x + params.cols + u * kStep, remaining, up);
-#pragma unroll
-                for (int i = 0; i < kVector<T>; ++i) v[u][i] = silu_times(v[u][i], up[i]);
-            }
-        }
+        constexpr uint32_t kStep = kPerStep * 128;
+        const uint32_t remaining = present && column0 < params.cols ? params.cols - column0 : 0u;
+        Vector<T> raw[STEPS], raw_up[GATED ? STEPS : 1];
+        load_steps<T, VECTOR>(x, remaining, kStep, raw);
+        if constexpr (GATED) load_steps<T, VECTOR>(x + params.cols, remaining, kStep, raw_up);
         uint8_t *q = params.q + static_cast<size_t>(row) * params.q_stride + column0;
         const uint32_t group0 = column0 / 128u;
         float *scales = params.scales + static_cast<size_t>(row) * params.scale_row_stride + static_cast<size_t>(group0) * params.scale_group_stride;
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
-            float amax = 0.0f;
+            float v[kVector<T>], amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kVector<T>; ++i) amax = max_nan(amax, fabsf(v[u][i]));
+            for (int i = 0; i < kVector<T>; ++i) {
+                v[i] = to_float(raw[u].items[i]);
+                if constexpr (GATED) v[i] = silu_times(v[i], to_float(raw_up[u].items[i]));
+                amax = max_nan(amax, fabsf(v[i]));
+            }
 #pragma unroll
             for (int offset = kLanes / 2; offset > 0; offset >>= 1)
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, offset));
             const float scale = group_scale(amax);
             uint32_t packed[kVector<T> / 4];
-            quantize_values(v[u], scale, packed);
+            quantize_values(v, scale, packed);
             if (column0 + u * (kPerStep * 128u) < params.cols) {
                 // q rows are padded to 16 bytes, so a vector that starts below cols fits
                 if constexpr (kVector<T> == 8) {
