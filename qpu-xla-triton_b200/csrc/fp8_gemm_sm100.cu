@@ -698,6 +698,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         uint4 *buffer_out = reinterpret_cast<uint4 *>(store + worker * kWideStoreBytes);
         const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + half * (kWideN / 2);
         const bool vector = (reinterpret_cast<uintptr_t>(params.out) & 15u) == 0 && params.out_stride * sizeof(Out) % 16 == 0;
+        const uint32_t tmem_full0 = smem_u32(&control->tmem_full[0]);
         uint32_t buffer = 0, buffer_phase = 0;
         for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
             const WideTile tile = locate(params, first_tile, n_tiles, group_rows, t);
@@ -707,14 +708,21 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             const bool block_inside = n0 < params.n;
             const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n0 / kBlockN) * params.k_blocks;
             const float *a_scales = params.a_scales + static_cast<size_t>(row0 + lane) * params.a_scale_row_stride;
-            auto fetch = [&](uint32_t kb, float &a, float &w) {
-                const bool inside = kb < params.k_blocks;
-                a = inside && row_inside ? a_scales[static_cast<size_t>(kb) * params.a_scale_group_stride] : 0.0f;
-                w = inside && block_inside ? __ldg(w_scales + kb) : 0.0f;
+            // A block's factor is fetched two blocks ahead; the fetches of the last two repeat the last block.
+            const float *a_at = row_inside ? a_scales : params.a_scales;
+            const float *w_at = block_inside ? w_scales : params.w_scales;
+            uint32_t fetched = 0;
+            auto fetch = [&](float &a, float &w) {
+                a = *a_at;
+                w = __ldg(w_at);
+                if (++fetched < params.k_blocks) {
+                    a_at += params.a_scale_group_stride;
+                    ++w_at;
+                }
             };
             float a_now, w_now, a_next, w_next;
-            fetch(0, a_now, w_now);
-            fetch(1, a_next, w_next);
+            fetch(a_now, w_now);
+            fetch(a_next, w_next);
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
@@ -726,11 +734,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pack2(r[2 * i], r[2 * i + 1]), factors, acc[c * 16 + i]);
             };
             auto arrived = [&]() {
-                bool full = true;
-                if (lane == 0) full = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
-                full = __shfl_sync(0xFFFFFFFFu, full ? 1 : 0, 0) != 0;
+                const bool full = wait_bounded(tmem_full0 + buffer * 8u, buffer_phase, &control->abort_flag, params.error_word);
+                const bool all = __all_sync(0xFFFFFFFFu, full) != 0;
                 tc_fence_after();
-                return full;
+                return all;
             };
             bool ok = arrived();
             if (ok) tmem_load_x32(taddr + buffer * kWideN, even);
@@ -739,7 +746,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 const uint64_t factors = pack2(factor, factor);
                 a_now = a_next;
                 w_now = w_next;
-                fetch(kb + 2, a_next, w_next);
+                fetch(a_next, w_next);
                 const uint32_t block = taddr + buffer * kWideN;
                 tmem_wait_load(even);
                 tmem_load_x32(block + 32, odd);

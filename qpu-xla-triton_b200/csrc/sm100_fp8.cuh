@@ -65,12 +65,12 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[N]) {
 }
 
 // fp32 pairs in one register pair: each half rounds as the scalar fma does, two per instruction.
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-    return static_cast<uint64_t>(__float_as_uint(lo)) | (static_cast<uint64_t>(__float_as_uint(hi)) << 32);
-}
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    return static_cast<uint64_t>(lo) | (static_cast<uint64_t>(hi) << 32);
+    uint64_t pair;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pair) : "r"(lo), "r"(hi));
+    return pair;
 }
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) { return pack2(__float_as_uint(lo), __float_as_uint(hi)); }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
