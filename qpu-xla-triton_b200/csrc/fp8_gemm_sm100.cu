@@ -11,6 +11,7 @@
 // Rows (tokens) are the narrow side here: the weight is the M = 128 operand and NT rows are the N
 // operand, so a few tokens cost a tile of NT = 16 and not 128. Tensor memory lane = output column,
 // tensor memory column = row.
+#include <atomic>
 #include <cstring>
 
 #include "element.cuh"
@@ -449,7 +450,6 @@ constexpr int kWideM = 128;
 constexpr int kWideN = 256;
 constexpr uint64_t kGroupBytes = 40ull << 20;  // rows of a group of tiles: part of the 126 MB L2
 constexpr uint64_t kGroupRows = 16;
-constexpr int kWideStages = 4;
 constexpr int kWideWarps = 8;  // epilogue: lane quarters x column halves
 constexpr int kWideThreads = 128 + 32 * kWideWarps;
 // Registers a thread: an epilogue thread holds 128 sums and 32 loaded values, the other four warps
@@ -458,13 +458,24 @@ constexpr int kWideThreads = 128 + 32 * kWideWarps;
 constexpr int kWideFewRegisters = 40;
 constexpr int kWideManyRegisters = 232;
 static_assert(128 * kWideFewRegisters + 256 * kWideManyRegisters <= 384 * 168, "register hand-over");
-constexpr int kWideABytes = kWideM * kBlockK;
-constexpr int kWideWBytes = kWideN * kBlockK;
-constexpr int kWideStageBytes = kWideABytes + kWideWBytes;
+// A stage per CTA. Alone: 128 rows and 256 weight rows. In a pair (cluster of two, tcgen05
+// cta_group::2, a tile of 256 x 256): 128 rows and this CTA's half of the weight rows, which both
+// CTAs' MMAs read; a third less shared-memory traffic per product.
+template <bool PAIR>
+struct Wide {
+    static constexpr int kRows = PAIR ? 2 * kWideM : kWideM;  // of a tile
+    static constexpr int kStages = PAIR ? 6 : 4;
+    static constexpr int kABytes = kWideM * kBlockK;
+    static constexpr int kWBytes = (PAIR ? kWideN / 2 : kWideN) * kBlockK;
+    static constexpr int kStageBytes = kABytes + kWBytes;
+};
 constexpr int kWideStoreBytes = 2048;  // per epilogue warp: 32 rows x 64 bytes on their way out
 constexpr size_t kWideTableBytes = (QPUCUDA_MAX_EXPERTS + 1) * sizeof(uint32_t);
-constexpr size_t kWideSharedBytes = kWideStages * kWideStageBytes + kWideWarps * kWideStoreBytes + kWideTableBytes + 256 + 1024;
-static_assert(kWideSharedBytes <= 227 * 1024, "shared memory");
+template <bool PAIR>
+constexpr size_t wide_shared_bytes() {
+    return Wide<PAIR>::kStages * Wide<PAIR>::kStageBytes + kWideWarps * kWideStoreBytes + kWideTableBytes + 256 + 1024;
+}
+static_assert(wide_shared_bytes<false>() <= 227 * 1024 && wide_shared_bytes<true>() <= 227 * 1024, "shared memory");
 
 struct WideTile {
     uint32_t expert, row0, row_end, n0;
@@ -485,6 +496,7 @@ __device__ __forceinline__ void order_tile(uint32_t tile, uint32_t m_blocks, uin
 }
 
 // first_tile[e]: tiles of the experts before e. The last e with first_tile[e] <= tile holds it.
+template <uint32_t HEIGHT>
 __device__ __forceinline__ WideTile locate(const GemmParams &params, const uint32_t *first_tile, uint32_t n_tiles,
                                            uint32_t group_rows, uint32_t tile) {
     WideTile result;
@@ -507,9 +519,9 @@ __device__ __forceinline__ WideTile locate(const GemmParams &params, const uint3
         end = static_cast<uint32_t>(min(max(params.offsets[low_e + 1], static_cast<int32_t>(begin)), rows));
     }
     uint32_t m_block, n_tile;
-    order_tile(local, (end - begin + kWideM - 1) / kWideM, n_tiles, group_rows, m_block, n_tile);
-    result.row0 = begin + m_block * kWideM;
-    result.row_end = min(end, result.row0 + kWideM);
+    order_tile(local, (end - begin + HEIGHT - 1) / HEIGHT, n_tiles, group_rows, m_block, n_tile);
+    result.row0 = begin + m_block * HEIGHT;
+    result.row_end = min(end, result.row0 + HEIGHT);
     result.n0 = n_tile * kWideN;
     return result;
 }
@@ -546,45 +558,57 @@ __device__ __forceinline__ void store_chunk(uint4 *buffer, const float (&v)[64 /
     }
 }
 
-// Persistent: one CTA per SM walks tiles blockIdx.x, + gridDim.x, ...
-//   warp 0   copies: a row box and two weight boxes per stage
-//   warp 1   tensor memory and MMA: 4 MMAs per stage into one of two accumulators
+// Persistent: one CTA (or pair) per SM (or two) walks tiles 0, 1, ... in steps of the CTAs or pairs.
+//   warp 0   copies: a row box and the weight boxes per stage (a pair's bytes all complete on rank 0's barriers)
+//   warp 1   tensor memory and MMA (rank 0 alone in a pair): 4 MMAs per stage into one of two accumulators
 //   warp 2   the experts' table of tiles, warp 3 nothing
 //   4 to 11  each block's accumulator into registers, scaled; at the tile's end the store
-template <typename Out>
+template <typename Out, bool PAIR>
 __global__ void __launch_bounds__(kWideThreads, 1)
     fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                          const GemmParams params, uint32_t n_tiles, uint32_t group_rows) {
-    using Ctl = Control<kWideStages, 2>;
+    using Shape = Wide<PAIR>;
+    constexpr int kStages = Shape::kStages;
+    using Ctl = Control<kStages, 2>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *stage_w = smem;
-    uint8_t *stage_a = smem + kWideStages * kWideWBytes;
-    uint8_t *store = smem + kWideStages * kWideStageBytes;
+    uint8_t *stage_a = smem + kStages * Shape::kWBytes;
+    uint8_t *store = smem + kStages * Shape::kStageBytes;
     uint32_t *first_tile = reinterpret_cast<uint32_t *>(store + kWideWarps * kWideStoreBytes);
     Ctl *control = reinterpret_cast<Ctl *>(store + kWideWarps * kWideStoreBytes + kWideTableBytes + 4);
     static_assert(sizeof(Ctl) <= 248 && (kWideTableBytes + 4) % 8 == 0, "control block");
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0u;
+    const uint32_t tile_first = PAIR ? blockIdx.x / 2 : blockIdx.x;
+    const uint32_t tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kWideStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&control->full[s]), 1);
             mbar_init(smem_u32(&control->empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&control->tmem_full[b]), 1);
-            mbar_init(smem_u32(&control->tmem_empty[b]), kWideWarps);
+            mbar_init(smem_u32(&control->tmem_empty[b]), (PAIR ? 2 : 1) * kWideWarps);
         }
         mbar_init(smem_u32(&control->drain), 1);
         control->abort_flag = 0;
         mbar_init_fence();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&control->tmem_base)),
-                     "r"(2 * kWideN)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&control->tmem_base)),
+                         "r"(2 * kWideN)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&control->tmem_base)),
+                         "r"(2 * kWideN)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     // The rows' copies, the offsets and every store come after the previous kernel. Weights are not
     // read early here: the tiles are long.
@@ -599,7 +623,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (e < params.experts) {
                 const int32_t begin = min(max(params.offsets[e], 0), rows);
                 const int32_t end = min(max(params.offsets[e + 1], begin), rows);
-                tiles = (static_cast<uint32_t>(end - begin) + kWideM - 1) / kWideM * n_tiles;
+                tiles = (static_cast<uint32_t>(end - begin) + Shape::kRows - 1) / Shape::kRows * n_tiles;
             }
             uint32_t through = tiles;
 #pragma unroll
@@ -614,9 +638,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any arrival or copy of the other
     tc_fence_after();
     const uint32_t tmem_base = control->tmem_base;
-    const uint32_t total = params.experts != 0 ? first_tile[params.experts] : (params.rows + kWideM - 1) / kWideM * n_tiles;
+    const uint32_t total = params.experts != 0 ? first_tile[params.experts] : (params.rows + Shape::kRows - 1) / Shape::kRows * n_tiles;
 
     if (warp == 0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
@@ -625,54 +650,80 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             prefetch_tensor_map(&map_a);
             uint32_t stage = 0, phase = 0, issued_mask = 0, issued_phases = 0;
             bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-                const WideTile tile = locate(params, first_tile, n_tiles, group_rows, t);
-                const int w_row = static_cast<int>(tile.expert * params.n + tile.n0);
+            for (uint32_t t = tile_first; ok && t < total; t += tile_step) {
+                const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, t);
+                const int w_row = static_cast<int>(tile.expert * params.n + tile.n0 + rank * kBlockN);
+                const int a_row = static_cast<int>(tile.row0 + rank * kWideM);
                 for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
                     ok = wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word);
                     if (!ok) break;
                     const uint32_t full = smem_u32(&control->full[stage]);
                     const int x = static_cast<int>(kb * kBlockK);
-                    mbar_expect_tx(full, kWideStageBytes);
-                    tma_load_2d(smem_u32(stage_a + stage * kWideABytes), &map_a, full, x, static_cast<int>(tile.row0));
-                    tma_load_2d(smem_u32(stage_w + stage * kWideWBytes), &map_w, full, x, w_row);
-                    tma_load_2d(smem_u32(stage_w + stage * kWideWBytes + kWideWBytes / 2), &map_w, full, x, w_row + kBlockN);
+                    if constexpr (PAIR) {
+                        if (rank == 0) mbar_expect_tx(full, 2 * Shape::kStageBytes);
+                        const uint32_t leader_full = map_to_rank(full, 0);
+                        tma_load_2d_pair(smem_u32(stage_a + stage * Shape::kABytes), &map_a, leader_full, x, a_row);
+                        tma_load_2d_pair(smem_u32(stage_w + stage * Shape::kWBytes), &map_w, leader_full, x, w_row);
+                    } else {
+                        mbar_expect_tx(full, Shape::kStageBytes);
+                        tma_load_2d(smem_u32(stage_a + stage * Shape::kABytes), &map_a, full, x, a_row);
+                        tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes), &map_w, full, x, w_row);
+                        tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes + Shape::kWBytes / 2), &map_w, full, x, w_row + kBlockN);
+                    }
                     issued_mask |= 1u << stage;
                     issued_phases = (issued_phases & ~(1u << stage)) | (phase << stage);
-                    if (++stage == kWideStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (!ok) {  // let every copy in flight land before the CTA exits
-                for (int s = 0; s < kWideStages; ++s)
-                    if ((issued_mask >> s) & 1u) wait_drain(smem_u32(&control->full[s]), (issued_phases >> s) & 1u);
+            if (!ok) {
+                // Let every copy in flight land before the CTA exits. Only rank 0's barriers see a
+                // pair's copies; the other CTA gives its own a bounded 200 us instead.
+                if (rank == 0) {
+                    for (int s = 0; s < kStages; ++s)
+                        if ((issued_mask >> s) & 1u) wait_drain(smem_u32(&control->full[s]), (issued_phases >> s) & 1u);
+                } else {
+                    const uint64_t start = globaltimer();
+                    while (globaltimer() - start < 200000ull) {
+                    }
+                }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
-        if (lane == 0) {
-            constexpr uint32_t instr = fp8_instr_desc(kWideM, kWideN);
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t instr = fp8_instr_desc(Shape::kRows, kWideN);
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 1;
             bool ok = true, any = false;
-            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            for (uint32_t t = tile_first; ok && t < total; t += tile_step) {
                 for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
                     ok = wait_bounded(smem_u32(&control->tmem_empty[buffer]), buffer_phase, &control->abort_flag, params.error_word) &&
                          wait_bounded(smem_u32(&control->full[stage]), phase, &control->abort_flag, params.error_word);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t a = smem_desc_sw128(smem_u32(stage_a + stage * kWideABytes));
-                    const uint64_t w = smem_desc_sw128(smem_u32(stage_w + stage * kWideWBytes));
+                    const uint64_t a = smem_desc_sw128(smem_u32(stage_a + stage * Shape::kABytes));
+                    const uint64_t w = smem_desc_sw128(smem_u32(stage_w + stage * Shape::kWBytes));
 #pragma unroll
-                    for (int kk = 0; kk < kBlockK / kMmaK; ++kk)
-                        mma_fp8(tmem_base + buffer * kWideN, a + static_cast<uint64_t>(kk * (kMmaK >> 4)),
-                                w + static_cast<uint64_t>(kk * (kMmaK >> 4)), instr, kk != 0 ? 1u : 0u);
-                    mma_commit(smem_u32(&control->empty[stage]));
-                    mma_commit(smem_u32(&control->tmem_full[buffer]));
+                    for (int kk = 0; kk < kBlockK / kMmaK; ++kk) {
+                        const uint64_t step = static_cast<uint64_t>(kk * (kMmaK >> 4));
+                        if constexpr (PAIR) {
+                            mma_fp8_pair(tmem_base + buffer * kWideN, a + step, w + step, instr, kk != 0 ? 1u : 0u);
+                        } else {
+                            mma_fp8(tmem_base + buffer * kWideN, a + step, w + step, instr, kk != 0 ? 1u : 0u);
+                        }
+                    }
+                    if constexpr (PAIR) {  // frees the stage and fills the accumulator in both CTAs
+                        mma_commit_pair(smem_u32(&control->empty[stage]));
+                        mma_commit_pair(smem_u32(&control->tmem_full[buffer]));
+                    } else {
+                        mma_commit(smem_u32(&control->empty[stage]));
+                        mma_commit(smem_u32(&control->tmem_full[buffer]));
+                    }
                     any = true;
-                    if (++stage == kWideStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -683,7 +734,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 }
             }
             if (!ok && any) {
-                mma_commit(smem_u32(&control->drain));
+                if constexpr (PAIR) {
+                    mma_commit_pair_local(smem_u32(&control->drain));
+                } else {
+                    mma_commit(smem_u32(&control->drain));
+                }
                 wait_drain(smem_u32(&control->drain), 0);
             }
         }
@@ -699,11 +754,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + half * (kWideN / 2);
         const bool vector = (reinterpret_cast<uintptr_t>(params.out) & 15u) == 0 && params.out_stride * sizeof(Out) % 16 == 0;
         const uint32_t tmem_full0 = smem_u32(&control->tmem_full[0]);
+        // released on the barrier of the CTA that issues the MMAs
+        const uint32_t tmem_empty0 = PAIR ? map_to_rank(smem_u32(&control->tmem_empty[0]), 0) : smem_u32(&control->tmem_empty[0]);
         uint32_t buffer = 0, buffer_phase = 0;
-        for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
-            const WideTile tile = locate(params, first_tile, n_tiles, group_rows, t);
+        for (uint32_t t = tile_first; t < total; t += tile_step) {
+            const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, t);
             const uint32_t n0 = tile.n0 + half * (kWideN / 2);
-            const uint32_t row0 = tile.row0 + quarter * 32u;
+            const uint32_t row0 = tile.row0 + rank * kWideM + quarter * 32u;
             const bool row_inside = row0 + lane < tile.row_end;
             const bool block_inside = n0 < params.n;
             const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n0 / kBlockN) * params.k_blocks;
@@ -760,7 +817,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 tmem_wait_load(odd);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
+                if (lane == 0) {
+                    if constexpr (PAIR) {
+                        arrive_cluster(tmem_empty0 + buffer * 8u);
+                    } else {
+                        mbar_arrive(tmem_empty0 + buffer * 8u);
+                    }
+                }
                 if (++buffer == 2) {
                     buffer = 0;
                     buffer_phase ^= 1u;
@@ -803,32 +866,85 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    // Neither CTA of a pair leaves while the other may still signal its barriers, read its shared
+    // memory or write its tensor memory.
+    if constexpr (PAIR) cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kWideN) : "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kWideN) : "memory");
+        } else {
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kWideN) : "memory");
+        }
     }
 }
 
-template <typename Out>
+template <typename Out, bool PAIR>
+cudaError_t configure_wide() {
+    return cudaFuncSetAttribute(fp8_gemm_wide_kernel<Out, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(wide_shared_bytes<PAIR>()));
+}
+
+// Pairs that can be resident at once, cached per device (0: not known yet).
+int resident_pairs(int sm_count) {
+    static std::atomic<int> cached[64] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return sm_count / 2;
+    const int known = cached[device].load(std::memory_order_relaxed);
+    if (known > 0) return known;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 2;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(sm_count & ~1));
+    config.blockDim = dim3(kWideThreads);
+    config.dynamicSmemBytes = wide_shared_bytes<true>();
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int pairs = 0;
+    if (cudaOccupancyMaxActiveClusters(&pairs, fp8_gemm_wide_kernel<float, true>, &config) != cudaSuccess || pairs <= 0) {
+        (void)cudaGetLastError();
+        return sm_count / 2;
+    }
+    cached[device].store(pairs, std::memory_order_relaxed);
+    return pairs;
+}
+
+template <typename Out, bool PAIR>
 cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, uint64_t tiles,
                         uint32_t n_tiles, uint32_t group_rows, int sm_count, cudaStream_t stream) {
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
-        return cudaFuncSetAttribute(fp8_gemm_wide_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(kWideSharedBytes));
+        const cudaError_t first = configure_wide<Out, PAIR>();
+        return first != cudaSuccess ? first : configure_wide<float, true>();  // resident_pairs asks about this one
     });
     if (error != cudaSuccess) return error;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+    const uint64_t resident = static_cast<uint64_t>(PAIR ? resident_pairs(sm_count) : sm_count);
+    const uint64_t walkers = tiles < resident ? tiles : resident;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = 2;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(tiles < static_cast<uint64_t>(sm_count) ? tiles : static_cast<uint64_t>(sm_count)));
+    config.gridDim = dim3(static_cast<unsigned>(walkers * (PAIR ? 2 : 1)));
     config.blockDim = dim3(kWideThreads);
-    config.dynamicSmemBytes = kWideSharedBytes;
+    config.dynamicSmemBytes = wide_shared_bytes<PAIR>();
     config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out>, map_w, map_a, params, n_tiles, group_rows);
+    config.attrs = attributes;
+    config.numAttrs = PAIR ? 2 : 1;
+    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR>, map_w, map_a, params, n_tiles, group_rows);
+}
+
+template <typename Out>
+cudaError_t launch_wide_type(bool pair, const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
+                             uint64_t tiles, uint32_t n_tiles, uint32_t group_rows, int sm_count, cudaStream_t stream) {
+    return pair ? launch_wide<Out, true>(map_w, map_a, params, tiles, n_tiles, group_rows, sm_count, stream)
+                : launch_wide<Out, false>(map_w, map_a, params, tiles, n_tiles, group_rows, sm_count, stream);
 }
 
 }  // namespace
@@ -864,14 +980,18 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
             !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, kWideM)) {
             return cudaErrorInvalidValue;
         }
-        uint64_t group = kGroupBytes / (static_cast<uint64_t>(kWideM) * desc.k);
+        // Pairs where tiles of 256 rows are not mostly padding.
+        const bool pair = desc.rows / matrices >= 2 * kWideM && sm_count >= 2;
+        const uint64_t height = pair ? 2 * kWideM : kWideM;
+        const uint64_t most_tiles = (static_cast<uint64_t>(desc.rows) + filled * (height - 1)) / height * n_tiles;
+        uint64_t group = kGroupBytes / (height * desc.k);
         group = group < kGroupRows ? kGroupRows : group;
         const uint32_t group_rows = static_cast<uint32_t>(group < 0x10000u ? group : 0x10000u);
         switch (desc.out_type) {
-            case QPUCUDA_DTYPE_F32: return launch_wide<float>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
+            case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
             case QPUCUDA_DTYPE_BF16:
-                return launch_wide<__nv_bfloat16>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
-            case QPUCUDA_DTYPE_F16: return launch_wide<__half>(map_w, map_a, params, wide_tiles, n_tiles, group_rows, sm_count, stream);
+                return launch_wide_type<__nv_bfloat16>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
+            case QPUCUDA_DTYPE_F16: return launch_wide_type<__half>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
         }
         return cudaErrorInvalidValue;
     }
