@@ -100,17 +100,16 @@ __device__ __forceinline__ uint32_t owned_rows(const GemmParams &params) {
 
 template <int NT>
 struct Narrow {
-    static constexpr int kWarps = NT >= 128 ? 8 : 4;        // epilogue warps: lane quarters x column halves
-    static constexpr int kColumns = NT / (kWarps / 4);      // accumulators of one epilogue thread
+    static constexpr int kWarps = 4;  // epilogue: one per lane quarter
     static constexpr int kThreads = 64 + 32 * kWarps;
-    static constexpr int kCtasPerSm = NT >= 128 ? 1 : 2;
+    static constexpr int kCtasPerSm = 2;
     static constexpr int kWBytes = kBlockN * kBlockK;
     static constexpr int kXBytes = NT * kBlockK;
     static constexpr int kStageBytes = kWBytes + kXBytes;
-    static constexpr int kStages = NT >= 128 ? 6 : (NT >= 64 ? 4 : 5);
-    static constexpr int kBuffers = NT >= 64 ? (NT >= 128 ? 4 : 4) : 4;  // tensor memory accumulators
-    static constexpr int kTmemColumns = kBuffers * NT;      // a power of two, 64 to 512
-    static constexpr int kScaleFloats = 2 * kColumns;       // per warp: this block's and the next's
+    static constexpr int kStages = 5;
+    static constexpr int kBuffers = 4;  // tensor memory accumulators
+    static constexpr int kTmemColumns = kBuffers * NT;      // a power of two
+    static constexpr int kScaleFloats = 2 * NT;             // per warp: this block's and the next's
     static constexpr size_t kSharedBytes = static_cast<size_t>(kStages) * kStageBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
     static_assert(kTmemColumns * kCtasPerSm <= 512, "tensor memory");
     static_assert(kSharedBytes * kCtasPerSm + 2048 <= 227 * 1024, "shared memory");
@@ -273,42 +272,35 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
     } else {
         if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        constexpr int kColumns = Shape::kColumns;
-        constexpr int kPerLane = (kColumns + 31) / 32;  // row scales one lane stages per block
+        constexpr int kColumns = NT;  // sums of a thread
         const uint32_t worker = warp - 2u;
         const uint32_t quarter = warp & 3u;  // tensor memory lanes this warp may read
-        const uint32_t column0 = (worker / 4u) * kColumns;
         float *scales = scale_rows + worker * Shape::kScaleFloats;
         const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n_block) * params.k_blocks;
-        const float *a_scales = params.a_scales + static_cast<size_t>(tile.row0 + column0) * params.a_scale_row_stride;
-        auto fetch = [&](uint32_t kb, float (&row_scale)[kPerLane], float &w_scale) {
+        const float *a_scales = params.a_scales + static_cast<size_t>(tile.row0) * params.a_scale_row_stride;
+        // Lane j stages row j's scale; rows past the tile hold zeros or another expert's values and
+        // are not stored. Fetched two blocks ahead.
+        const bool staging = lane < kColumns && tile.row0 + lane < params.rows;
+        auto fetch = [&](uint32_t kb, float &row_scale, float &w_scale) {
             const bool inside = kb < kb_end;
             w_scale = inside ? __ldg(w_scales + kb) : 0.0f;
-#pragma unroll
-            for (int p = 0; p < kPerLane; ++p) {
-                const uint32_t j = lane + 32u * p;
-                // rows past the tile hold zeros or another expert's values and are not stored
-                row_scale[p] = inside && j < kColumns && tile.row0 + column0 + j < params.rows
-                                   ? a_scales[static_cast<size_t>(j) * params.a_scale_row_stride + static_cast<size_t>(kb) * params.a_scale_group_stride]
-                                   : 0.0f;
-            }
+            row_scale = inside && staging ? a_scales[static_cast<size_t>(lane) * params.a_scale_row_stride +
+                                                     static_cast<size_t>(kb) * params.a_scale_group_stride]
+                                          : 0.0f;
         };
-        float row_now[kPerLane], row_next[kPerLane], w_now, w_next;
+        float row_now, row_next, w_now, w_next;
         fetch(kb_begin, row_now, w_now);
         fetch(kb_begin + 1, row_next, w_next);
         uint64_t acc[kColumns / 2];
 #pragma unroll
         for (int i = 0; i < kColumns / 2; ++i) acc[i] = 0;
-        const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + column0;
+        const uint32_t taddr = tmem_base + ((quarter * 32u) << 16);
         uint32_t buffer = 0, buffer_phase = 0;
         bool ok = true;
         for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
             float *products = scales + (kb & 1u) * kColumns;
-#pragma unroll
-            for (int p = 0; p < kPerLane; ++p)
-                if (lane + 32u * p < kColumns) products[lane + 32u * p] = row_now[p] * w_now;
-#pragma unroll
-            for (int p = 0; p < kPerLane; ++p) row_now[p] = row_next[p];
+            if (lane < kColumns) products[lane] = row_now * w_now;
+            row_now = row_next;
             w_now = w_next;
             fetch(kb + 2, row_next, w_next);
             if (lane == 0) ok = wait_bounded(smem_u32(&control->tmem_full[buffer]), buffer_phase, &control->abort_flag, params.error_word);
@@ -316,27 +308,21 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
             __syncwarp();
             if (!ok) break;
             tc_fence_after();
-            constexpr int kChunk = kColumns < 32 ? kColumns : 32;
+            uint32_t r[kColumns];
+            if constexpr (kColumns == 16) {
+                tmem_load_x16(taddr + buffer * NT, r);
+            } else {
+                tmem_load_x32(taddr + buffer * NT, r);
+            }
+            tmem_wait_load(r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
 #pragma unroll
-            for (int c = 0; c < kColumns; c += kChunk) {
-                uint32_t r[kChunk];
-                if constexpr (kChunk == 16) {
-                    tmem_load_x16(taddr + buffer * NT + c, r);
-                } else {
-                    tmem_load_x32(taddr + buffer * NT + c, r);
-                }
-                tmem_wait_load(r);
-                if (c + kChunk == kColumns) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&control->tmem_empty[buffer]));
-                }
-#pragma unroll
-                for (int i = 0; i < kChunk; i += 4) {
-                    const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(products + c + i);
-                    acc[(c + i) / 2] = fma2(pack2(r[i], r[i + 1]), s.x, acc[(c + i) / 2]);
-                    acc[(c + i) / 2 + 1] = fma2(pack2(r[i + 2], r[i + 3]), s.y, acc[(c + i) / 2 + 1]);
-                }
+            for (int i = 0; i < kColumns; i += 4) {
+                const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(products + i);
+                acc[i / 2] = fma2(pack2(r[i], r[i + 1]), s.x, acc[i / 2]);
+                acc[i / 2 + 1] = fma2(pack2(r[i + 2], r[i + 3]), s.y, acc[i / 2 + 1]);
             }
             if (++buffer == Shape::kBuffers) {
                 buffer = 0;
@@ -349,13 +335,13 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
             float *partial = reinterpret_cast<float *>(smem);
 #pragma unroll
             for (int i = 0; i < kColumns / 2; ++i) {
-                partial[(column0 + 2 * i) * kBlockN + column] = low(acc[i]);
-                partial[(column0 + 2 * i + 1) * kBlockN + column] = high(acc[i]);
+                partial[(2 * i) * kBlockN + column] = low(acc[i]);
+                partial[(2 * i + 1) * kBlockN + column] = high(acc[i]);
             }
         } else if (ok && n0 + column < params.n) {
             const float bias = params.bias != nullptr ? __ldg(params.bias + n0 + column) : 0.0f;
-            Out *out = static_cast<Out *>(params.out) + static_cast<size_t>(tile.row0 + column0) * params.out_stride + n0 + column;
-            const uint32_t rows = tile.row_end - tile.row0 > column0 ? tile.row_end - tile.row0 - column0 : 0u;
+            Out *out = static_cast<Out *>(params.out) + static_cast<size_t>(tile.row0) * params.out_stride + n0 + column;
+            const uint32_t rows = tile.row_end - tile.row0;
 #pragma unroll
             for (uint32_t i = 0; i < kColumns; ++i) {
                 const float v = (i & 1u) ? high(acc[i / 2]) : low(acc[i / 2]);
@@ -369,13 +355,11 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
         if (tile.valid && warp >= 2) {
             const uint32_t rows = tile.row_end - tile.row0;
             const float *partial = reinterpret_cast<const float *>(smem);
-            // the tile's rows in turn over the ranks and the warp groups, 128 columns across
-            const uint32_t worker = threadIdx.x - 64u;
-            const uint32_t column = worker % kBlockN;
+            // the tile's rows in turn over the ranks, 128 columns across
+            const uint32_t column = threadIdx.x - 64u;
             const bool inside = n0 + column < params.n;
             const float bias = params.bias != nullptr && inside ? __ldg(params.bias + n0 + column) : 0.0f;
-            constexpr uint32_t kGroups = Shape::kWarps / 4;
-            for (uint32_t row = rank * kGroups + worker / kBlockN; row < rows; row += split * kGroups) {
+            for (uint32_t row = rank; row < rows; row += split) {
                 const uint32_t address = smem_u32(partial + row * kBlockN + column);
                 float sum = 0.0f;
                 for (uint32_t r = 0; r < split; ++r) sum += load_cluster(map_to_rank(address, r));
@@ -386,11 +370,9 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
         }
     }
     if (params.experts != 0 && rank == 0 && warp >= 2) {
-        const uint32_t worker = threadIdx.x - 64u;
-        const uint32_t column = n0 + worker % kBlockN;
+        const uint32_t column = n0 + threadIdx.x - 64u;
         if (column < params.n)
-            for (uint32_t row = owned_rows(params) + blockIdx.y * (Shape::kWarps / 4) + worker / kBlockN; row < params.rows;
-                 row += gridDim.y * (Shape::kWarps / 4))
+            for (uint32_t row = owned_rows(params) + blockIdx.y; row < params.rows; row += gridDim.y)
                 static_cast<Out *>(params.out)[static_cast<size_t>(row) * params.out_stride + column] = from_float<Out>(0.0f);
     }
     tc_fence_before();
@@ -433,12 +415,8 @@ cudaError_t launch_narrow(const CUtensorMap &map_w, const CUtensorMap &map_a, co
 template <typename Out>
 cudaError_t launch_narrow_rows(int nt, const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
                                uint32_t tiles, uint32_t split, cudaStream_t stream) {
-    switch (nt) {
-        case 16: return launch_narrow<16, Out>(map_w, map_a, params, tiles, split, stream);
-        case 32: return launch_narrow<32, Out>(map_w, map_a, params, tiles, split, stream);
-        case 64: return launch_narrow<64, Out>(map_w, map_a, params, tiles, split, stream);
-        default: return launch_narrow<128, Out>(map_w, map_a, params, tiles, split, stream);
-    }
+    return nt == 16 ? launch_narrow<16, Out>(map_w, map_a, params, tiles, split, stream)
+                    : launch_narrow<32, Out>(map_w, map_a, params, tiles, split, stream);
 }
 
 // ---- the wide kernel --------------------------------------------------------------------------
@@ -476,6 +454,13 @@ constexpr size_t wide_shared_bytes() {
     return Wide<PAIR>::kStages * Wide<PAIR>::kStageBytes + kWideWarps * kWideStoreBytes + kWideTableBytes + 256 + 1024;
 }
 static_assert(wide_shared_bytes<false>() <= 227 * 1024 && wide_shared_bytes<true>() <= 227 * 1024, "shared memory");
+
+struct WideLaunch {
+    bool pair;
+    uint32_t split;
+    uint64_t tiles;  // at most, whatever the offsets
+    uint32_t n_tiles, group_rows;
+};
 
 struct WideTile {
     uint32_t expert, row0, row_end, n0;
@@ -558,12 +543,21 @@ __device__ __forceinline__ void store_chunk(uint4 *buffer, const float (&v)[64 /
     }
 }
 
+template <int N>
+__device__ __forceinline__ void add_bias(const GemmParams &params, uint32_t n, float (&v)[N]) {
+    if (params.bias == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += n + i < params.n ? __ldg(params.bias + n + i) : 0.0f;
+}
+
 // Persistent: one CTA (or pair) per SM (or two) walks tiles 0, 1, ... in steps of the CTAs or pairs.
 //   warp 0   copies: a row box and the weight boxes per stage (a pair's bytes all complete on rank 0's barriers)
 //   warp 1   tensor memory and MMA (rank 0 alone in a pair): 4 MMAs per stage into one of two accumulators
 //   warp 2   the experts' table of tiles, warp 3 nothing
 //   4 to 11  each block's accumulator into registers, scaled; at the tile's end the store
-template <typename Out, bool PAIR>
+// SPLIT: few tiles. The CTAs of a cluster share one tile's K blocks and add their sums, in slice
+// order, through distributed shared memory; each CTA has one tile.
+template <typename Out, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1)
     fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                          const GemmParams params, uint32_t n_tiles, uint32_t group_rows) {
@@ -581,9 +575,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31;
+    static_assert(!(PAIR && SPLIT), "a cluster is a pair or shares K");
     const uint32_t rank = PAIR ? cluster_rank() : 0u;
-    const uint32_t tile_first = PAIR ? blockIdx.x / 2 : blockIdx.x;
-    const uint32_t tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
+    const uint32_t slices = SPLIT ? cluster_size() : 1u;
+    const uint32_t slice = SPLIT ? cluster_rank() : 0u;
+    const uint32_t tile_first = PAIR ? blockIdx.x / 2 : blockIdx.x / slices;
+    const uint32_t tile_step = PAIR ? gridDim.x / 2 : gridDim.x / slices;
+    const uint32_t kb_begin = SPLIT ? static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * slice / slices) : 0u;
+    const uint32_t kb_end = SPLIT ? static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * (slice + 1) / slices) : params.k_blocks;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&control->full[s]), 1);
@@ -654,7 +653,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, t);
                 const int w_row = static_cast<int>(tile.expert * params.n + tile.n0 + rank * kBlockN);
                 const int a_row = static_cast<int>(tile.row0 + rank * kWideM);
-                for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+                for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
                     ok = wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word);
                     if (!ok) break;
                     const uint32_t full = smem_u32(&control->full[stage]);
@@ -692,6 +691,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         }
         __syncwarp();
+        if constexpr (SPLIT) cluster_sync();
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
         if (lane == 0 && rank == 0) {
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 1;
             bool ok = true, any = false;
             for (uint32_t t = tile_first; ok && t < total; t += tile_step) {
-                for (uint32_t kb = 0; kb < params.k_blocks; ++kb) {
+                for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
                     ok = wait_bounded(smem_u32(&control->tmem_empty[buffer]), buffer_phase, &control->abort_flag, params.error_word) &&
                          wait_bounded(smem_u32(&control->full[stage]), phase, &control->abort_flag, params.error_word);
                     if (!ok) break;
@@ -743,8 +743,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         }
         __syncwarp();
+        if constexpr (SPLIT) cluster_sync();
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
+        if constexpr (SPLIT) cluster_sync();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideManyRegisters));
         const uint32_t worker = warp - 4u;
@@ -766,13 +768,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n0 / kBlockN) * params.k_blocks;
             const float *a_scales = params.a_scales + static_cast<size_t>(row0 + lane) * params.a_scale_row_stride;
             // A block's factor is fetched two blocks ahead; the fetches of the last two repeat the last block.
-            const float *a_at = row_inside ? a_scales : params.a_scales;
-            const float *w_at = block_inside ? w_scales : params.w_scales;
-            uint32_t fetched = 0;
+            const float *a_at = (row_inside ? a_scales : params.a_scales) + static_cast<size_t>(kb_begin) * params.a_scale_group_stride;
+            const float *w_at = (block_inside ? w_scales : params.w_scales) + kb_begin;
+            uint32_t fetched = kb_begin;
             auto fetch = [&](float &a, float &w) {
                 a = *a_at;
                 w = __ldg(w_at);
-                if (++fetched < params.k_blocks) {
+                if (++fetched < kb_end) {
                     a_at += params.a_scale_group_stride;
                     ++w_at;
                 }
@@ -799,7 +801,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 return all;
             };
             bool ok = arrived();
-            for (uint32_t kb = 0; ok && kb < params.k_blocks; ++kb) {
+            for (uint32_t kb = kb_begin; ok && kb < kb_end; ++kb) {
                 const float factor = a_now * w_now;
                 const uint64_t factors = pack2(factor, factor);
                 a_now = a_next;
@@ -829,11 +831,20 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     buffer = 0;
                     buffer_phase ^= 1u;
                 }
-                if (kb + 1 < params.k_blocks) ok = arrived();
+                if (kb + 1 < kb_end) ok = arrived();
                 add(2, even, factors);
                 add(3, odd, factors);
             }
             if (!ok) break;
+            if constexpr (SPLIT) {
+                // The only tile of this CTA, and its MMAs are complete: the stages hold the partial
+                // sums, [column / 4][row] float4, which the cluster's CTAs add up below.
+                float4 *partial = reinterpret_cast<float4 *>(smem) + half * (kWideN / 8) * kWideM + quarter * 32u + lane;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    partial[i * kWideM] = make_float4(low(acc[2 * i]), high(acc[2 * i]), low(acc[2 * i + 1]), high(acc[2 * i + 1]));
+                continue;
+            }
             if (row0 >= tile.row_end || !block_inside) continue;
             constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
             const uint32_t rows = tile.row_end - row0;
@@ -847,12 +858,43 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     v[i] = low(acc[(c + i) / 2]);
                     v[i + 1] = high(acc[(c + i) / 2]);
                 }
-                if (params.bias != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < kChunk; ++i) v[i] += n + i < params.n ? __ldg(params.bias + n + i) : 0.0f;
-                }
+                add_bias(params, n, v);
                 store_chunk<Out>(buffer_out, v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
                                  params.out_stride, rows, params.n - n, vector, lane);
+            }
+        }
+        if constexpr (SPLIT) {
+            __syncwarp();
+            cluster_sync();  // every slice's partial sums are in place
+            if (tile_first < total) {
+                // This CTA's share of the columns, summed in slice order: 256 / slices of them, half to
+                // each four warps, a row to a thread.
+                const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, tile_first);
+                constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
+                const uint32_t row0 = tile.row0 + quarter * 32u;
+                const uint32_t columns = kWideN / slices / 2u;
+                const uint32_t column0 = slice * (kWideN / slices) + half * columns;
+                if (row0 < tile.row_end) {
+                    for (uint32_t c = column0; c < column0 + columns && tile.n0 + c < params.n; c += kChunk) {
+                        const uint32_t address = smem_u32(smem) + ((c / 4u) * kWideM + quarter * 32u + lane) * 16u;
+                        float v[kChunk] = {};
+                        for (uint32_t r = 0; r < slices; ++r) {
+                            const uint32_t remote = map_to_rank(address, r);
+#pragma unroll
+                            for (int i = 0; i < kChunk / 4; ++i) {
+                                const float4 part = load_cluster4(remote + i * kWideM * 16u);
+                                v[4 * i] += part.x;
+                                v[4 * i + 1] += part.y;
+                                v[4 * i + 2] += part.z;
+                                v[4 * i + 3] += part.w;
+                            }
+                        }
+                        const uint32_t n = tile.n0 + c;
+                        add_bias(params, n, v);
+                        store_chunk<Out>(buffer_out, v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
+                                         params.out_stride, tile.row_end - row0, params.n - n, vector, lane);
+                    }
+                }
             }
         }
         if (params.experts != 0) {
@@ -865,6 +907,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    // No slice leaves while another reads its sums.
+    if constexpr (SPLIT) cluster_sync();
     // Neither CTA of a pair leaves while the other may still signal its barriers, read its shared
     // memory or write its tensor memory.
     if constexpr (PAIR) cluster_sync();
@@ -878,9 +922,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
 }
 
-template <typename Out, bool PAIR>
+template <typename Out, bool PAIR, bool SPLIT>
 cudaError_t configure_wide() {
-    return cudaFuncSetAttribute(fp8_gemm_wide_kernel<Out, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(fp8_gemm_wide_kernel<Out, PAIR, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(wide_shared_bytes<PAIR>()));
 }
 
@@ -903,7 +947,7 @@ int resident_pairs(int sm_count) {
     config.attrs = &attribute;
     config.numAttrs = 1;
     int pairs = 0;
-    if (cudaOccupancyMaxActiveClusters(&pairs, fp8_gemm_wide_kernel<float, true>, &config) != cudaSuccess || pairs <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&pairs, fp8_gemm_wide_kernel<float, true, false>, &config) != cudaSuccess || pairs <= 0) {
         (void)cudaGetLastError();
         return sm_count / 2;
     }
@@ -911,39 +955,56 @@ int resident_pairs(int sm_count) {
     return pairs;
 }
 
-template <typename Out, bool PAIR>
-cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, uint64_t tiles,
-                        uint32_t n_tiles, uint32_t group_rows, int sm_count, cudaStream_t stream) {
+// split: CTAs of a cluster that share a tile's K blocks (1, 2 or 4; then tiles * split CTAs, one tile each).
+template <typename Out, bool PAIR, bool SPLIT>
+cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, const WideLaunch &launch,
+                        int sm_count, cudaStream_t stream) {
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
-        const cudaError_t first = configure_wide<Out, PAIR>();
-        return first != cudaSuccess ? first : configure_wide<float, true>();  // resident_pairs asks about this one
+        const cudaError_t first = configure_wide<Out, PAIR, SPLIT>();
+        return first != cudaSuccess || !PAIR ? first : configure_wide<float, true, false>();  // resident_pairs asks about this one
     });
     if (error != cudaSuccess) return error;
-    const uint64_t resident = static_cast<uint64_t>(PAIR ? resident_pairs(sm_count) : sm_count);
-    const uint64_t walkers = tiles < resident ? tiles : resident;
+    const uint64_t resident = PAIR ? static_cast<uint64_t>(resident_pairs(sm_count)) : (SPLIT ? launch.tiles : static_cast<uint64_t>(sm_count));
+    const uint64_t walkers = launch.tiles < resident ? launch.tiles : resident;
+    const uint32_t cluster = PAIR ? 2u : launch.split;
     cudaLaunchAttribute attributes[2] = {};
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
     attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = 2;
+    attributes[1].val.clusterDim.x = cluster;
     attributes[1].val.clusterDim.y = 1;
     attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(walkers * (PAIR ? 2 : 1)));
+    config.gridDim = dim3(static_cast<unsigned>(walkers * cluster));
     config.blockDim = dim3(kWideThreads);
     config.dynamicSmemBytes = wide_shared_bytes<PAIR>();
     config.stream = stream;
     config.attrs = attributes;
-    config.numAttrs = PAIR ? 2 : 1;
-    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR>, map_w, map_a, params, n_tiles, group_rows);
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR, SPLIT>, map_w, map_a, params, launch.n_tiles, launch.group_rows);
 }
 
 template <typename Out>
-cudaError_t launch_wide_type(bool pair, const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
-                             uint64_t tiles, uint32_t n_tiles, uint32_t group_rows, int sm_count, cudaStream_t stream) {
-    return pair ? launch_wide<Out, true>(map_w, map_a, params, tiles, n_tiles, group_rows, sm_count, stream)
-                : launch_wide<Out, false>(map_w, map_a, params, tiles, n_tiles, group_rows, sm_count, stream);
+cudaError_t launch_wide_type(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, const WideLaunch &launch,
+                             int sm_count, cudaStream_t stream) {
+    if (launch.pair) return launch_wide<Out, true, false>(map_w, map_a, params, launch, sm_count, stream);
+    if (launch.split > 1) return launch_wide<Out, false, true>(map_w, map_a, params, launch, sm_count, stream);
+    return launch_wide<Out, false, false>(map_w, map_a, params, launch, sm_count, stream);
+}
+
+// Rows per matrix from which pairs' tiles of 256 rows are worth their padding with uneven experts: 512
+// rows each (4096 tokens, 4 of 32, 5632 x 2048) took 303 us in pairs and 292 alone, 1024 rows 525 and 534.
+constexpr uint64_t kPairShare = 1024;
+
+// Many rows per matrix, or weights that fill the SMs with wide tiles already: the wide kernel's deeper
+// copies then stream them at least as fast. One matrix of 11008 x 4096: 65 rows 17 us wide, 64 rows 19
+// us narrow, 24 rows 15 us narrow and 20 wide; of 2048 x 2048: 64 rows 9 us narrow, 65 rows 11 us wide.
+// 32 experts of 5632 x 2048 with 8 rows each: 70 us wide, 73 narrow; with 32 rows 77 against 104.
+bool use_wide(uint64_t share, uint64_t matrices, uint64_t n_tiles, uint64_t sms) {
+    if (share > 64) return true;
+    if (matrices > 1) return share > 4 && matrices * n_tiles * 4 >= sms * 3;
+    return share > 32 && n_tiles >= 16;
 }
 
 }  // namespace
@@ -968,43 +1029,47 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
     params.weights_settled = desc.weights_settled != 0 ? 1u : 0u;
     params.error_word = error_word;
     const uint64_t matrices = desc.experts != 0 ? desc.experts : 1u;
-    // Rows of an even share, and tiles of 128 x 256 at most, whatever the offsets.
-    const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;
-    const uint32_t n_tiles = (desc.n + kWideN - 1) / kWideN;
-    const uint64_t wide_tiles = (static_cast<uint64_t>(desc.rows) + filled * (kWideM - 1)) / kWideM * n_tiles;
-    if (wide_tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
-    if (desc.rows / matrices >= kWideM && wide_tiles >= static_cast<uint64_t>(sm_count)) {
+    const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;  // matrices that can have rows
+    const uint64_t share = (desc.rows + matrices - 1) / matrices;
+    const uint64_t sms = static_cast<uint64_t>(sm_count);
+    // Tiles of `height` rows, at most, whatever the offsets: one partly filled tile per matrix.
+    const auto most_tiles = [&](uint64_t height) { return (desc.rows + filled * (height - 1)) / height; };
+    WideLaunch wide{};
+    wide.n_tiles = (desc.n + kWideN - 1) / kWideN;
+    if (use_wide(share, filled, wide.n_tiles, sms)) {
+        // Pairs where tiles of 256 rows hold hardly more padding than tiles of 128.
+        wide.pair = sms >= 2 && (desc.experts != 0 ? share >= kPairShare : most_tiles(2 * kWideM) * 2 * 12 <= most_tiles(kWideM) * 13);
+        const uint64_t height = wide.pair ? 2 * kWideM : kWideM;
+        wide.tiles = most_tiles(height) * wide.n_tiles;
+        if (wide.tiles > 0x3FFFFFFFull) return cudaErrorInvalidValue;
+        wide.split = 1;
+        if (wide.tiles * 2 <= sms) {
+            wide.pair = false;
+            wide.tiles = most_tiles(kWideM) * wide.n_tiles;
+            while (wide.split < 4 && wide.tiles * wide.split * 2 <= sms && wide.split * 8 <= params.k_blocks) wide.split *= 2;
+        }
         CUtensorMap map_w, map_a;
         if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
             !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, kWideM)) {
             return cudaErrorInvalidValue;
         }
-        // Pairs where tiles of 256 rows are not mostly padding.
-        const bool pair = desc.rows / matrices >= 2 * kWideM && sm_count >= 2;
-        const uint64_t height = pair ? 2 * kWideM : kWideM;
-        const uint64_t most_tiles = (static_cast<uint64_t>(desc.rows) + filled * (height - 1)) / height * n_tiles;
-        uint64_t group = kGroupBytes / (height * desc.k);
-        group = group < kGroupRows ? kGroupRows : group;
-        const uint32_t group_rows = static_cast<uint32_t>(group < 0x10000u ? group : 0x10000u);
+        const uint64_t group = kGroupBytes / (height * desc.k);
+        wide.group_rows = static_cast<uint32_t>(group < kGroupRows ? kGroupRows : (group < 0x10000u ? group : 0x10000u));
         switch (desc.out_type) {
-            case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
-            case QPUCUDA_DTYPE_BF16:
-                return launch_wide_type<__nv_bfloat16>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
-            case QPUCUDA_DTYPE_F16: return launch_wide_type<__half>(pair, map_w, map_a, params, most_tiles, n_tiles, group_rows, sm_count, stream);
+            case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(map_w, map_a, params, wide, sm_count, stream);
+            case QPUCUDA_DTYPE_BF16: return launch_wide_type<__nv_bfloat16>(map_w, map_a, params, wide, sm_count, stream);
+            case QPUCUDA_DTYPE_F16: return launch_wide_type<__half>(map_w, map_a, params, wide, sm_count, stream);
         }
         return cudaErrorInvalidValue;
     }
-    // The tile's height: the smallest that holds an expert's even share of the rows.
-    const uint64_t share = (desc.rows + matrices - 1) / matrices;
-    const int nt = share <= 16 ? 16 : (share <= 32 ? 32 : (share <= 64 ? 64 : 128));
+    // The tile's height: 16 rows, or 32 where a matrix has more (uneven experts: more than 4 on average).
+    const int nt = share <= (desc.experts != 0 ? 4u : 16u) ? 16 : 32;
     CUtensorMap map_w, map_a;
     if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
         !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, static_cast<uint32_t>(nt))) {
         return cudaErrorInvalidValue;
     }
-    // At most this many tiles of rows, whatever the offsets: one partly filled tile per matrix.
-    const uint64_t tiles = (static_cast<uint64_t>(desc.rows) + filled * (nt - 1)) / nt;
-    if (tiles > 65535u) return cudaErrorInvalidValue;
+    const uint64_t tiles = most_tiles(static_cast<uint64_t>(nt));
     // K is split over a cluster while the tiles leave SMs idle, two CTAs each.
     uint32_t split = 1;
     while (split < kMaxSplit && tiles * params.n_blocks * split * 2 <= static_cast<uint64_t>(sm_count) * 2 &&

@@ -120,6 +120,11 @@ __device__ __forceinline__ float load_cluster(uint32_t cluster_address) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 load_cluster4(uint32_t cluster_address) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_address) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
