@@ -41,6 +41,7 @@ struct GemmParams {
     void *out;
     size_t out_stride;
     uint32_t weights_settled;
+    uint32_t tma_store;  // the output's rows can be written by the copy engine
     unsigned int *error_word;
 };
 
@@ -442,12 +443,13 @@ static_assert(128 * kWideFewRegisters + 256 * kWideManyRegisters <= 384 * 168, "
 template <bool PAIR>
 struct Wide {
     static constexpr int kRows = PAIR ? 2 * kWideM : kWideM;  // of a tile
-    static constexpr int kStages = PAIR ? 6 : 4;
+    static constexpr int kStages = PAIR ? 4 : 3;
     static constexpr int kABytes = kWideM * kBlockK;
     static constexpr int kWBytes = (PAIR ? kWideN / 2 : kWideN) * kBlockK;
     static constexpr int kStageBytes = kABytes + kWBytes;
 };
-constexpr int kWideStoreBytes = 2048;  // per epilogue warp: 32 rows x 64 bytes on their way out
+constexpr int kWideBoxBytes = 4096;    // 32 rows x 128 bytes of the output
+constexpr int kWideStoreBytes = 2 * kWideBoxBytes;  // per epilogue warp, on their way out
 constexpr size_t kWideTableBytes = (QPUCUDA_MAX_EXPERTS + 1) * sizeof(uint32_t);
 template <bool PAIR>
 constexpr size_t wide_shared_bytes() {
@@ -550,6 +552,55 @@ __device__ __forceinline__ void add_bias(const GemmParams &params, uint32_t n, f
     for (int i = 0; i < N; ++i) v[i] += n + i < params.n ? __ldg(params.bias + n + i) : 0.0f;
 }
 
+// One box of a warp's 32 rows (a row to a lane, 128 bytes each) on its way out. Staged in shared
+// memory in the 128-byte swizzle (16-byte slot c of row r at c ^ (r & 7): no bank conflicts) and copied
+// out from there: by the copy engine while the warp goes on, where the output's rows are aligned and
+// all 32 are the tile's (`map` then), else by the warp, eight lanes to a row.
+template <typename Out>
+__device__ __forceinline__ void store_box(uint8_t *buffer, const float (&v)[128 / sizeof(Out)], const CUtensorMap *map, Out *out,
+                                          size_t out_stride, int row, uint32_t column, uint32_t rows, uint32_t columns, bool vector,
+                                          uint32_t lane) {
+    constexpr uint32_t kColumns = 128 / sizeof(Out);
+    constexpr uint32_t kPerSlot = kColumns / 8;
+    uint4 *slots = reinterpret_cast<uint4 *>(buffer);
+    if (lane == 0) bulk_wait_read_all_but_one();  // the copy that last read this buffer is two copies back
+    __syncwarp();
+#pragma unroll
+    for (uint32_t c = 0; c < 8; ++c) {
+        Vector<Out> slot;
+#pragma unroll
+        for (uint32_t i = 0; i < kPerSlot; ++i) slot.items[i] = from_float<Out>(v[c * kPerSlot + i]);
+        slots[lane * 8u + (c ^ (lane & 7u))] = slot.bits;
+    }
+    if (map != nullptr) {
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, smem_u32(buffer), static_cast<int>(column * sizeof(Out)), row);
+            bulk_commit();
+        }
+        return;
+    }
+    __syncwarp();
+    if (vector && columns >= kColumns) {
+        const uint32_t c = lane & 7u;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t r = i * 4u + lane / 8u;
+            const uint4 value = slots[r * 8u + (c ^ (r & 7u))];
+            if (r < rows) *reinterpret_cast<uint4 *>(out + r * out_stride + c * kPerSlot) = value;
+        }
+    } else {
+        const Out *items = reinterpret_cast<const Out *>(buffer);
+        for (uint32_t r = 0; r < min(rows, 32u); ++r)
+#pragma unroll
+            for (uint32_t j = lane; j < kColumns; j += 32)
+                if (j < columns) out[r * out_stride + j] = items[(r * 8u + ((j / kPerSlot) ^ (r & 7u))) * kPerSlot + j % kPerSlot];
+    }
+    if (lane == 0) bulk_commit();  // an empty group keeps the count of two buffers
+    __syncwarp();
+}
+
 // Persistent: one CTA (or pair) per SM (or two) walks tiles 0, 1, ... in steps of the CTAs or pairs.
 //   warp 0   copies: a row box and the weight boxes per stage (a pair's bytes all complete on rank 0's barriers)
 //   warp 1   tensor memory and MMA (rank 0 alone in a pair): 4 MMAs per stage into one of two accumulators
@@ -560,6 +611,7 @@ __device__ __forceinline__ void add_bias(const GemmParams &params, uint32_t n, f
 template <typename Out, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1)
     fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                         const __grid_constant__ CUtensorMap map_out,
                          const GemmParams params, uint32_t n_tiles, uint32_t group_rows) {
     using Shape = Wide<PAIR>;
     constexpr int kStages = Shape::kStages;
@@ -752,7 +804,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t worker = warp - 4u;
         const uint32_t quarter = warp & 3u;
         const uint32_t half = worker / 4u;
-        uint4 *buffer_out = reinterpret_cast<uint4 *>(store + worker * kWideStoreBytes);
+        uint8_t *buffer_out = store + worker * kWideStoreBytes;
         const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + half * (kWideN / 2);
         const bool vector = (reinterpret_cast<uintptr_t>(params.out) & 15u) == 0 && params.out_stride * sizeof(Out) % 16 == 0;
         const uint32_t tmem_full0 = smem_u32(&control->tmem_full[0]);
@@ -846,8 +898,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 continue;
             }
             if (row0 >= tile.row_end || !block_inside) continue;
-            constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
+            constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));
             const uint32_t rows = tile.row_end - row0;
+            // rows past the last expert's would be overwritten by a copy of the whole box; rows past
+            // the output are cut off by it
+            const bool whole = params.tma_store != 0 && (params.experts == 0 || rows >= 32);
 #pragma unroll
             for (int c = 0; c < kWideN / 2; c += kChunk) {
                 const uint32_t n = n0 + c;
@@ -859,8 +914,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     v[i + 1] = high(acc[(c + i) / 2]);
                 }
                 add_bias(params, n, v);
-                store_chunk<Out>(buffer_out, v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
-                                 params.out_stride, rows, params.n - n, vector, lane);
+                store_box<Out>(buffer_out + (c / kChunk & 1) * kWideBoxBytes, v, whole ? &map_out : nullptr,
+                               static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n, params.out_stride,
+                               static_cast<int>(row0), n, rows, params.n - n, vector, lane);
             }
         }
         if constexpr (SPLIT) {
@@ -891,7 +947,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         }
                         const uint32_t n = tile.n0 + c;
                         add_bias(params, n, v);
-                        store_chunk<Out>(buffer_out, v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
+                        store_chunk<Out>(reinterpret_cast<uint4 *>(buffer_out), v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
                                          params.out_stride, tile.row_end - row0, params.n - n, vector, lane);
                     }
                 }
@@ -904,6 +960,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 for (uint32_t n = lane; n < params.n; n += 32)
                     static_cast<Out *>(params.out)[static_cast<size_t>(row) * params.out_stride + n] = from_float<Out>(0.0f);
         }
+        if (lane == 0) bulk_wait_all();  // every copy out is complete before the CTA ends
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -957,7 +1015,7 @@ int resident_pairs(int sm_count) {
 
 // split: CTAs of a cluster that share a tile's K blocks (1, 2 or 4; then tiles * split CTAs, one tile each).
 template <typename Out, bool PAIR, bool SPLIT>
-cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, const WideLaunch &launch,
+cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, GemmParams params, const WideLaunch &launch,
                         int sm_count, cudaStream_t stream) {
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
@@ -982,7 +1040,14 @@ cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, cons
     config.stream = stream;
     config.attrs = attributes;
     config.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR, SPLIT>, map_w, map_a, params, launch.n_tiles, launch.group_rows);
+    CUtensorMap map_out;
+    std::memset(&map_out, 0, sizeof(map_out));
+    params.tma_store = encode_tensor_map_2d_u8(&map_out, params.out, static_cast<uint64_t>(params.n) * sizeof(Out), params.rows,
+                                               params.out_stride * sizeof(Out), 128u, 32u)
+                           ? 1u
+                           : 0u;
+    return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR, SPLIT>, map_w, map_a, map_out, params, launch.n_tiles,
+                              launch.group_rows);
 }
 
 template <typename Out>
