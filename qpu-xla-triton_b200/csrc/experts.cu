@@ -2,12 +2,15 @@
 //
 // The sort is a stable counting sort in integers. A choice's row is
 //   offsets[e] + (choices of e in earlier chunks) + (in earlier warps of its chunk) + (earlier in its warp),
-// every term an exact count, so the order never depends on timing. Moving the rows is bound by HBM:
-// each kernel reads a token's vector once, in registers, for all of its choices, and writes each
+// every term an exact count, so the order never depends on timing. Up to 32768 choices (a prompt of
+// 4096 tokens with 8 choices) it is one launch of one cluster, whose CTAs read each other's counts in
+// distributed shared memory; above, a kernel counts the chunks first. Moving the rows is bound by
+// HBM: each kernel reads a token's vector once, in registers, for all of its choices, and writes each
 // row once.
 #include "element.cuh"
 #include "qpucuda_fp8_internal.h"
 #include "qpucuda_internal.h"
+#include "sm100_fp8.cuh"
 
 namespace qpucuda {
 namespace {
@@ -16,13 +19,15 @@ namespace {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-// A chunk is one CTA's share. Up to kSortChunk choices take one CTA and one launch; above, at most
-// kSortMaxChunks CTAs, so that each can add up the counts of all chunks by itself.
+// A chunk is one CTA's share: the CTAs of one cluster, or above kSortCluster chunks a grid whose CTAs
+// each add up the counts of all chunks, at most kSortMaxChunks of them.
 constexpr uint32_t kSortChunk = 4096;
+constexpr uint32_t kSortCluster = 8;
 constexpr uint32_t kSortMaxChunks = 64;
 constexpr uint32_t kMaxExperts = QPUCUDA_MAX_EXPERTS;
 
 uint32_t sort_chunk(uint32_t total) {
+    if (total <= kSortCluster * kSortChunk) return kSortChunk;
     const uint32_t least = (total + kSortMaxChunks - 1) / kSortMaxChunks;
     const uint32_t chunk = least > kSortChunk ? least : kSortChunk;
     return (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
@@ -55,13 +60,14 @@ __global__ void __launch_bounds__(kSortThreads) expert_count_kernel(const Id *__
         counts[static_cast<size_t>(blockIdx.x) * experts + e] = histogram[e];
 }
 
-// Rows of one chunk per CTA. counts: [gridDim.x][experts], or null for a single chunk.
+// Rows of one chunk per CTA. counts: [gridDim.x][experts], or null where the grid is one cluster: the
+// CTAs then publish their chunk's counts in shared memory, behind `next`.
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *__restrict__ ids, uint32_t total,
                                                                       uint32_t chunk, uint32_t experts,
                                                                       const int32_t *counts, int32_t *offsets,
                                                                       int32_t *source, int32_t *position) {
-    extern __shared__ int32_t next[];  // [kSortWarps][experts]: counts, then the next row of (warp, expert)
+    extern __shared__ int32_t next[];  // [kSortWarps + 1][experts]: counts, then the next row of (warp, expert)
     __shared__ int32_t warp_sums[kSortWarps];
     __shared__ int32_t kept;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -83,6 +89,7 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
     // Thread t takes experts 2t and 2t + 1: their counts over this chunk's warps become offsets
     // inside the chunk, their totals over all chunks are scanned into the experts' first rows.
     int32_t in_all[2], before[2];
+    int32_t *published = next + kSortWarps * experts;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const uint32_t e = 2u * threadIdx.x + s;
@@ -95,16 +102,25 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
                 in_chunk += count;
             }
             in_all[s] = in_chunk;
-            if (counts != nullptr) {
-                int32_t sum = 0;
-                for (uint32_t c = 0; c < gridDim.x; ++c) {
-                    if (c == blockIdx.x) before[s] = sum;
-                    sum += counts[static_cast<size_t>(c) * experts + e];
-                }
-                in_all[s] = sum;
-            }
+            published[e] = in_chunk;
         }
     }
+    const bool cluster = counts == nullptr && gridDim.x > 1;
+    if (cluster) sm100::cluster_sync();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const uint32_t e = 2u * threadIdx.x + s;
+        if (e < experts && gridDim.x > 1) {
+            int32_t sum = 0;
+            for (uint32_t c = 0; c < gridDim.x; ++c) {
+                if (c == blockIdx.x) before[s] = sum;
+                sum += cluster ? sm100::load_cluster_s32(sm100::map_to_rank(sm100::smem_u32(published + e), c))
+                               : counts[static_cast<size_t>(c) * experts + e];
+            }
+            in_all[s] = sum;
+        }
+    }
+    if (cluster) sm100::cluster_sync();  // no CTA ends while another reads its counts
     const int32_t pair = in_all[0] + in_all[1];
     int32_t inclusive = pair;
 #pragma unroll
@@ -154,32 +170,42 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
 
 constexpr int kRowThreads = 256;
 
-// VEC elements of T move as one: 16 bytes, or a single element where a base or a stride is not a
-// multiple of 16 bytes.
-template <typename T, int VEC>
-struct Pack {
-    T items[VEC];
+// The elements of a row that one thread moves: kVector<T> of them, 16 bytes. Where every base and row
+// stride is a multiple of 16 bytes (ALIGNED) they are contiguous and move as one; otherwise they are
+// 32 apart, so that a warp's loads and stores of single elements stay contiguous.
+template <typename T, bool ALIGNED>
+struct Columns {
+    uint32_t first, width;
+
+    // packs of a row; a warp never crosses the row's end when elements are 32 apart
+    static uint32_t packs(uint32_t width) {
+        constexpr uint32_t kItems = kVector<T>;
+        return ALIGNED ? width / kItems : (width + 32 * kItems - 1) / (32 * kItems) * 32;
+    }
+    __device__ __forceinline__ Columns(uint32_t pack, uint32_t width_)
+        : first(ALIGNED ? pack * kVector<T> : pack / 32 * (32 * kVector<T>) + pack % 32), width(width_) {}
+
+    __device__ __forceinline__ void load(const T *row, Vector<T> &v) const {
+        if constexpr (ALIGNED) {
+            v.bits = load_stream16(row + first);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVector<T>; ++i) {
+                v.items[i] = from_float<T>(0.0f);
+                if (first + 32 * i < width) v.items[i] = __ldg(row + first + 32 * i);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const Vector<T> &v) const {
+        if constexpr (ALIGNED) {
+            *reinterpret_cast<uint4 *>(row + first) = v.bits;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVector<T>; ++i)
+                if (first + 32 * i < width) row[first + 32 * i] = v.items[i];
+        }
+    }
 };
-
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
-    Pack<T, VEC> result;
-    if constexpr (VEC == 1) {
-        result.items[0] = *p;
-    } else {
-        *reinterpret_cast<uint4 *>(&result) = load_stream16(p);
-    }
-    return result;
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &value) {
-    if constexpr (VEC == 1) {
-        *p = value.items[0];
-    } else {
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&value);
-    }
-}
 
 // (row, pack) of a flat index; the division is 32 bits wide where the whole range is.
 __device__ __forceinline__ void split_index(uint64_t index, uint64_t total, uint32_t packs, uint32_t &row, uint32_t &pack) {
@@ -193,55 +219,39 @@ __device__ __forceinline__ void split_index(uint64_t index, uint64_t total, uint
 }
 
 // The rows no expert owns, [offsets[experts], count), become zero.
-template <typename T, int VEC>
-__device__ __forceinline__ void zero_tail(T *rows, size_t stride, uint32_t count, uint32_t packs, const int32_t *end) {
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void zero_tail(T *rows, size_t stride, uint32_t count, uint32_t width, uint32_t packs, const int32_t *end) {
     const int32_t raw = *end;
     const uint32_t first = raw < 0 ? 0u : min(static_cast<uint32_t>(raw), count);
     const uint64_t total = static_cast<uint64_t>(count - first) * packs;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * blockDim.x;
-    Pack<T, VEC> zero;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero.items[i] = from_float<T>(0.0f);
+    Vector<T> zero;
+    zero.bits = make_uint4(0, 0, 0, 0);
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
         uint32_t row, pack;
         split_index(i, total, packs, row, pack);
-        store_pack<T, VEC>(rows + static_cast<size_t>(first + row) * stride + static_cast<size_t>(pack) * VEC, zero);
+        Columns<T, ALIGNED>(pack, width).store(rows + static_cast<size_t>(first + row) * stride, zero);
     }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kRowThreads) expert_gather_kernel(const T *__restrict__ x, size_t x_stride,
-                                                                    uint32_t tokens, uint32_t choices, uint32_t packs,
-                                                                    const int32_t *position, const int32_t *end,
-                                                                    T *rows, size_t rows_stride) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t count = tokens * choices;
-    const uint64_t total = static_cast<uint64_t>(tokens) * packs;
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kRowThreads;
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRowThreads + threadIdx.x; i < total; i += step) {
-        uint32_t token, pack;
-        split_index(i, total, packs, token, pack);
-        const size_t column = static_cast<size_t>(pack) * VEC;
-        const Pack<T, VEC> value = load_pack<T, VEC>(x + static_cast<size_t>(token) * x_stride + column);
-        const int32_t *at = position + static_cast<size_t>(token) * choices;
-        for (uint32_t j = 0; j < choices; ++j) {
-            const uint32_t row = static_cast<uint32_t>(at[j]);  // -1 is out of range as well
-            if (row < count) store_pack<T, VEC>(rows + static_cast<size_t>(row) * rows_stride + column, value);
-        }
-    }
-    zero_tail<T, VEC>(rows, rows_stride, count, packs, end);
-}
-
-// out[t] = sum_j w[t, j] rows[position[t, j]]: fp32 in the order of j, rounded once. The rows of up
-// to kAhead choices are loaded before the first is added.
+// A token's choices are taken kAhead at a time: their rows are known, and where they are read also
+// loaded, before the first is used.
 constexpr int kAhead = 4;
 
-template <typename T, int VEC, bool WEIGHTED>
-__global__ void __launch_bounds__(kRowThreads) expert_combine_kernel(const T *__restrict__ rows, size_t rows_stride,
-                                                                     uint32_t tokens, uint32_t choices, uint32_t packs,
-                                                                     const int32_t *position, const float *weights,
-                                                                     T *out, size_t out_stride) {
+// The row of choice j0 + a, or `count` (no row) when it is dropped or there is none.
+__device__ __forceinline__ void choice_rows(const int32_t *position, uint32_t j0, uint32_t choices, uint32_t count, uint32_t (&row)[kAhead]) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+        const uint32_t at = j0 + a < choices ? static_cast<uint32_t>(__ldg(position + j0 + a)) : count;  // -1 is out of range as well
+        row[a] = min(at, count);
+    }
+}
+
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kRowThreads) expert_gather_kernel(const T *__restrict__ x, size_t x_stride,
+                                                                    uint32_t tokens, uint32_t choices, uint32_t width,
+                                                                    uint32_t packs, const int32_t *__restrict__ position,
+                                                                    const int32_t *end, T *rows, size_t rows_stride) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t count = tokens * choices;
@@ -250,50 +260,80 @@ __global__ void __launch_bounds__(kRowThreads) expert_combine_kernel(const T *__
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRowThreads + threadIdx.x; i < total; i += step) {
         uint32_t token, pack;
         split_index(i, total, packs, token, pack);
-        const size_t column = static_cast<size_t>(pack) * VEC;
-        const size_t at = static_cast<size_t>(token) * choices;
-        float sum[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) sum[v] = 0.0f;
+        const Columns<T, ALIGNED> columns(pack, width);
+        Vector<T> value;
+        columns.load(x + static_cast<size_t>(token) * x_stride, value);
+        const int32_t *at = position + static_cast<size_t>(token) * choices;
         for (uint32_t j0 = 0; j0 < choices; j0 += kAhead) {
-            Pack<T, VEC> value[kAhead];
-            bool present[kAhead];
+            uint32_t row[kAhead];
+            choice_rows(at, j0, choices, count, row);
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (row[a] < count) columns.store(rows + static_cast<size_t>(row[a]) * rows_stride, value);
+        }
+    }
+    zero_tail<T, ALIGNED>(rows, rows_stride, count, width, packs, end);
+}
+
+// out[t] = sum_j w[t, j] rows[position[t, j]]: fp32 in the order of j, rounded once.
+template <typename T, bool ALIGNED, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowThreads) expert_combine_kernel(const T *__restrict__ rows, size_t rows_stride,
+                                                                     uint32_t tokens, uint32_t choices, uint32_t width,
+                                                                     uint32_t packs, const int32_t *__restrict__ position,
+                                                                     const float *__restrict__ weights, T *out,
+                                                                     size_t out_stride) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t count = tokens * choices;
+    const uint64_t total = static_cast<uint64_t>(tokens) * packs;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kRowThreads;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRowThreads + threadIdx.x; i < total; i += step) {
+        uint32_t token, pack;
+        split_index(i, total, packs, token, pack);
+        const Columns<T, ALIGNED> columns(pack, width);
+        const size_t at = static_cast<size_t>(token) * choices;
+        float sum[kVector<T>];
+#pragma unroll
+        for (int v = 0; v < kVector<T>; ++v) sum[v] = 0.0f;
+        for (uint32_t j0 = 0; j0 < choices; j0 += kAhead) {
+            uint32_t row[kAhead];
+            choice_rows(position + at, j0, choices, count, row);
+            Vector<T> value[kAhead];
             float weight[kAhead];
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                const uint32_t row = j0 + a < choices ? static_cast<uint32_t>(position[at + j0 + a]) : count;
-                present[a] = row < count;
                 weight[a] = 1.0f;
-                if (present[a]) {
-                    value[a] = load_pack<T, VEC>(rows + static_cast<size_t>(row) * rows_stride + column);
-                    if (WEIGHTED) weight[a] = weights[at + j0 + a];
+                if (row[a] < count) {
+                    columns.load(rows + static_cast<size_t>(row[a]) * rows_stride, value[a]);
+                    if (WEIGHTED) weight[a] = __ldg(weights + at + j0 + a);
                 }
             }
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                if (!present[a]) continue;
+                if (row[a] >= count) continue;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
+                for (int v = 0; v < kVector<T>; ++v) {
                     const float x = to_float(value[a].items[v]);
                     sum[v] = WEIGHTED ? fmaf(weight[a], x, sum[v]) : sum[v] + x;
                 }
             }
         }
-        Pack<T, VEC> result;
+        Vector<T> result;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) result.items[v] = from_float<T>(sum[v]);
-        store_pack<T, VEC>(out + static_cast<size_t>(token) * out_stride + column, result);
+        for (int v = 0; v < kVector<T>; ++v) result.items[v] = from_float<T>(sum[v]);
+        columns.store(out + static_cast<size_t>(token) * out_stride, result);
     }
 }
 
 // One CTA per token: grad[t] is read once per kAhead choices, each choice's row once; its dot
 // product with grad[t] is summed per thread, then over the CTA in a fixed order.
-template <typename T, int VEC>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kRowThreads)
     expert_combine_backward_kernel(const T *__restrict__ rows, size_t rows_stride, const T *__restrict__ grad,
-                                   size_t grad_stride, uint32_t tokens, uint32_t choices, uint32_t packs,
-                                   const int32_t *position, const int32_t *end, const float *weights, T *grad_rows,
-                                   size_t grad_rows_stride, float *grad_weights) {
+                                   size_t grad_stride, uint32_t tokens, uint32_t choices, uint32_t width, uint32_t packs,
+                                   const int32_t *__restrict__ position, const int32_t *end,
+                                   const float *__restrict__ weights, T *grad_rows, size_t grad_rows_stride,
+                                   float *grad_weights) {
     __shared__ float partial[kRowThreads / 32][kAhead];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -304,31 +344,31 @@ __global__ void __launch_bounds__(kRowThreads)
         const size_t at = static_cast<size_t>(token) * choices;
         for (uint32_t j0 = 0; j0 < choices; j0 += kAhead) {
             uint32_t row[kAhead];
+            choice_rows(position + at, j0, choices, count, row);
             float weight[kAhead], dot[kAhead];
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                row[a] = j0 + a < choices ? static_cast<uint32_t>(position[at + j0 + a]) : count;
-                weight[a] = row[a] < count ? weights[at + j0 + a] : 0.0f;
+                weight[a] = row[a] < count ? __ldg(weights + at + j0 + a) : 0.0f;
                 dot[a] = 0.0f;
             }
             for (uint32_t pack = threadIdx.x; pack < packs; pack += blockDim.x) {
-                const size_t column = static_cast<size_t>(pack) * VEC;
-                const Pack<T, VEC> upstream = load_pack<T, VEC>(g + column);
-                Pack<T, VEC> value[kAhead];
+                const Columns<T, ALIGNED> columns(pack, width);
+                Vector<T> upstream, value[kAhead];
+                columns.load(g, upstream);
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a)
-                    if (row[a] < count) value[a] = load_pack<T, VEC>(rows + static_cast<size_t>(row[a]) * rows_stride + column);
+                    if (row[a] < count) columns.load(rows + static_cast<size_t>(row[a]) * rows_stride, value[a]);
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
                     if (row[a] >= count) continue;
-                    Pack<T, VEC> scaled;
+                    Vector<T> scaled;
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) {
+                    for (int v = 0; v < kVector<T>; ++v) {
                         const float u = to_float(upstream.items[v]);
                         dot[a] = fmaf(to_float(value[a].items[v]), u, dot[a]);
                         scaled.items[v] = from_float<T>(weight[a] * u);
                     }
-                    store_pack<T, VEC>(grad_rows + static_cast<size_t>(row[a]) * grad_rows_stride + column, scaled);
+                    columns.store(grad_rows + static_cast<size_t>(row[a]) * grad_rows_stride, scaled);
                 }
             }
 #pragma unroll
@@ -346,24 +386,28 @@ __global__ void __launch_bounds__(kRowThreads)
             __syncthreads();
         }
     }
-    zero_tail<T, VEC>(grad_rows, grad_rows_stride, count, packs, end);
+    zero_tail<T, ALIGNED>(grad_rows, grad_rows_stride, count, width, packs, end);
 }
 
 // ---- launches -----------------------------------------------------------------------------------
 
 template <typename... Parameters, typename... Arguments>
-cudaError_t launch(void (*kernel)(Parameters...), uint32_t blocks, uint32_t threads, size_t shared, cudaStream_t stream,
-                   Arguments... arguments) {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch(void (*kernel)(Parameters...), uint32_t blocks, uint32_t threads, size_t shared, uint32_t cluster,
+                   cudaStream_t stream, Arguments... arguments) {
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = shared;
     config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
 }
 
@@ -383,63 +427,64 @@ cudaError_t sort_typed(const Id *ids, uint32_t total, uint32_t experts, int32_t 
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
         return cudaFuncSetAttribute(expert_scatter_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(kSortWarps * kMaxExperts * sizeof(int32_t)));
+                                    static_cast<int>((kSortWarps + 1) * kMaxExperts * sizeof(int32_t)));
     });
     if (error != cudaSuccess) return error;
     const uint32_t chunk = sort_chunk(total);
     const uint32_t chunks = total == 0 ? 1u : (total + chunk - 1) / chunk;
-    if (chunks > 1) {
+    const uint32_t cluster = chunks <= kSortCluster ? chunks : 1u;
+    if (chunks > cluster) {
         const cudaError_t counted =
-            launch(expert_count_kernel<Id>, chunks, kSortThreads, 0, stream, ids, total, chunk, experts, counts);
+            launch(expert_count_kernel<Id>, chunks, kSortThreads, 0, 1, stream, ids, total, chunk, experts, counts);
         if (counted != cudaSuccess) return counted;
     }
-    return launch(expert_scatter_kernel<Id>, chunks, kSortThreads, kSortWarps * experts * sizeof(int32_t), stream, ids,
-                  total, chunk, experts, chunks > 1 ? counts : nullptr, offsets, source, position);
+    return launch(expert_scatter_kernel<Id>, chunks, kSortThreads, (kSortWarps + 1) * experts * sizeof(int32_t), cluster, stream,
+                  ids, total, chunk, experts, chunks > cluster ? counts : nullptr, offsets, source, position);
 }
 
-template <typename T, int VEC>
+template <typename T, bool ALIGNED>
 cudaError_t gather_typed(const void *x, size_t x_stride, uint32_t tokens, uint32_t choices, uint32_t width,
                          const int32_t *position, const int32_t *end, void *rows, size_t rows_stride, int sm_count,
                          cudaStream_t stream) {
-    const uint32_t packs = width / VEC;
-    return launch(expert_gather_kernel<T, VEC>, row_blocks(static_cast<uint64_t>(tokens) * packs, sm_count), kRowThreads,
-                  0, stream, static_cast<const T *>(x), x_stride, tokens, choices, packs, position, end,
+    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
+    return launch(expert_gather_kernel<T, ALIGNED>, row_blocks(static_cast<uint64_t>(tokens) * packs, sm_count), kRowThreads,
+                  0, 1, stream, static_cast<const T *>(x), x_stride, tokens, choices, width, packs, position, end,
                   static_cast<T *>(rows), rows_stride);
 }
 
-template <typename T, int VEC>
+template <typename T, bool ALIGNED>
 cudaError_t combine_typed(const void *rows, size_t rows_stride, uint32_t tokens, uint32_t choices, uint32_t width,
                           const int32_t *position, const float *weights, void *out, size_t out_stride, int sm_count,
                           cudaStream_t stream) {
-    const uint32_t packs = width / VEC;
+    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
     const uint32_t blocks = row_blocks(static_cast<uint64_t>(tokens) * packs, sm_count);
-    auto kernel = weights != nullptr ? expert_combine_kernel<T, VEC, true> : expert_combine_kernel<T, VEC, false>;
-    return launch(kernel, blocks, kRowThreads, 0, stream, static_cast<const T *>(rows), rows_stride, tokens, choices,
-                  packs, position, weights, static_cast<T *>(out), out_stride);
+    auto kernel = weights != nullptr ? expert_combine_kernel<T, ALIGNED, true> : expert_combine_kernel<T, ALIGNED, false>;
+    return launch(kernel, blocks, kRowThreads, 0, 1, stream, static_cast<const T *>(rows), rows_stride, tokens, choices,
+                  width, packs, position, weights, static_cast<T *>(out), out_stride);
 }
 
-template <typename T, int VEC>
+template <typename T, bool ALIGNED>
 cudaError_t combine_backward_typed(const void *rows, size_t rows_stride, const void *grad, size_t grad_stride,
                                    uint32_t tokens, uint32_t choices, uint32_t width, const int32_t *position,
                                    const int32_t *end, const float *weights, void *grad_rows, size_t grad_rows_stride,
                                    float *grad_weights, int sm_count, cudaStream_t stream) {
-    const uint32_t packs = width / VEC;
+    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
     uint32_t threads = 32;
     while (threads < kRowThreads && threads < packs) threads *= 2;
     const uint32_t most = static_cast<uint32_t>(sm_count) * 64u;
-    return launch(expert_combine_backward_kernel<T, VEC>, tokens < most ? tokens : most, threads, 0, stream,
+    return launch(expert_combine_backward_kernel<T, ALIGNED>, tokens < most ? tokens : most, threads, 0, 1, stream,
                   static_cast<const T *>(rows), rows_stride, static_cast<const T *>(grad), grad_stride, tokens, choices,
-                  packs, position, end, weights, static_cast<T *>(grad_rows), grad_rows_stride, grad_weights);
+                  width, packs, position, end, weights, static_cast<T *>(grad_rows), grad_rows_stride, grad_weights);
 }
 
-// Calls f<T, VEC>(...) for the element type, 16-byte vectors where every row allows them.
-#define QPUCUDA_ROWS_DISPATCH(f, type, vector, ...)                                          \
-    switch (type) {                                                                          \
-        case QPUCUDA_DTYPE_F32: return vector ? f<float, 4>(__VA_ARGS__) : f<float, 1>(__VA_ARGS__);             \
-        case QPUCUDA_DTYPE_BF16:                                                             \
-            return vector ? f<__nv_bfloat16, 8>(__VA_ARGS__) : f<__nv_bfloat16, 1>(__VA_ARGS__);                 \
-        case QPUCUDA_DTYPE_F16: return vector ? f<__half, 8>(__VA_ARGS__) : f<__half, 1>(__VA_ARGS__);           \
-    }                                                                                        \
+// Calls f<T, ALIGNED>(...) for the element type.
+#define QPUCUDA_ROWS_DISPATCH(f, type, aligned, ...)                                                              \
+    switch (type) {                                                                                               \
+        case QPUCUDA_DTYPE_F32: return aligned ? f<float, true>(__VA_ARGS__) : f<float, false>(__VA_ARGS__);      \
+        case QPUCUDA_DTYPE_BF16:                                                                                  \
+            return aligned ? f<__nv_bfloat16, true>(__VA_ARGS__) : f<__nv_bfloat16, false>(__VA_ARGS__);          \
+        case QPUCUDA_DTYPE_F16: return aligned ? f<__half, true>(__VA_ARGS__) : f<__half, false>(__VA_ARGS__);    \
+    }                                                                                                             \
     return cudaErrorInvalidValue
 
 size_t item_bytes(int type) { return type == QPUCUDA_DTYPE_F32 ? 4 : 2; }
@@ -451,7 +496,7 @@ size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts
     if (total == 0 || total > 0x7FFFFFFFull) return 0;
     const uint32_t chunk = sort_chunk(static_cast<uint32_t>(total));
     const uint32_t chunks = static_cast<uint32_t>((total + chunk - 1) / chunk);
-    return chunks > 1 ? static_cast<size_t>(chunks) * experts * sizeof(int32_t) : 0;
+    return chunks > kSortCluster ? static_cast<size_t>(chunks) * experts * sizeof(int32_t) : 0;
 }
 
 cudaError_t launch_expert_sort(const void *ids, bool ids_64, uint32_t tokens, uint32_t choices, uint32_t experts,
@@ -468,8 +513,8 @@ cudaError_t launch_expert_gather(const void *x, int type, size_t x_stride, uint3
                                  uint32_t width, const int32_t *position, const int32_t *offsets, uint32_t experts,
                                  void *rows, size_t rows_stride, int sm_count, cudaStream_t stream) {
     const size_t item = item_bytes(type);
-    const bool vector = width * item % 16u == 0 && vector_rows(x, x_stride, item) && vector_rows(rows, rows_stride, item);
-    QPUCUDA_ROWS_DISPATCH(gather_typed, type, vector, x, x_stride, tokens, choices, width, position, offsets + experts,
+    const bool aligned = width * item % 16u == 0 && vector_rows(x, x_stride, item) && vector_rows(rows, rows_stride, item);
+    QPUCUDA_ROWS_DISPATCH(gather_typed, type, aligned, x, x_stride, tokens, choices, width, position, offsets + experts,
                           rows, rows_stride, sm_count, stream);
 }
 
@@ -477,8 +522,8 @@ cudaError_t launch_expert_combine(const void *rows, int type, size_t rows_stride
                                   uint32_t width, const int32_t *position, const float *weights, void *out,
                                   size_t out_stride, int sm_count, cudaStream_t stream) {
     const size_t item = item_bytes(type);
-    const bool vector = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) && vector_rows(out, out_stride, item);
-    QPUCUDA_ROWS_DISPATCH(combine_typed, type, vector, rows, rows_stride, tokens, choices, width, position, weights, out,
+    const bool aligned = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) && vector_rows(out, out_stride, item);
+    QPUCUDA_ROWS_DISPATCH(combine_typed, type, aligned, rows, rows_stride, tokens, choices, width, position, weights, out,
                           out_stride, sm_count, stream);
 }
 
@@ -488,9 +533,9 @@ cudaError_t launch_expert_combine_backward(const void *rows, int type, size_t ro
                                            const float *weights, void *grad_rows, size_t grad_rows_stride,
                                            float *grad_weights, int sm_count, cudaStream_t stream) {
     const size_t item = item_bytes(type);
-    const bool vector = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) &&
+    const bool aligned = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) &&
                         vector_rows(grad, grad_stride, item) && vector_rows(grad_rows, grad_rows_stride, item);
-    QPUCUDA_ROWS_DISPATCH(combine_backward_typed, type, vector, rows, rows_stride, grad, grad_stride, tokens, choices,
+    QPUCUDA_ROWS_DISPATCH(combine_backward_typed, type, aligned, rows, rows_stride, grad, grad_stride, tokens, choices,
                           width, position, offsets + experts, weights, grad_rows, grad_rows_stride, grad_weights,
                           sm_count, stream);
 }

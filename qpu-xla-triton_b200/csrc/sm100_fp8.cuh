@@ -131,6 +131,11 @@ __device__ __forceinline__ float load_cluster(uint32_t cluster_address) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address) : "memory");
     return v;
 }
+__device__ __forceinline__ int32_t load_cluster_s32(uint32_t cluster_address) {
+    int32_t v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_address) : "memory");
+    return v;
+}
 __device__ __forceinline__ float4 load_cluster4(uint32_t cluster_address) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_address) : "memory");

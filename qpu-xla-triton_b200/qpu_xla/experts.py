@@ -19,7 +19,6 @@ from typing import Any, Self
 
 import torch
 
-from qpu_xla import _native
 from qpu_xla.device import Device
 from qpu_xla.fp8 import (
     MAX_EXPERTS,
@@ -28,6 +27,7 @@ from qpu_xla.fp8 import (
     check_matrix,
     dtype_code,
     launch,
+    made,
     require_cuda,
 )
 
@@ -89,17 +89,19 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     if expert_ids.numel() >= 2**31:
         raise ValueError("sort_tokens takes fewer than 2**31 choices")
     ids = expert_ids.contiguous()
-    tokens, choices = (int(extent) for extent in ids.shape)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=torch_device)
-    source = torch.empty(tokens * choices, dtype=torch.int32, device=torch_device)
-    position = torch.empty((tokens, choices), dtype=torch.int32, device=torch_device)
-    needed = int(_native.load().qpucuda_expert_sort_workspace(tokens, choices, experts))
+    tokens, choices = ids.shape
+    total = tokens * choices
+    # one allocation for the three tables
+    offsets, source, position = torch.empty(experts + 1 + 2 * total, dtype=torch.int32, device=torch_device).split_with_sizes(
+        [experts + 1, total, total]
+    )
+    needed = device.backend.native.library.qpucuda_expert_sort_workspace(tokens, choices, experts)  # type: ignore[attr-defined]
     workspace = torch.empty(needed, dtype=torch.uint8, device=torch_device) if needed else None
     launch(
-        device, "qpucuda_expert_sort", ids.data_ptr(), int(ids.dtype == torch.int64), tokens, choices, experts, offsets.data_ptr(),
+        device, "qpucuda_expert_sort", ids.data_ptr(), ids.dtype == torch.int64, tokens, choices, experts, offsets.data_ptr(),
         source.data_ptr(), position.data_ptr(), None if workspace is None else workspace.data_ptr(), needed,
     )
-    return ExpertOrder(offsets, source, position)
+    return made(ExpertOrder, offsets=offsets, source=source, position=position.view(tokens, choices))
 
 
 def _destination(out: Any, rows: int, width: int, read: Any, torch_device: Any, what: str) -> tuple[Any, int]:

@@ -84,6 +84,14 @@ def launch(device: Device, name: str, *args: Any, stream: int | None = None) -> 
     backend.call(name, args, backend.current_stream_handle if stream is None else stream)  # type: ignore[attr-defined]
 
 
+def made(cls: type, **fields: Any) -> Any:
+    """A frozen dataclass around tensors this package has just allocated, without its checks."""
+    result = object.__new__(cls)
+    for name, value in fields.items():
+        object.__setattr__(result, name, value)
+    return result
+
+
 @dataclass(frozen=True, slots=True)
 class QuantizedRowsFP8:
     """e4m3 rows ``[M, K]`` and their fp32 scales ``[M, ceil(K / 128)]`` (any strides)."""
@@ -184,7 +192,7 @@ def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> Qu
     if rows:
         desc = _quantize_desc(source, stride, cols, gated, rows, values.data_ptr(), q_stride, scales.data_ptr(), (groups_of(cols), 1))
         launch(device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
-    return QuantizedRowsFP8(values if q_stride == cols else values[:, :cols], scales)
+    return made(QuantizedRowsFP8, values=values if q_stride == cols else values[:, :cols], scales=scales)
 
 
 class _PreparedFP8:

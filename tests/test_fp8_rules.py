@@ -92,9 +92,9 @@ def test_null_arguments_are_rejected_without_a_device() -> None:
     assert library.qpucuda_expert_combine_backward(None, None, 0, 0, None, 0, 0, 0, 0, None, None, 0, None, None, 0, None) == _native.Status.INVALID_ARGUMENT
 
 
-def test_sort_workspace_is_only_needed_past_one_chunk() -> None:
+def test_sort_workspace_is_only_needed_past_one_cluster() -> None:
     size = _native.load().qpucuda_expert_sort_workspace
-    assert size(1, 1, 1) == 0 and size(512, 8, 64) == 0
-    assert size(4096, 8, 64) > 0 and size(4096, 8, 64) % (4 * 64) == 0
+    assert size(1, 1, 1) == 0 and size(4096, 8, 64) == 0
+    assert size(4097, 8, 64) > 0 and size(4097, 8, 64) % (4 * 64) == 0
     assert size(0, 8, 64) == 0 and size(8, 0, 64) == 0 and size(8, 8, 1025) == 0
     assert size(2**31, 2, 4) == 0
