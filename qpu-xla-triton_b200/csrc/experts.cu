@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortAhead = 8;
 // A chunk is one CTA's share: the CTAs of one cluster, or above kSortCluster chunks a grid whose CTAs
 // each add up the counts of all chunks, at most kSortMaxChunks of them.
 constexpr uint32_t kSortChunk = 4096;
@@ -81,9 +82,14 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
     const uint32_t warp_begin = begin + warp * share;
     const uint32_t warp_end = min(end, warp_begin + share);
     int32_t *own = next + warp * experts;
-    for (uint32_t i = warp_begin + lane; i < warp_end; i += 32) {
-        const uint32_t e = expert_of(ids, i, warp_end, experts);
-        if (e < experts) atomicAdd(&own[e], 1);
+    // kSortAhead steps of 32 ids are loaded before the first is used (both passes).
+    for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
+        uint32_t e[kSortAhead];
+#pragma unroll
+        for (int a = 0; a < kSortAhead; ++a) e[a] = expert_of(ids, i0 + 32 * a + lane, warp_end, experts);
+#pragma unroll
+        for (int a = 0; a < kSortAhead; ++a)
+            if (e[a] < experts) atomicAdd(&own[e[a]], 1);
     }
     __syncthreads();
     // Thread t takes experts 2t and 2t + 1: their counts over this chunk's warps become offsets
@@ -146,19 +152,24 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = kept;
-    for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32) {
-        const uint32_t i = i0 + lane;
-        const uint32_t e = expert_of(ids, i, warp_end, experts);
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
-        const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
-        int32_t row = -1;
-        if (e < experts) row = own[e] + static_cast<int32_t>(earlier);
-        __syncwarp();
-        if (e < experts && earlier == 0) own[e] += __popc(same);
-        __syncwarp();
-        if (i < warp_end) {
-            position[i] = row;
-            if (row >= 0) source[row] = static_cast<int32_t>(i);
+    for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
+        uint32_t e[kSortAhead];
+#pragma unroll
+        for (int a = 0; a < kSortAhead; ++a) e[a] = expert_of(ids, i0 + 32 * a + lane, warp_end, experts);
+#pragma unroll
+        for (int a = 0; a < kSortAhead; ++a) {
+            const uint32_t i = i0 + 32 * a + lane;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, e[a]);
+            const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
+            int32_t row = -1;
+            if (e[a] < experts) row = own[e[a]] + static_cast<int32_t>(earlier);
+            __syncwarp();
+            if (e[a] < experts && earlier == 0) own[e[a]] += __popc(same);
+            __syncwarp();
+            if (i < warp_end) {
+                position[i] = row;
+                if (row >= 0) source[row] = static_cast<int32_t>(i);
+            }
         }
     }
     const uint32_t stride = gridDim.x * kSortThreads;

@@ -28,6 +28,7 @@ from qpu_xla.fp8 import (
     dtype_code,
     launch,
     made,
+    new_matrix,
     require_cuda,
 )
 
@@ -108,7 +109,7 @@ def _destination(out: Any, rows: int, width: int, read: Any, torch_device: Any, 
     """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride. It may not overlap
     ``read``: the kernels read and write in no particular order."""
     if out is None:
-        return torch.empty((rows, width), dtype=read.dtype, device=torch_device), max(width, 1)
+        return new_matrix(rows, width, read.dtype, torch_device), max(width, 1)
     if out.dtype != read.dtype:
         raise ValueError(f"{what} must have the type of its source")
     stride = check_matrix(out, torch_device, what, rows, width)[2]
@@ -188,8 +189,8 @@ def combine_tokens_backward(device: Device, rows: Any, weights: Any, grad: Any, 
     _, width, stride = check_matrix(rows, torch_device, f"{name} rows", tokens * choices)
     grad_stride = check_matrix(grad, torch_device, f"{name} grad", tokens, width)[2]
     _check_weights(weights, order, torch_device, name)
-    grad_rows = torch.empty((tokens * choices, width), dtype=rows.dtype, device=torch_device)
-    grad_weights = torch.empty((tokens, choices), dtype=torch.float32, device=torch_device)
+    grad_rows = new_matrix(tokens * choices, width, rows.dtype, torch_device)
+    grad_weights = new_matrix(tokens, choices, torch.float32, torch_device)
     if tokens and width:
         launch(
             device, "qpucuda_expert_combine_backward", rows.data_ptr(), code, stride, grad.data_ptr(), grad_stride, tokens, choices, width,

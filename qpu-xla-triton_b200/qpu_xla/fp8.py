@@ -78,6 +78,11 @@ def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = N
     return have_rows, have_cols, stride
 
 
+def new_matrix(rows: int, cols: int, dtype: Any, torch_device: Any) -> Any:
+    """An uninitialised row-major matrix (``empty_strided`` costs the host a third less than ``empty``)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=torch_device)
+
+
 def launch(device: Device, name: str, *args: Any, stream: int | None = None) -> None:
     """Call one libqpucuda entry point on ``stream`` (a cudaStream_t; default: the device's current stream)."""
     backend = device.backend
@@ -187,8 +192,8 @@ def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> Qu
         raise ValueError("quantize_rows_fp8 source must have columns, an even number of them when gated")
     cols = cols // 2 if gated else cols
     q_stride = (cols + 15) // 16 * 16
-    values = torch.empty((rows, q_stride), dtype=torch.float8_e4m3fn, device=torch_device)
-    scales = torch.empty((rows, groups_of(cols)), dtype=torch.float32, device=torch_device)
+    values = new_matrix(rows, q_stride, torch.float8_e4m3fn, torch_device)
+    scales = new_matrix(rows, groups_of(cols), torch.float32, torch_device)
     if rows:
         desc = _quantize_desc(source, stride, cols, gated, rows, values.data_ptr(), q_stride, scales.data_ptr(), (groups_of(cols), 1))
         launch(device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
@@ -255,7 +260,7 @@ class _PreparedFP8:
         if out is None:
             dtype = default if dtype is None else dtype
             dtype_code(dtype, f"{self._name} output")
-            return torch.empty((rows, self.output_count), dtype=dtype, device=self._torch_device), self.output_count
+            return new_matrix(rows, self.output_count, dtype, self._torch_device), self.output_count
         if dtype is not None and out.dtype != dtype:
             raise ValueError(f"{self._name} out and dtype differ")
         dtype_code(out.dtype, f"{self._name} output")
@@ -279,7 +284,7 @@ class _PreparedFP8:
         The weight is older than the quantizer's launch, so the product may read it early; so are the
         offsets."""
         padded = self._padded
-        scratch = torch.empty(rows * (padded + 4 * self._groups), dtype=torch.uint8, device=self._torch_device)
+        scratch = new_matrix(rows, padded + 4 * self._groups, torch.uint8, self._torch_device)
         values = scratch.data_ptr()
         scales = values + rows * padded
         quantize = _native.Fp8QuantizeDesc(
