@@ -51,7 +51,7 @@ typedef struct qpucuda_fp8_quantize_desc {
     uint32_t row_divisor;
     uint32_t source_rows;
     uint8_t *q;              /* [rows] rows of q_stride bytes, 16-byte aligned */
-    size_t q_stride;         /* a multiple of 16, at least cols; bytes past cols may be zeroed */
+    size_t q_stride;         /* a multiple of 16, at least cols; up to 7 bytes past cols are zeroed */
     float *scales;           /* group g of row r at r * scale_row_stride + g * scale_group_stride */
     size_t scale_row_stride;
     size_t scale_group_stride;
@@ -70,8 +70,8 @@ qpucuda_status qpucuda_fp8_quantize_blocks(
     float *scales);
 
 typedef struct qpucuda_fp8_gemm_desc {
-    const uint8_t *a;        /* e4m3 [rows] of a_stride bytes */
-    size_t a_stride;         /* multiples of 16, bases 16-byte aligned (as w) */
+    const uint8_t *a;        /* e4m3 [rows] of a_stride bytes; bytes past k do not count */
+    size_t a_stride;         /* a multiple of 16, base 16-byte aligned (as w) */
     const float *a_scales;   /* strided as in qpucuda_fp8_quantize_desc */
     size_t a_scale_row_stride;
     size_t a_scale_group_stride;

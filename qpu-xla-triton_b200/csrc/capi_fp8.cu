@@ -54,6 +54,7 @@ qpucuda_status check_quantize(qpucuda_context *context, const qpucuda_fp8_quanti
 qpucuda_status check_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc) {
     const uint64_t matrices = desc->experts != 0 ? desc->experts : 1u;
     if (!known_type(desc->out_type) || desc->n == 0 || desc->k == 0 || desc->k > INT32_MAX || desc->rows > INT32_MAX ||
+        desc->n > INT32_MAX / 4 ||
         desc->a == nullptr || desc->a_scales == nullptr || desc->w == nullptr || desc->w_scales == nullptr ||
         desc->out == nullptr || desc->a_stride < desc->k || desc->w_stride < desc->k || desc->a_stride % 16 != 0 ||
         desc->w_stride % 16 != 0 || !aligned(desc->a, 16) || !aligned(desc->w, 16) || desc->out_stride < desc->n ||

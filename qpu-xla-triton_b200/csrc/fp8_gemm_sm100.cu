@@ -900,8 +900,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (row0 >= tile.row_end || !block_inside) continue;
             constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));
             const uint32_t rows = tile.row_end - row0;
-            // rows past the last expert's would be overwritten by a copy of the whole box; rows past
-            // the output are cut off by it
+            // Rows past an expert's would be overwritten by a copy of the whole box; rows past the output
+            // are cut off by it. So are columns, but only to 16 bytes: the last, partly filled box goes
+            // the other way.
             const bool whole = params.tma_store != 0 && (params.experts == 0 || rows >= 32);
 #pragma unroll
             for (int c = 0; c < kWideN / 2; c += kChunk) {
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     v[i + 1] = high(acc[(c + i) / 2]);
                 }
                 add_bias(params, n, v);
-                store_box<Out>(buffer_out + (c / kChunk & 1) * kWideBoxBytes, v, whole ? &map_out : nullptr,
+                store_box<Out>(buffer_out + (c / kChunk & 1) * kWideBoxBytes, v, whole && n + kChunk <= params.n ? &map_out : nullptr,
                                static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n, params.out_stride,
                                static_cast<int>(row0), n, rows, params.n - n, vector, lane);
             }

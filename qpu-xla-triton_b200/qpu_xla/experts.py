@@ -9,7 +9,8 @@ floating-point values.
 
 The functions run on the current stream of their device. There is no autograd:
 each step's gradient is a function of its own (``gather_tokens_backward``,
-``combine_tokens_backward``).
+``combine_tokens_backward``), and tensors that require grad are refused while
+gradients are recorded (inside an ``autograd.Function`` they are not).
 """
 
 from __future__ import annotations
@@ -158,6 +159,8 @@ def _check_weights(weights: Any, order: ExpertOrder, torch_device: Any, name: st
         raise ValueError(f"{name} requires contiguous float32 weights [tokens, choices]")
     if weights.device != torch_device:
         raise ValueError(f"{name} weights must be on {torch_device}")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} weights require grad, and there is no autograd here")
 
 
 def gather_tokens_backward(device: Device, grad_rows: Any, order: ExpertOrder, out: Any = None) -> Any:

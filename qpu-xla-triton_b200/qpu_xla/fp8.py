@@ -12,8 +12,8 @@ that holds a NaN or an infinity dequantizes to NaN, and so do that row's outputs
 
 Everything here runs on the current stream of the plan's device, allocates its
 scratch from PyTorch per call (so calls on several streams, and several captured
-CUDA graphs, share no workspace) and has no CPU path. There is no autograd:
-results carry no gradient.
+CUDA graphs, share no workspace) and has no CPU path. There is no autograd: a
+source that requires grad is refused while gradients are recorded.
 """
 
 from __future__ import annotations
@@ -67,6 +67,8 @@ def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = N
         raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}], not {list(shape)}")
     if tensor.device != torch_device:
         raise ValueError(f"{what} must be on {torch_device}, the device it is used with")
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires grad, and there is no autograd here: call under torch.no_grad() or from an autograd.Function")
     have_rows, have_cols = shape
     stride, inner = tensor.stride()
     if inner != 1 and have_cols > 1:

@@ -21,8 +21,9 @@ from qpu_xla.fp8 import PreparedFP8Experts, quantize_blocks_fp8, quantize_rows_f
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
-# tokens, choices, experts: one of each, more experts than a warp, several chunks of the sort, one expert
-ROUTINGS = [(1, 1, 1), (5, 2, 3), (8, 8, 64), (100, 3, 7), (33, 1, 1024), (1000, 8, 256), (3000, 4, 40), (40000, 2, 1), (2048, 2, 8)]
+# tokens, choices, experts: one of each, more experts than a warp, several chunks of the sort in one cluster
+# (the largest: 4096 x 8) and in a grid, one expert
+ROUTINGS = [(1, 1, 1), (5, 2, 3), (8, 8, 64), (100, 3, 7), (33, 1, 1024), (1000, 8, 256), (3000, 4, 40), (40000, 2, 1), (2048, 2, 8), (4096, 8, 1024), (4097, 8, 1024), (70000, 8, 100)]
 
 
 def draw(shape, dtype=torch.float32, seed=0) -> torch.Tensor:
@@ -278,6 +279,8 @@ def test_refusals_on_the_gpu(cuda_device) -> None:
         lambda: combine_tokens(cuda_device, rows, weights, order, out=rows[:4]),
         lambda: combine_tokens_backward(cuda_device, rows, weights, x.half(), order),
         lambda: combine_tokens_backward(cuda_device, rows, weights, x[:, :8], order),
+        lambda: gather_tokens(cuda_device, x.clone().requires_grad_(), order),
+        lambda: combine_tokens(cuda_device, rows, weights.clone().requires_grad_(), order),
     ):
         with pytest.raises(ValueError):
             call()

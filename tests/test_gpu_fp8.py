@@ -144,6 +144,51 @@ def test_linear_shapes(cuda_device, rows, n, k) -> None:
         check_product(plan.forward(x), exact, magnitude, k)
 
 
+# One tile shape of the product each: a few rows, with and without a split K; few wide tiles whose K is
+# split in 4 and in 2; wide tiles alone and in pairs, more of them than SMs; a ragged last tile everywhere.
+KERNELS = [(5, 300, 4096), (30, 40000, 300), (200, 1000, 4096), (333, 5000, 2049), (640, 9000, 300), (1023, 5001, 384), (1023, 10000, 130)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, n, k", KERNELS)
+def test_every_kernel_and_output_layout(cuda_device, dtype, rows, n, k) -> None:
+    """Contiguous, aligned and unaligned outputs inside a wider tensor, whose rest stays as it was."""
+    weight = blocks(cuda_device, n, k)
+    bias = draw((n,), seed=8)
+    x = draw((rows, k), seed=rows)
+    values, scales = ref.quantize_rows(x)
+    exact, magnitude = ref.product(values, scales, weight.values, weight.scales)
+    exact, magnitude = exact + bias.double(), magnitude + bias.double().abs()
+    with PreparedFP8Linear(cuda_device, weight, bias=bias) as plan:
+        y = plan.forward(x, dtype=dtype)
+        check_product(y, exact, magnitude, k)
+        assert torch.equal(plan.forward(x, dtype=dtype), y)
+        for start, extra in ((8, 16 - n % 8), (3, 7)):
+            wide = torch.full((rows + 2, n + start + extra), 7.0, dtype=dtype, device="cuda")
+            plan.forward(x, out=wide[1:-1, start : start + n])
+            assert torch.equal(wide[1:-1, start : start + n], y)
+            wide[1:-1, start : start + n] = 7.0
+            assert (wide == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "counts, trailing, n, k",
+    [([130, 0, 1, 255, 40], 9, 300, 4096), ([70, 90], 3, 1000, 2048), ([500, 0, 700, 129, 640], 40, 3000, 300), ([1100, 1500, 900, 1025], 17, 3001, 256), ([1100, 1500, 900, 1025], 17, 3200, 256)],
+)
+def test_every_kernel_with_experts(cuda_device, dtype, counts, trailing, n, k) -> None:
+    weight, x, offsets, exact, magnitude = expert_case(cuda_device, counts, n, k, trailing)
+    with PreparedFP8Experts(cuda_device, weight) as plan:
+        y = plan.forward(x, offsets, dtype=dtype)
+        check_product(y, exact, magnitude, k)
+        assert (y[sum(counts) :] == 0).all()
+        wide = torch.full((x.shape[0] + 2, n + 16 - n % 8), 7.0, dtype=dtype, device="cuda")
+        plan.forward(x, offsets, out=wide[1:-1, 8 : 8 + n])
+        assert torch.equal(wide[1:-1, 8 : 8 + n], y)
+        wide[1:-1, 8 : 8 + n] = 7.0
+        assert (wide == 7.0).all()
+
+
 @pytest.mark.parametrize("source", DTYPES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [3, 150, 520])
@@ -184,6 +229,18 @@ def test_quantized_rows_give_the_same_product(cuda_device, rows) -> None:
         moved = quantize_rows_fp8(cuda_device, x)
         transposed = QuantizedRowsFP8(moved.values, moved.scales.t().contiguous().t())
         assert torch.equal(plan.forward_quantized(transposed), plan.forward(x))
+
+
+@pytest.mark.parametrize("rows", [4, 30, 300])
+@pytest.mark.parametrize("k", [1, 17, 100, 250])
+def test_bytes_behind_a_row_do_not_count(cuda_device, rows, k) -> None:
+    """Quantized rows end inside their last 16 bytes; whatever lies behind (NaN here) is not read as theirs."""
+    values = torch.full((rows, (k + 15) // 16 * 16), 0x7F, dtype=torch.uint8, device="cuda")
+    values[:, :k] = 0x38  # 1.0
+    ones = QuantizedBlocksFP8(torch.ones((300, k), device="cuda").to(torch.float8_e4m3fn), torch.ones((3, -(-k // 128)), device="cuda"))
+    with PreparedFP8Linear(cuda_device, ones) as plan:
+        y = plan.forward_quantized(QuantizedRowsFP8(values.view(torch.float8_e4m3fn)[:, :k], torch.ones((rows, -(-k // 128)), device="cuda")))
+        assert (y == k).all()
 
 
 @pytest.mark.parametrize("rows", [20, 300])
@@ -273,7 +330,7 @@ def test_experts_nan_rows_do_not_reach_a_neighbouring_expert(cuda_device) -> Non
     check_product(y[9:], exact[9:], magnitude[9:], 256)
 
 
-@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("rows", [4, 200, 2100])
 def test_one_plan_on_two_streams_and_in_two_graphs(cuda_device, rows) -> None:
     weight = blocks(cuda_device, 1024, 1024)
     inputs = [draw((rows, 1024), torch.bfloat16, seed=s) for s in range(2)]
@@ -318,7 +375,7 @@ def test_execute_on_a_queue(cuda_device) -> None:
 
 
 def test_results_repeat_bit_for_bit(cuda_device) -> None:
-    for rows, n, k in ((1, 2048, 2048), (50, 640, 4096), (400, 1000, 1500)):
+    for rows, n, k in ((1, 2048, 2048), (50, 640, 4096), (400, 1000, 1500), (1024, 6000, 512)):
         weight = blocks(cuda_device, n, k)
         x = draw((rows, k), seed=rows)
         with PreparedFP8Linear(cuda_device, weight) as plan:
@@ -338,6 +395,10 @@ def test_refusals_on_the_gpu(cuda_device) -> None:
                 plan.forward(x, out=out)
         with pytest.raises(ValueError, match="16-byte"):
             plan.forward_quantized(QuantizedRowsFP8(torch.empty((4, 132), dtype=torch.float8_e4m3fn, device="cuda")[:, :128], torch.ones((4, 1), device="cuda")))
+        with pytest.raises(ValueError, match="requires grad"):
+            plan.forward(x.clone().requires_grad_())
+        with torch.no_grad():
+            assert torch.equal(plan.forward(x.clone().requires_grad_()), plan.forward(x))
     with pytest.raises(RuntimeError, match="closed"):
         plan.forward(x)
     with PreparedFP8Experts(cuda_device, blocks(cuda_device, 64, 128, experts=2)) as plan:
