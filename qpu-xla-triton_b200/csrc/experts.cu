@@ -20,18 +20,21 @@ namespace {
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortAhead = 8;
-// A chunk is one CTA's share: the CTAs of one cluster, or above kSortCluster chunks a grid whose CTAs
-// each add up the counts of all chunks, at most kSortMaxChunks of them.
+// A chunk is one CTA's share. Up to kSortCluster CTAs of one cluster share kSortCluster * kSortChunk
+// choices, whose ranks stay in registers; above, the CTAs of a grid each add up the counts of all
+// chunks, at most kSortMaxChunks of them, and rank their choices a second time.
 constexpr uint32_t kSortChunk = 4096;
 constexpr uint32_t kSortCluster = 8;
 constexpr uint32_t kSortMaxChunks = 64;
 constexpr uint32_t kMaxExperts = QPUCUDA_MAX_EXPERTS;
+static_assert(kSortChunk == kSortThreads * kSortAhead, "a cluster's choices stay in registers");
+
+bool sort_in_cluster(uint32_t total) { return total <= kSortCluster * kSortChunk; }
 
 uint32_t sort_chunk(uint32_t total) {
-    if (total <= kSortCluster * kSortChunk) return kSortChunk;
-    const uint32_t least = (total + kSortMaxChunks - 1) / kSortMaxChunks;
-    const uint32_t chunk = least > kSortChunk ? least : kSortChunk;
-    return (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
+    const uint32_t parts = sort_in_cluster(total) ? kSortCluster : kSortMaxChunks;
+    const uint32_t chunk = (total + parts - 1) / parts;
+    return (chunk == 0 ? 1 : (chunk + kSortThreads - 1) / kSortThreads) * kSortThreads;
 }
 
 template <typename Id>
@@ -61,35 +64,59 @@ __global__ void __launch_bounds__(kSortThreads) expert_count_kernel(const Id *__
         counts[static_cast<size_t>(blockIdx.x) * experts + e] = histogram[e];
 }
 
-// Rows of one chunk per CTA. counts: [gridDim.x][experts], or null where the grid is one cluster: the
-// CTAs then publish their chunk's counts in shared memory, behind `next`.
-template <typename Id>
+// Whole warp: the order of each lane's choice among the warp's choices of its expert so far, counted
+// on in `own`.
+__device__ __forceinline__ int32_t rank_in_warp(int32_t *own, uint32_t e, uint32_t experts, uint32_t lane) {
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
+    const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
+    int32_t rank = 0;
+    if (e < experts) rank = own[e] + static_cast<int32_t>(earlier);
+    __syncwarp();
+    if (e < experts && earlier == 0) own[e] += __popc(same);
+    __syncwarp();
+    return rank;
+}
+
+// Rows of one chunk per CTA. CLUSTER: the grid is one cluster, whose CTAs publish their chunk's
+// counts in shared memory behind `next`. Otherwise counts: [gridDim.x][experts].
+template <typename Id, bool CLUSTER>
 __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *__restrict__ ids, uint32_t total,
                                                                       uint32_t chunk, uint32_t experts,
                                                                       const int32_t *counts, int32_t *offsets,
                                                                       int32_t *source, int32_t *position) {
-    extern __shared__ int32_t next[];  // [kSortWarps + 1][experts]: counts, then the next row of (warp, expert)
+    extern __shared__ int32_t next[];  // [kSortWarps + 1][experts]: counts, then the first row of (warp, expert)
     __shared__ int32_t warp_sums[kSortWarps];
     __shared__ int32_t kept;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x & 31u;
-    for (uint32_t i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) next[i] = 0;
-    __syncthreads();
     const uint32_t begin = blockIdx.x * chunk;
     const uint32_t end = min(total, begin + chunk);
     const uint32_t share = chunk / kSortWarps;  // a multiple of 32
     const uint32_t warp_begin = begin + warp * share;
     const uint32_t warp_end = min(end, warp_begin + share);
     int32_t *own = next + warp * experts;
-    // kSortAhead steps of 32 ids are loaded before the first is used (both passes).
-    for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
-        uint32_t e[kSortAhead];
+    uint32_t e[kSortAhead];
+    int32_t rank[kSortAhead];
+    // kSortAhead steps of 32 ids are loaded before the first is used.
+    auto load = [&](uint32_t i0) {
 #pragma unroll
         for (int a = 0; a < kSortAhead; ++a) e[a] = expert_of(ids, i0 + 32 * a + lane, warp_end, experts);
+    };
+    if (CLUSTER) load(warp_begin);
+    for (uint32_t i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) next[i] = 0;
+    __syncthreads();
+    if (CLUSTER) {
 #pragma unroll
         for (int a = 0; a < kSortAhead; ++a)
-            if (e[a] < experts) atomicAdd(&own[e[a]], 1);
+            if (32u * a < share) rank[a] = rank_in_warp(own, e[a], experts, lane);
+    } else {
+        for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
+            load(i0);
+#pragma unroll
+            for (int a = 0; a < kSortAhead; ++a)
+                if (e[a] < experts) atomicAdd(&own[e[a]], 1);
+        }
     }
     __syncthreads();
     // Thread t takes experts 2t and 2t + 1: their counts over this chunk's warps become offsets
@@ -98,35 +125,47 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
     int32_t *published = next + kSortWarps * experts;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        const uint32_t e = 2u * threadIdx.x + s;
+        const uint32_t x = 2u * threadIdx.x + s;
         in_all[s] = before[s] = 0;
-        if (e < experts) {
-            int32_t in_chunk = 0;
+        if (x < experts) {
+            int32_t count[kSortWarps], in_chunk = 0;
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) count[w] = next[w * experts + x];
+#pragma unroll
             for (int w = 0; w < kSortWarps; ++w) {
-                const int32_t count = next[w * experts + e];
-                next[w * experts + e] = in_chunk;
-                in_chunk += count;
+                next[w * experts + x] = in_chunk;
+                in_chunk += count[w];
             }
             in_all[s] = in_chunk;
-            published[e] = in_chunk;
+            if (CLUSTER) published[x] = in_chunk;
         }
     }
-    const bool cluster = counts == nullptr && gridDim.x > 1;
-    if (cluster) sm100::cluster_sync();
+    if (gridDim.x > 1) {
+        if (CLUSTER) sm100::cluster_sync();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const uint32_t e = 2u * threadIdx.x + s;
-        if (e < experts && gridDim.x > 1) {
-            int32_t sum = 0;
-            for (uint32_t c = 0; c < gridDim.x; ++c) {
-                if (c == blockIdx.x) before[s] = sum;
-                sum += cluster ? sm100::load_cluster_s32(sm100::map_to_rank(sm100::smem_u32(published + e), c))
-                               : counts[static_cast<size_t>(c) * experts + e];
+        for (int s = 0; s < 2; ++s) {
+            const uint32_t x = 2u * threadIdx.x + s;
+            if (x < experts) {
+                int32_t sum = 0;
+                for (uint32_t c0 = 0; c0 < gridDim.x; c0 += kSortCluster) {
+                    int32_t count[kSortCluster];
+#pragma unroll
+                    for (uint32_t c = 0; c < kSortCluster; ++c) {
+                        count[c] = 0;
+                        if (c0 + c < gridDim.x)
+                            count[c] = CLUSTER ? sm100::load_cluster_s32(sm100::map_to_rank(sm100::smem_u32(published + x), c0 + c))
+                                               : counts[static_cast<size_t>(c0 + c) * experts + x];
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < kSortCluster; ++c) {
+                        if (c0 + c == blockIdx.x) before[s] = sum;
+                        sum += count[c];
+                    }
+                }
+                in_all[s] = sum;
             }
-            in_all[s] = sum;
         }
     }
-    if (cluster) sm100::cluster_sync();  // no CTA ends while another reads its counts
     const int32_t pair = in_all[0] + in_all[1];
     int32_t inclusive = pair;
 #pragma unroll
@@ -143,38 +182,40 @@ __global__ void __launch_bounds__(kSortThreads) expert_scatter_kernel(const Id *
     if (threadIdx.x == kSortThreads - 1) kept = first + pair;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        const uint32_t e = 2u * threadIdx.x + s;
-        if (e < experts) {
-            for (int w = 0; w < kSortWarps; ++w) next[w * experts + e] += first + before[s];
-            if (blockIdx.x == 0) offsets[e] = first;
+        const uint32_t x = 2u * threadIdx.x + s;
+        if (x < experts) {
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) next[w * experts + x] += first + before[s];
+            if (blockIdx.x == 0) offsets[x] = first;
         }
         first += in_all[s];
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = kept;
-    for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
-        uint32_t e[kSortAhead];
+    auto place = [&](uint32_t i, int32_t row) {
+        if (i < warp_end) {
+            position[i] = row;
+            if (row >= 0) source[row] = static_cast<int32_t>(i);
+        }
+    };
+    if (CLUSTER) {
 #pragma unroll
-        for (int a = 0; a < kSortAhead; ++a) e[a] = expert_of(ids, i0 + 32 * a + lane, warp_end, experts);
+        for (int a = 0; a < kSortAhead; ++a)
+            if (32u * a < share) place(warp_begin + 32 * a + lane, e[a] < experts ? own[e[a]] + rank[a] : -1);
+    } else {
+        for (uint32_t i0 = warp_begin; i0 < warp_end; i0 += 32 * kSortAhead) {
+            load(i0);
 #pragma unroll
-        for (int a = 0; a < kSortAhead; ++a) {
-            const uint32_t i = i0 + 32 * a + lane;
-            const uint32_t same = __match_any_sync(0xFFFFFFFFu, e[a]);
-            const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
-            int32_t row = -1;
-            if (e[a] < experts) row = own[e[a]] + static_cast<int32_t>(earlier);
-            __syncwarp();
-            if (e[a] < experts && earlier == 0) own[e[a]] += __popc(same);
-            __syncwarp();
-            if (i < warp_end) {
-                position[i] = row;
-                if (row >= 0) source[row] = static_cast<int32_t>(i);
+            for (int a = 0; a < kSortAhead; ++a) {
+                const int32_t row = rank_in_warp(own, e[a], experts, lane);
+                place(i0 + 32 * a + lane, e[a] < experts ? row : -1);
             }
         }
     }
     const uint32_t stride = gridDim.x * kSortThreads;
     for (uint32_t row = static_cast<uint32_t>(kept) + blockIdx.x * kSortThreads + threadIdx.x; row < total; row += stride)
         source[row] = -1;
+    if (CLUSTER && gridDim.x > 1) sm100::cluster_sync();  // no CTA ends while another reads its counts
 }
 
 // ---- rows -------------------------------------------------------------------------------------
@@ -435,22 +476,26 @@ uint32_t row_blocks(uint64_t items, int sm_count) {
 template <typename Id>
 cudaError_t sort_typed(const Id *ids, uint32_t total, uint32_t experts, int32_t *offsets, int32_t *source,
                        int32_t *position, int32_t *counts, cudaStream_t stream) {
+    constexpr size_t kTable = (kSortWarps + 1) * sizeof(int32_t);  // per expert
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
-        return cudaFuncSetAttribute(expert_scatter_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>((kSortWarps + 1) * kMaxExperts * sizeof(int32_t)));
+        const int bytes = static_cast<int>(kTable * kMaxExperts);
+        const cudaError_t first = cudaFuncSetAttribute(expert_scatter_kernel<Id, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        return first != cudaSuccess
+                   ? first
+                   : cudaFuncSetAttribute(expert_scatter_kernel<Id, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     });
     if (error != cudaSuccess) return error;
     const uint32_t chunk = sort_chunk(total);
     const uint32_t chunks = total == 0 ? 1u : (total + chunk - 1) / chunk;
-    const uint32_t cluster = chunks <= kSortCluster ? chunks : 1u;
-    if (chunks > cluster) {
-        const cudaError_t counted =
-            launch(expert_count_kernel<Id>, chunks, kSortThreads, 0, 1, stream, ids, total, chunk, experts, counts);
-        if (counted != cudaSuccess) return counted;
+    if (sort_in_cluster(total)) {
+        return launch(expert_scatter_kernel<Id, true>, chunks, kSortThreads, kTable * experts, chunks, stream, ids, total, chunk,
+                      experts, nullptr, offsets, source, position);
     }
-    return launch(expert_scatter_kernel<Id>, chunks, kSortThreads, (kSortWarps + 1) * experts * sizeof(int32_t), cluster, stream,
-                  ids, total, chunk, experts, chunks > cluster ? counts : nullptr, offsets, source, position);
+    const cudaError_t counted = launch(expert_count_kernel<Id>, chunks, kSortThreads, 0, 1, stream, ids, total, chunk, experts, counts);
+    if (counted != cudaSuccess) return counted;
+    return launch(expert_scatter_kernel<Id, false>, chunks, kSortThreads, kTable * experts, 1, stream, ids, total, chunk, experts,
+                  counts, offsets, source, position);
 }
 
 template <typename T, bool ALIGNED>
@@ -505,9 +550,9 @@ size_t item_bytes(int type) { return type == QPUCUDA_DTYPE_F32 ? 4 : 2; }
 size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts) {
     const uint64_t total = static_cast<uint64_t>(tokens) * choices;
     if (total == 0 || total > 0x7FFFFFFFull) return 0;
+    if (sort_in_cluster(static_cast<uint32_t>(total))) return 0;
     const uint32_t chunk = sort_chunk(static_cast<uint32_t>(total));
-    const uint32_t chunks = static_cast<uint32_t>((total + chunk - 1) / chunk);
-    return chunks > kSortCluster ? static_cast<size_t>(chunks) * experts * sizeof(int32_t) : 0;
+    return static_cast<size_t>((total + chunk - 1) / chunk) * experts * sizeof(int32_t);
 }
 
 cudaError_t launch_expert_sort(const void *ids, bool ids_64, uint32_t tokens, uint32_t choices, uint32_t experts,

@@ -114,7 +114,7 @@ __device__ __forceinline__ void load_steps(const T *x, uint32_t remaining, uint3
 // STEPS steps of one or two neighbouring groups of one row, at fixed distances from one address, and
 // loads them all before it uses the first. Each input is read once, each output written once; what
 // it has to keep below HBM's time is its instructions.
-constexpr int kRowsThreads = 256;
+constexpr int kRowsThreads = 128;
 
 template <typename T, bool GATED, bool VECTOR, int STEPS>
 __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const RowsParams params, uint32_t chunks) {
