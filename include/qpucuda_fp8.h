@@ -88,8 +88,8 @@ typedef struct qpucuda_fp8_gemm_desc {
     void *out;               /* [rows][n] */
     int out_type;            /* qpucuda_dtype */
     size_t out_stride;       /* elements */
-    /* Nonzero: no kernel that is still unfinished when the one launched just before this call
-     * starts writes w, w_scales or offsets, nor does that one, so they may be read early. */
+    /* Nonzero: w, w_scales and offsets were complete before the kernel queued just before this one
+     * started, so they may be read while that kernel is still running. */
     int weights_settled;
 } qpucuda_fp8_gemm_desc;
 
@@ -97,9 +97,10 @@ typedef struct qpucuda_fp8_gemm_desc {
 
 qpucuda_status qpucuda_fp8_gemm(qpucuda_context *context, const qpucuda_fp8_gemm_desc *desc);
 
-/* Both in one call: the rows into quantize->q and ->scales, then the product that reads them (its a,
- * a_stride, a_scales, rows and k must be those; weights_settled may then be set unless the call just
- * before this one still writes the weight when the rows are quantized). */
+/* The product of rows that are quantized in the same call: gemm->a, a_stride, a_scales, rows and k
+ * must be quantize's, whose q and scales serve as scratch and hold nothing certain afterwards (a few
+ * rows of a small matrix never leave the kernel). With weights_settled the weight must also not be
+ * written by the work queued just before this call; offsets may be. */
 qpucuda_status qpucuda_fp8_linear(qpucuda_context *context, const qpucuda_fp8_quantize_desc *quantize,
                                   const qpucuda_fp8_gemm_desc *gemm);
 

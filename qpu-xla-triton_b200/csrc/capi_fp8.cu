@@ -124,10 +124,8 @@ qpucuda_status qpucuda_fp8_linear(qpucuda_context *context, const qpucuda_fp8_qu
     qpucuda_status checked = check_quantize(context, quantize);
     if (checked == QPUCUDA_OK) checked = check_gemm(context, gemm);
     if (checked != QPUCUDA_OK) return checked;
-    return submit(context, "fp8_linear", [&] {
-        const cudaError_t error = launch_fp8_quantize_rows(*quantize, context->sm_count, context->stream);
-        return error != cudaSuccess ? error : launch_fp8_gemm(*gemm, context->d_error, context->sm_count, context->stream);
-    });
+    return submit(context, "fp8_linear",
+                  [&] { return launch_fp8_linear(*quantize, *gemm, context->d_error, context->sm_count, context->stream); });
 }
 
 size_t qpucuda_expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts) {

@@ -13,8 +13,9 @@
 // tensor memory column = row.
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
-#include "element.cuh"
+#include "fp8_quantize.cuh"
 #include "qpucuda_fp8_internal.h"
 #include "qpucuda_internal.h"
 #include "sm100_fp8.cuh"
@@ -43,6 +44,15 @@ struct GemmParams {
     uint32_t weights_settled;
     uint32_t tma_store;  // the output's rows can be written by the copy engine
     unsigned int *error_word;
+};
+
+// Rows that the product quantizes itself.
+struct FusedRows {
+    const void *x;
+    size_t stride;
+    int type;
+    uint32_t gated;
+    uint32_t vector;  // rows and, gated, their second halves allow 16-byte loads
 };
 
 // The rows of one tile: [row0, row_end) of matrix `expert`, at most the tile's height of them.
@@ -99,23 +109,80 @@ __device__ __forceinline__ uint32_t owned_rows(const GemmParams &params) {
 
 // ---- the narrow kernel ------------------------------------------------------------------------
 
-template <int NT>
+// A few rows of a small matrix are quantized by the product itself: every CTA those of its K blocks,
+// at most kFusedBlocks, into shared memory, while its first weights arrive. One launch instead of two
+// (1 x 2048 x 2048 bf16: 14.4 -> 12.4 us a call, 5.3 -> 4.4 in a captured graph), as long as its four
+// warps are done in three steps each (4 x 2048 x 5632, three steps: 7.5 -> 6.9 us in a graph; 16 x 2048
+// x 2048, four: 6.0 -> 6.4).
+constexpr uint32_t kFusedBlocks = 8;
+constexpr uint32_t kFusedSteps = 3;
+
+template <int NT, bool FUSED>
 struct Narrow {
     static constexpr int kWarps = 4;  // epilogue: one per lane quarter
     static constexpr int kThreads = 64 + 32 * kWarps;
     static constexpr int kCtasPerSm = 2;
     static constexpr int kWBytes = kBlockN * kBlockK;
     static constexpr int kXBytes = NT * kBlockK;
-    static constexpr int kStageBytes = kWBytes + kXBytes;
+    static constexpr int kStageBytes = kWBytes + (FUSED ? 0 : kXBytes);
+    static constexpr int kFusedBytes = FUSED ? static_cast<int>(kFusedBlocks) * (kXBytes + NT * 4) : 0;  // values, then scales
     static constexpr int kStages = 5;
     static constexpr int kBuffers = 4;  // tensor memory accumulators
     static constexpr int kTmemColumns = kBuffers * NT;      // a power of two
     static constexpr int kScaleFloats = 2 * NT;             // per warp: this block's and the next's
-    static constexpr size_t kSharedBytes = static_cast<size_t>(kStages) * kStageBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
+    static constexpr size_t kSharedBytes =
+        static_cast<size_t>(kStages) * kStageBytes + kFusedBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
     static_assert(kTmemColumns * kCtasPerSm <= 512, "tensor memory");
     static_assert(kSharedBytes * kCtasPerSm + 2048 <= 227 * 1024, "shared memory");
     static_assert(static_cast<size_t>(NT) * kBlockN * 4 <= static_cast<size_t>(kStages) * kStageBytes, "split sums");
 };
+
+// Groups of this CTA's rows and K blocks, `items` of them, quantized by four warps: group i is row
+// i / blocks, block i % blocks. Values go to `values` in the MMA's layout ([block][row] of 128 bytes,
+// 128-byte swizzle), scales to scales[block * NT + row].
+template <typename T, bool GATED, int NT>
+__device__ __forceinline__ void fuse_rows(const FusedRows &rows, const GemmParams &params, uint32_t row0, uint32_t items,
+                                          uint32_t kb_begin, uint32_t blocks, uint8_t *values, float *scales, uint32_t worker,
+                                          uint32_t lane) {
+    constexpr int kLanes = 128 / kVector<T>;
+    constexpr uint32_t kPerStep = 32 / kLanes;
+    const uint32_t inner = lane % kLanes * kVector<T>;
+    for (uint32_t first = worker * kPerStep; first < items; first += 4 * kPerStep) {
+        const uint32_t item = first + lane / kLanes;
+        const bool present = item < items;
+        const uint32_t row = present ? item / blocks : 0u, block = present ? item % blocks : 0u;
+        const uint32_t column = (kb_begin + block) * kBlockK + inner;
+        const T *x = static_cast<const T *>(rows.x) + static_cast<size_t>(row0 + row) * rows.stride + column;
+        const uint32_t remaining = present && column < params.k ? params.k - column : 0u;
+        Vector<T> raw[1], raw_up[1];
+        if (rows.vector != 0) {
+            load_steps<T, true>(x, remaining, 128u, raw);
+            if (GATED) load_steps<T, true>(x + params.k, remaining, 128u, raw_up);
+        } else {
+            load_steps<T, false>(x, remaining, 128u, raw);
+            if (GATED) load_steps<T, false>(x + params.k, remaining, 128u, raw_up);
+        }
+        float v[kVector<T>], amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kVector<T>; ++i) {
+            v[i] = to_float(raw[0].items[i]);
+            if (GATED) v[i] = silu_times(v[i], to_float(raw_up[0].items[i]));
+            amax = max_nan(amax, fabsf(v[i]));
+        }
+        const float scale = group_scale(group_max<kLanes>(amax));
+        uint32_t packed[kVector<T> / 4];
+        quantize_values(v, scale, packed);
+        if (present) {
+            uint8_t *q = values + (block * NT + row) * 128u + (((inner >> 4) ^ (row & 7u)) << 4) + (inner & 15u);
+            if constexpr (kVector<T> == 8) {
+                *reinterpret_cast<uint2 *>(q) = make_uint2(packed[0], packed[kVector<T> / 4 - 1]);
+            } else {
+                *reinterpret_cast<uint32_t *>(q) = packed[0];
+            }
+            if (lane % kLanes == 0) scales[block * NT + row] = scale;
+        }
+    }
+}
 
 template <int STAGES, int BUFFERS>
 struct Control {
@@ -124,6 +191,7 @@ struct Control {
     uint64_t tmem_full[BUFFERS];
     uint64_t tmem_empty[BUFFERS];
     uint64_t drain;
+    uint64_t rows_ready;  // the product's own quantized rows are in place
     uint32_t tmem_base;
     volatile int abort_flag;
 };
@@ -134,17 +202,18 @@ struct Control {
 //   warp 0   copies: a weight and a row box per stage
 //   warp 1   tensor memory and MMA: 4 MMAs per stage into the next of kBuffers accumulators
 //   others   each block's accumulator into registers, scaled; then the sums over the cluster, the store
-template <int NT, typename Out>
-__global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
+template <int NT, bool FUSED, typename Out>
+__global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>::kCtasPerSm)
     fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                           const GemmParams params) {
-    using Shape = Narrow<NT>;
+                           const GemmParams params, const FusedRows fused) {
+    using Shape = Narrow<NT, FUSED>;
     using Ctl = Control<Shape::kStages, Shape::kBuffers>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *stage_w = smem;
-    uint8_t *stage_x = smem + Shape::kStages * Shape::kWBytes;
-    float *scale_rows = reinterpret_cast<float *>(smem + Shape::kStages * Shape::kStageBytes);
+    uint8_t *stage_x = smem + Shape::kStages * Shape::kWBytes;  // FUSED: one tile per K block of this CTA
+    float *fused_scales = reinterpret_cast<float *>(stage_x + kFusedBlocks * Shape::kXBytes);
+    float *scale_rows = reinterpret_cast<float *>(smem + Shape::kStages * Shape::kStageBytes + Shape::kFusedBytes);
     Ctl *control = reinterpret_cast<Ctl *>(scale_rows + Shape::kWarps * Shape::kScaleFloats);
     static_assert(sizeof(Ctl) <= 256, "control block");
 
@@ -165,6 +234,7 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
             mbar_init(smem_u32(&control->tmem_empty[b]), Shape::kWarps);
         }
         mbar_init(smem_u32(&control->drain), 1);
+        mbar_init(smem_u32(&control->rows_ready), 1);
         control->abort_flag = 0;
         mbar_init_fence();
     }
@@ -193,7 +263,7 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
     } else if (warp == 0) {
         if (lane == 0) {
             prefetch_tensor_map(&map_w);
-            prefetch_tensor_map(&map_a);
+            if (!FUSED) prefetch_tensor_map(&map_a);
             const int w_row = static_cast<int>(tile.expert * params.n + n0);
             auto load_w = [&](uint32_t kb, uint32_t stage) {
                 const uint32_t full = smem_u32(&control->full[stage]);
@@ -201,6 +271,7 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
                 tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes), &map_w, full, static_cast<int>(kb * kBlockK), w_row);
             };
             auto load_x = [&](uint32_t kb, uint32_t stage) {
+                if (FUSED) return;
                 tma_load_2d(smem_u32(stage_x + stage * Shape::kXBytes), &map_a, smem_u32(&control->full[stage]),
                             static_cast<int>(kb * kBlockK), row0);
             };
@@ -241,13 +312,14 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
             constexpr uint32_t instr = fp8_instr_desc(kBlockN, NT);
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 1;
             bool ok = true, any = false;
-            for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
+            if (FUSED) ok = wait_bounded(smem_u32(&control->rows_ready), 0, &control->abort_flag, params.error_word);
+            for (uint32_t kb = kb_begin; ok && kb < kb_end; ++kb) {
                 ok = wait_bounded(smem_u32(&control->tmem_empty[buffer]), buffer_phase, &control->abort_flag, params.error_word) &&
                      wait_bounded(smem_u32(&control->full[stage]), phase, &control->abort_flag, params.error_word);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t w = smem_desc_sw128(smem_u32(stage_w + stage * Shape::kWBytes));
-                const uint64_t x = smem_desc_sw128(smem_u32(stage_x + stage * Shape::kXBytes));
+                const uint64_t x = smem_desc_sw128(smem_u32(stage_x + (FUSED ? kb - kb_begin : stage) * Shape::kXBytes));
 #pragma unroll
                 for (int kk = 0; kk < kBlockK / kMmaK; ++kk)
                     mma_fp8(tmem_base + buffer * NT, w + static_cast<uint64_t>(kk * (kMmaK >> 4)),
@@ -278,16 +350,43 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
         const uint32_t quarter = warp & 3u;  // tensor memory lanes this warp may read
         float *scales = scale_rows + worker * Shape::kScaleFloats;
         const float *w_scales = params.w_scales + (static_cast<size_t>(tile.expert) * params.n_blocks + n_block) * params.k_blocks;
-        const float *a_scales = params.a_scales + static_cast<size_t>(tile.row0) * params.a_scale_row_stride;
+        if constexpr (FUSED) {
+            const uint32_t blocks = kb_end - kb_begin;
+            const uint32_t items = (tile.row_end - tile.row0) * blocks;
+            auto quantize = [&](auto element, auto gated) {
+                fuse_rows<decltype(element), decltype(gated)::value, NT>(fused, params, tile.row0, items, kb_begin, blocks, stage_x,
+                                                                         fused_scales, worker, lane);
+            };
+            auto choose = [&](auto element) {
+                if (fused.gated != 0) {
+                    quantize(element, std::true_type{});
+                } else {
+                    quantize(element, std::false_type{});
+                }
+            };
+            if (fused.type == QPUCUDA_DTYPE_F32) {
+                choose(float{});
+            } else if (fused.type == QPUCUDA_DTYPE_BF16) {
+                choose(__nv_bfloat16{});
+            } else {
+                choose(__half{});
+            }
+            fence_proxy_async_shared();  // the MMA reads what was just written
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (worker == 0 && lane == 0) mbar_arrive(smem_u32(&control->rows_ready));
+        }
+        const float *a_scales = FUSED ? fused_scales : params.a_scales + static_cast<size_t>(tile.row0) * params.a_scale_row_stride;
         // Lane j stages row j's scale; rows past the tile hold zeros or another expert's values and
         // are not stored. Fetched two blocks ahead.
-        const bool staging = lane < kColumns && tile.row0 + lane < params.rows;
+        const bool staging = lane < kColumns && tile.row0 + lane < (FUSED ? tile.row_end : params.rows);
+        const size_t scale_row = FUSED ? 1 : params.a_scale_row_stride, scale_block = FUSED ? NT : params.a_scale_group_stride;
+        const uint32_t scale_first = FUSED ? kb_begin : 0u;
         auto fetch = [&](uint32_t kb, float &row_scale, float &w_scale) {
             const bool inside = kb < kb_end;
             w_scale = inside ? __ldg(w_scales + kb) : 0.0f;
-            row_scale = inside && staging ? a_scales[static_cast<size_t>(lane) * params.a_scale_row_stride +
-                                                     static_cast<size_t>(kb) * params.a_scale_group_stride]
-                                          : 0.0f;
+            row_scale = inside && staging
+                            ? a_scales[static_cast<size_t>(lane) * scale_row + static_cast<size_t>(kb - scale_first) * scale_block]
+                            : 0.0f;
         };
         float row_now, row_next, w_now, w_next;
         fetch(kb_begin, row_now, w_now);
@@ -386,13 +485,20 @@ __global__ void __launch_bounds__(Narrow<NT>::kThreads, Narrow<NT>::kCtasPerSm)
     }
 }
 
-template <int NT, typename Out>
-cudaError_t launch_narrow(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, uint32_t tiles,
-                          uint32_t split, cudaStream_t stream) {
-    using Shape = Narrow<NT>;
+// A narrow product's tiles: their height, their number at most (whatever the offsets) and the CTAs
+// that share the K blocks of one.
+struct NarrowLaunch {
+    int height;
+    uint32_t tiles, split;
+};
+
+template <int NT, bool FUSED, typename Out>
+cudaError_t launch_narrow(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params, const NarrowLaunch &launch,
+                          const FusedRows &fused, cudaStream_t stream) {
+    using Shape = Narrow<NT, FUSED>;
     static PerDeviceOnce configured;
     const cudaError_t error = configured.run([] {
-        return cudaFuncSetAttribute(fp8_gemm_narrow_kernel<NT, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(fp8_gemm_narrow_kernel<NT, FUSED, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(Shape::kSharedBytes));
     });
     if (error != cudaSuccess) return error;
@@ -400,24 +506,26 @@ cudaError_t launch_narrow(const CUtensorMap &map_w, const CUtensorMap &map_a, co
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
     attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = split;
+    attributes[1].val.clusterDim.x = launch.split;
     attributes[1].val.clusterDim.y = 1;
     attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.n_blocks * split, tiles, 1);
+    config.gridDim = dim3(params.n_blocks * launch.split, launch.tiles, 1);
     config.blockDim = dim3(Shape::kThreads);
     config.dynamicSmemBytes = Shape::kSharedBytes;
     config.stream = stream;
     config.attrs = attributes;
     config.numAttrs = 2;
-    return cudaLaunchKernelEx(&config, fp8_gemm_narrow_kernel<NT, Out>, map_w, map_a, params);
+    return cudaLaunchKernelEx(&config, fp8_gemm_narrow_kernel<NT, FUSED, Out>, map_w, map_a, params, fused);
 }
 
 template <typename Out>
-cudaError_t launch_narrow_rows(int nt, const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
-                               uint32_t tiles, uint32_t split, cudaStream_t stream) {
-    return nt == 16 ? launch_narrow<16, Out>(map_w, map_a, params, tiles, split, stream)
-                    : launch_narrow<32, Out>(map_w, map_a, params, tiles, split, stream);
+cudaError_t launch_narrow_rows(const CUtensorMap &map_w, const CUtensorMap &map_a, const GemmParams &params,
+                               const NarrowLaunch &launch, const FusedRows *fused, cudaStream_t stream) {
+    if (fused != nullptr) return launch_narrow<16, true, Out>(map_w, map_a, params, launch, *fused, stream);
+    const FusedRows none{};
+    return launch.height == 16 ? launch_narrow<16, false, Out>(map_w, map_a, params, launch, none, stream)
+                               : launch_narrow<32, false, Out>(map_w, map_a, params, launch, none, stream);
 }
 
 // ---- the wide kernel --------------------------------------------------------------------------
@@ -1073,10 +1181,7 @@ bool use_wide(uint64_t share, uint64_t matrices, uint64_t n_tiles, uint64_t sms)
     return share > 32 && n_tiles >= 16;
 }
 
-}  // namespace
-
-cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word, int sm_count,
-                            cudaStream_t stream) {
+GemmParams gemm_params(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word) {
     GemmParams params{};
     params.rows = desc.rows;
     params.n = desc.n;
@@ -1094,32 +1199,58 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
     params.out_stride = desc.out_stride;
     params.weights_settled = desc.weights_settled != 0 ? 1u : 0u;
     params.error_word = error_word;
+    return params;
+}
+
+// Tiles of `height` rows, at most, whatever the offsets: one partly filled tile per matrix.
+uint64_t most_tiles(const qpucuda_fp8_gemm_desc &desc, uint64_t filled, uint64_t height) {
+    return (desc.rows + filled * (height - 1)) / height;
+}
+
+NarrowLaunch plan_narrow(const qpucuda_fp8_gemm_desc &desc, const GemmParams &params, uint64_t share, uint64_t filled, uint64_t sms) {
+    NarrowLaunch launch{};
+    // 16 rows, or 32 where a matrix has more (uneven experts: more than 4 on average)
+    launch.height = share <= (desc.experts != 0 ? 4u : 16u) ? 16 : 32;
+    const uint64_t tiles = most_tiles(desc, filled, static_cast<uint64_t>(launch.height));
+    launch.tiles = static_cast<uint32_t>(tiles);
+    // K is split over a cluster while the tiles leave SMs idle, two CTAs each.
+    launch.split = 1;
+    while (launch.split < kMaxSplit && tiles * params.n_blocks * launch.split * 2 <= sms * 2 && launch.split * 2 <= params.k_blocks)
+        launch.split *= 2;
+    return launch;
+}
+
+cudaError_t launch_gemm(const qpucuda_fp8_gemm_desc &desc, const qpucuda_fp8_quantize_desc *quantize, unsigned int *error_word,
+                        int sm_count, cudaStream_t stream) {
+    const GemmParams params = gemm_params(desc, error_word);
     const uint64_t matrices = desc.experts != 0 ? desc.experts : 1u;
     const uint64_t filled = matrices < desc.rows ? matrices : desc.rows;  // matrices that can have rows
     const uint64_t share = (desc.rows + matrices - 1) / matrices;
     const uint64_t sms = static_cast<uint64_t>(sm_count);
-    // Tiles of `height` rows, at most, whatever the offsets: one partly filled tile per matrix.
-    const auto most_tiles = [&](uint64_t height) { return (desc.rows + filled * (height - 1)) / height; };
+    CUtensorMap map_w, map_a;
     WideLaunch wide{};
     wide.n_tiles = (desc.n + kWideN - 1) / kWideN;
     if (use_wide(share, filled, wide.n_tiles, sms)) {
-        // Pairs where tiles of 256 rows hold hardly more padding than tiles of 128.
-        wide.pair = sms >= 2 && (desc.experts != 0 ? share >= kPairShare : most_tiles(2 * kWideM) * 2 * 12 <= most_tiles(kWideM) * 13);
-        const uint64_t height = wide.pair ? 2 * kWideM : kWideM;
-        wide.tiles = most_tiles(height) * wide.n_tiles;
-        if (wide.tiles > 0x3FFFFFFFull) return cudaErrorInvalidValue;
-        wide.split = 1;
-        if (wide.tiles * 2 <= sms) {
-            wide.pair = false;
-            wide.tiles = most_tiles(kWideM) * wide.n_tiles;
-            while (wide.split < 4 && wide.tiles * wide.split * 2 <= sms && wide.split * 8 <= params.k_blocks) wide.split *= 2;
+        if (quantize != nullptr) {
+            const cudaError_t error = launch_fp8_quantize_rows(*quantize, sm_count, stream);
+            if (error != cudaSuccess) return error;
         }
-        CUtensorMap map_w, map_a;
+        // Pairs where tiles of 256 rows hold hardly more padding than tiles of 128.
+        const uint64_t single_tiles = most_tiles(desc, filled, kWideM), pair_tiles = most_tiles(desc, filled, 2 * kWideM);
+        wide.pair = sms >= 2 && (desc.experts != 0 ? share >= kPairShare : pair_tiles * 2 * 12 <= single_tiles * 13);
+        wide.split = 1;
+        if ((wide.pair ? pair_tiles : single_tiles) * wide.n_tiles * 2 <= sms) {
+            wide.pair = false;
+            while (wide.split < 4 && single_tiles * wide.n_tiles * wide.split * 2 <= sms && wide.split * 8 <= params.k_blocks)
+                wide.split *= 2;
+        }
+        wide.tiles = (wide.pair ? pair_tiles : single_tiles) * wide.n_tiles;
+        if (wide.tiles > 0x3FFFFFFFull) return cudaErrorInvalidValue;
         if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
             !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, kWideM)) {
             return cudaErrorInvalidValue;
         }
-        const uint64_t group = kGroupBytes / (height * desc.k);
+        const uint64_t group = kGroupBytes / (static_cast<uint64_t>(wide.pair ? 2 * kWideM : kWideM) * desc.k);
         wide.group_rows = static_cast<uint32_t>(group < kGroupRows ? kGroupRows : (group < 0x10000u ? group : 0x10000u));
         switch (desc.out_type) {
             case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(map_w, map_a, params, wide, sm_count, stream);
@@ -1128,27 +1259,49 @@ cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *err
         }
         return cudaErrorInvalidValue;
     }
-    // The tile's height: 16 rows, or 32 where a matrix has more (uneven experts: more than 4 on average).
-    const int nt = share <= (desc.experts != 0 ? 4u : 16u) ? 16 : 32;
-    CUtensorMap map_w, map_a;
-    if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
-        !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, static_cast<uint32_t>(nt))) {
+    const NarrowLaunch narrow = plan_narrow(desc, params, share, filled, sms);
+    FusedRows fused{};
+    bool fuse = false;
+    if (quantize != nullptr) {
+        const uint64_t blocks = (params.k_blocks + narrow.split - 1) / narrow.split;
+        fuse = desc.experts == 0 && quantize->row_source == nullptr && narrow.tiles == 1 && narrow.height == 16 &&
+               blocks <= kFusedBlocks &&
+               blocks * desc.rows <= kFusedSteps * 4u * (quantize->x_type == QPUCUDA_DTYPE_F32 ? 1u : 2u);  // groups of a step
+        if (fuse) {
+            fused.x = quantize->x;
+            fused.stride = quantize->x_stride;
+            fused.type = quantize->x_type;
+            fused.gated = quantize->gated != 0 ? 1u : 0u;
+            fused.vector = fp8_vector_rows(*quantize) ? 1u : 0u;
+        } else {
+            const cudaError_t error = launch_fp8_quantize_rows(*quantize, sm_count, stream);
+            if (error != cudaSuccess) return error;
+        }
+    }
+    if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN)) return cudaErrorInvalidValue;
+    if (fuse) {
+        map_a = map_w;  // not used
+    } else if (!encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, static_cast<uint32_t>(narrow.height))) {
         return cudaErrorInvalidValue;
     }
-    const uint64_t tiles = most_tiles(static_cast<uint64_t>(nt));
-    // K is split over a cluster while the tiles leave SMs idle, two CTAs each.
-    uint32_t split = 1;
-    while (split < kMaxSplit && tiles * params.n_blocks * split * 2 <= static_cast<uint64_t>(sm_count) * 2 &&
-           split * 2 <= params.k_blocks) {
-        split *= 2;
-    }
-    const uint32_t grid_tiles = static_cast<uint32_t>(tiles);
+    const FusedRows *rows = fuse ? &fused : nullptr;
     switch (desc.out_type) {
-        case QPUCUDA_DTYPE_F32: return launch_narrow_rows<float>(nt, map_w, map_a, params, grid_tiles, split, stream);
-        case QPUCUDA_DTYPE_BF16: return launch_narrow_rows<__nv_bfloat16>(nt, map_w, map_a, params, grid_tiles, split, stream);
-        case QPUCUDA_DTYPE_F16: return launch_narrow_rows<__half>(nt, map_w, map_a, params, grid_tiles, split, stream);
+        case QPUCUDA_DTYPE_F32: return launch_narrow_rows<float>(map_w, map_a, params, narrow, rows, stream);
+        case QPUCUDA_DTYPE_BF16: return launch_narrow_rows<__nv_bfloat16>(map_w, map_a, params, narrow, rows, stream);
+        case QPUCUDA_DTYPE_F16: return launch_narrow_rows<__half>(map_w, map_a, params, narrow, rows, stream);
     }
     return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_gemm(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word, int sm_count, cudaStream_t stream) {
+    return launch_gemm(desc, nullptr, error_word, sm_count, stream);
+}
+
+cudaError_t launch_fp8_linear(const qpucuda_fp8_quantize_desc &quantize, const qpucuda_fp8_gemm_desc &gemm, unsigned int *error_word,
+                              int sm_count, cudaStream_t stream) {
+    return launch_gemm(gemm, &quantize, error_word, sm_count, stream);
 }
 
 }  // namespace qpucuda

@@ -7,65 +7,12 @@
 // scale, at least 2^-120) a normal number; a group below 448 * 2^-60 only loses relative precision.
 // The maximum propagates NaN: a group with a NaN or an infinity has such a scale and dequantizes to
 // NaN throughout.
-#include <cuda_fp8.h>
-
-#include "element.cuh"
+#include "fp8_quantize.cuh"
 #include "qpucuda_fp8_internal.h"
 #include "qpucuda_internal.h"
-#include "sm100_fp8.cuh"
 
 namespace qpucuda {
 namespace {
-
-constexpr float kE4m3Max = 448.0f;
-constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
-// max(RN(amax / 448), 2^-60), the quotient by Markstein's correction of a product with the rounded
-// reciprocal: q0 = RN(a y) with y = RN(1 / 448) is within one step of a / 448, the remainder a - 448 q0
-// is exact in an fma, and RN(q0 + remainder * y) is then the rounded quotient (amax above 2^-100;
-// anything smaller ends at the floor). An infinite amax gives NaN, which serves as well.
-__device__ __forceinline__ float group_scale(float amax) {
-    constexpr float kReciprocal = 1.0f / 448.0f;
-    const float q0 = __fmul_rn(amax, kReciprocal);
-    const float remainder = __fmaf_rn(-q0, kE4m3Max, amax);
-    return max_nan(__fmaf_rn(remainder, kReciprocal, q0), kScaleFloor);
-}
-
-// e4m3(RN(x / s)) of N values, two to an instruction. A hardware division per value, or a branch to
-// one near the borders of e4m3 (bf16 values over a bf16 maximum lie on borders in 1 of 500 cases, so
-// half of the warps took it), costs more than the copy itself. Markstein's correction instead, twice:
-// with y = RN(1 / s), q1 = RN(q0 + (x - q0 s) y) is within one step of x / s, its remainder is exact in
-// an fma, and RN(q1 + (x - q1 s) y) is the rounded quotient (Markstein 1990). That needs remainders
-// above the smallest normal number: true for every quotient above 2^-10, the smallest border of e4m3,
-// as s is at least 2^-60; smaller quotients end as zero whatever their last bits.
-template <int N>
-__device__ __forceinline__ void quantize_values(const float (&v)[N], float scale, uint32_t (&packed)[N / 4]) {
-    using sm100::fma2;
-    using sm100::pack2;
-    const float inverse = __frcp_rn(scale);
-    const uint64_t y = pack2(inverse, inverse), minus_s = pack2(-scale, -scale), zero = pack2(-0.0f, -0.0f);
-    uint16_t pairs[N / 2];
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        const uint64_t x = pack2(v[i], v[i + 1]);
-        uint64_t q = fma2(x, y, zero);
-        q = fma2(fma2(q, minus_s, x), y, q);
-        q = fma2(fma2(q, minus_s, x), y, q);
-        pairs[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(sm100::low(q), sm100::high(q)), __NV_SATFINITE, __NV_E4M3);
-    }
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) packed[i] = pairs[2 * i] | (static_cast<uint32_t>(pairs[2 * i + 1]) << 16);
-}
-
-// silu(g) * u in fp32. exp(-g) overflows to infinity below g = -88.7, where the quotient is then -0
-// as it should be to fp32's range.
-__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 struct RowsParams {
     const void *x;
@@ -78,36 +25,6 @@ struct RowsParams {
     float *scales;
     size_t scale_row_stride, scale_group_stride;
 };
-
-// kVector elements at x, zero from `remaining` of them on. Full vectors first and the ragged end of a
-// row in a pass of its own, so that nothing stands between the loads of several steps.
-template <typename T, bool VECTOR, int STEPS>
-__device__ __forceinline__ void load_steps(const T *x, uint32_t remaining, uint32_t step, Vector<T> (&raw)[STEPS]) {
-    constexpr uint32_t kItems = kVector<T>;
-#pragma unroll
-    for (int u = 0; u < STEPS; ++u) {
-        const uint32_t left = remaining > u * step ? remaining - u * step : 0u;
-        raw[u].bits = make_uint4(0, 0, 0, 0);
-        if (VECTOR) {
-            if (left >= kItems) raw[u].bits = load_stream16(x + u * step);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kItems; ++i)
-                if (i < left) raw[u].items[i] = x[u * step + i];
-        }
-    }
-    if (VECTOR && remaining % step != 0 && remaining % step < kItems) {
-#pragma unroll
-        for (int u = 0; u < STEPS; ++u) {
-            const uint32_t left = remaining > u * step ? remaining - u * step : 0u;
-            if (left < kItems) {
-#pragma unroll
-                for (uint32_t i = 0; i < kItems; ++i)
-                    if (i < left) raw[u].items[i] = x[u * step + i];
-            }
-        }
-    }
-}
 
 // One group is 128 columns of a row: kVector elements on each of 32 (fp32) or 16 (16-bit) lanes, so
 // every lane moves 16 bytes and the maximum is a shuffle reduction inside those lanes. A warp takes
@@ -162,10 +79,7 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
                 if constexpr (GATED) v[i] = silu_times(v[i], to_float(raw_up[u].items[i]));
                 amax = max_nan(amax, fabsf(v[i]));
             }
-#pragma unroll
-            for (int offset = kLanes / 2; offset > 0; offset >>= 1)
-                amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, offset));
-            const float scale = group_scale(amax);
+            const float scale = group_scale(group_max<kLanes>(amax));
             uint32_t packed[kVector<T> / 4];
             quantize_values(v, scale, packed);
             if (column0 + u * (kPerStep * 128u) < params.cols) {
@@ -259,14 +173,17 @@ cudaError_t launch_rows_type(const qpucuda_fp8_quantize_desc &desc, int sm_count
     params.scales = desc.scales;
     params.scale_row_stride = desc.scale_row_stride;
     params.scale_group_stride = desc.scale_group_stride;
-    // 16-byte loads need aligned rows and, gated, an aligned second half.
-    const bool vector = (reinterpret_cast<uintptr_t>(desc.x) & 15u) == 0 && desc.x_stride % kVector<T> == 0 &&
-                        (desc.gated == 0 || desc.cols % kVector<T> == 0);
+    const bool vector = fp8_vector_rows(desc);
     return desc.gated != 0 ? launch_rows_steps<T, true>(params, vector, sm_count, stream)
                            : launch_rows_steps<T, false>(params, vector, sm_count, stream);
 }
 
 }  // namespace
+
+bool fp8_vector_rows(const qpucuda_fp8_quantize_desc &desc) {
+    const size_t items = desc.x_type == QPUCUDA_DTYPE_F32 ? 4 : 8;  // of 16 bytes
+    return (reinterpret_cast<uintptr_t>(desc.x) & 15u) == 0 && desc.x_stride % items == 0 && (desc.gated == 0 || desc.cols % items == 0);
+}
 
 cudaError_t launch_fp8_quantize_rows(const qpucuda_fp8_quantize_desc &desc, int sm_count, cudaStream_t stream) {
     switch (desc.x_type) {

@@ -220,6 +220,19 @@ def test_gated_linear_is_the_product_of_the_gated_rows(cuda_device, rows) -> Non
         check_product(plan.forward(x), exact, magnitude, k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows, n, k", [(1, 1, 1), (1, 500, 900), (3, 130, 77), (4, 2048, 1000), (12, 300, 128), (16, 100, 100), (1, 2000, 2047), (5, 130, 1024), (1, 200, 9000)])
+def test_rows_quantized_inside_the_product(cuda_device, dtype, gated, rows, n, k) -> None:
+    """A few rows of a small matrix take one launch: bit for bit what the two steps give."""
+    weight = blocks(cuda_device, n, k)
+    wide = draw((rows + 1, 2 * k + 3), dtype, seed=k)
+    for source in (wide[1:, : 2 * k if gated else k], wide[1:, 3 : 3 + (2 * k if gated else k)].contiguous()):
+        with PreparedFP8Linear(cuda_device, weight, gated=gated) as plan:
+            expected = plan.forward_quantized(quantize_rows_fp8(cuda_device, source, gated=gated), dtype=dtype)
+            assert torch.equal(plan.forward(source), expected)
+
+
 @pytest.mark.parametrize("rows", [1, 30, 200])
 def test_quantized_rows_give_the_same_product(cuda_device, rows) -> None:
     weight = blocks(cuda_device, 500, 900)
