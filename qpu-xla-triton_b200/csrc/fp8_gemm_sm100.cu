@@ -558,7 +558,8 @@ struct Wide {
 };
 constexpr int kWideBoxBytes = 4096;    // 32 rows x 128 bytes of the output
 constexpr int kWideStoreBytes = 2 * kWideBoxBytes;  // per epilogue warp, on their way out
-constexpr size_t kWideTableBytes = (QPUCUDA_MAX_EXPERTS + 1) * sizeof(uint32_t);
+// The experts' tables: their first tiles and first rows, with one entry past the end each.
+constexpr size_t kWideTableBytes = 2 * (QPUCUDA_MAX_EXPERTS + 1) * sizeof(uint32_t);
 template <bool PAIR>
 constexpr size_t wide_shared_bytes() {
     return Wide<PAIR>::kStages * Wide<PAIR>::kStageBytes + kWideWarps * kWideStoreBytes + kWideTableBytes + 256 + 1024;
@@ -590,10 +591,11 @@ __device__ __forceinline__ void order_tile(uint32_t tile, uint32_t m_blocks, uin
     n_tile = local / height;
 }
 
-// first_tile[e]: tiles of the experts before e. The last e with first_tile[e] <= tile holds it.
+// first_tile[e]: tiles of the experts before e. The last e with first_tile[e] <= tile holds it, in its
+// rows from first_row[e] on.
 template <uint32_t HEIGHT>
-__device__ __forceinline__ WideTile locate(const GemmParams &params, const uint32_t *first_tile, uint32_t n_tiles,
-                                           uint32_t group_rows, uint32_t tile) {
+__device__ __forceinline__ WideTile locate(const GemmParams &params, const uint32_t *first_tile, const uint32_t *first_row,
+                                           uint32_t n_tiles, uint32_t group_rows, uint32_t tile) {
     WideTile result;
     uint32_t begin = 0, end = params.rows, local = tile;
     result.expert = 0;
@@ -609,9 +611,8 @@ __device__ __forceinline__ WideTile locate(const GemmParams &params, const uint3
         }
         result.expert = low_e;
         local = tile - first_tile[low_e];
-        const int32_t rows = static_cast<int32_t>(params.rows);
-        begin = static_cast<uint32_t>(min(max(params.offsets[low_e], 0), rows));
-        end = static_cast<uint32_t>(min(max(params.offsets[low_e + 1], static_cast<int32_t>(begin)), rows));
+        begin = first_row[low_e];
+        end = max(first_row[low_e + 1], begin);
     }
     uint32_t m_block, n_tile;
     order_tile(local, (end - begin + HEIGHT - 1) / HEIGHT, n_tiles, group_rows, m_block, n_tile);
@@ -730,8 +731,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     uint8_t *stage_a = smem + kStages * Shape::kWBytes;
     uint8_t *store = smem + kStages * Shape::kStageBytes;
     uint32_t *first_tile = reinterpret_cast<uint32_t *>(store + kWideWarps * kWideStoreBytes);
-    Ctl *control = reinterpret_cast<Ctl *>(store + kWideWarps * kWideStoreBytes + kWideTableBytes + 4);
-    static_assert(sizeof(Ctl) <= 248 && (kWideTableBytes + 4) % 8 == 0, "control block");
+    Ctl *control = reinterpret_cast<Ctl *>(store + kWideWarps * kWideStoreBytes + kWideTableBytes);
+    uint32_t *first_row = first_tile + QPUCUDA_MAX_EXPERTS + 1;
+    static_assert(sizeof(Ctl) <= 256 && kWideTableBytes % 8 == 0, "control block");
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31;
@@ -790,10 +792,16 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, through, offset);
                 if (lane >= static_cast<uint32_t>(offset)) through += other;
             }
-            if (e < params.experts) first_tile[e] = before + through - tiles;
+            if (e < params.experts) {
+                first_tile[e] = before + through - tiles;
+                first_row[e] = static_cast<uint32_t>(min(max(params.offsets[e], 0), rows));
+            }
             before += __shfl_sync(0xFFFFFFFFu, through, 31);
         }
-        if (lane == 0) first_tile[params.experts] = before;
+        if (lane == 0) {
+            first_tile[params.experts] = before;
+            first_row[params.experts] = static_cast<uint32_t>(min(max(params.offsets[params.experts], 0), rows));
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -810,7 +818,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             uint32_t stage = 0, phase = 0, issued_mask = 0, issued_phases = 0;
             bool ok = true;
             for (uint32_t t = tile_first; ok && t < total; t += tile_step) {
-                const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, t);
+                const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, t);
                 const int w_row = static_cast<int>(tile.expert * params.n + tile.n0 + rank * kBlockN);
                 const int a_row = static_cast<int>(tile.row0 + rank * kWideM);
                 for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
@@ -920,7 +928,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t tmem_empty0 = PAIR ? map_to_rank(smem_u32(&control->tmem_empty[0]), 0) : smem_u32(&control->tmem_empty[0]);
         uint32_t buffer = 0, buffer_phase = 0;
         for (uint32_t t = tile_first; t < total; t += tile_step) {
-            const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, t);
+            const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, t);
             const uint32_t n0 = tile.n0 + half * (kWideN / 2);
             const uint32_t row0 = tile.row0 + rank * kWideM + quarter * 32u;
             const bool row_inside = row0 + lane < tile.row_end;
@@ -1034,7 +1042,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (tile_first < total) {
                 // This CTA's share of the columns, summed in slice order: 256 / slices of them, half to
                 // each four warps, a row to a thread.
-                const WideTile tile = locate<Shape::kRows>(params, first_tile, n_tiles, group_rows, tile_first);
+                const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, tile_first);
                 constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
                 const uint32_t row0 = tile.row0 + quarter * 32u;
                 const uint32_t columns = kWideN / slices / 2u;
