@@ -4,9 +4,13 @@
 //   offsets[e] + (choices of e in earlier chunks) + (in earlier warps of its chunk) + (earlier in its warp),
 // every term an exact count, so the order never depends on timing. Up to 32768 choices (a prompt of
 // 4096 tokens with 8 choices) it is one launch of one cluster, whose CTAs read each other's counts in
-// distributed shared memory; above, a kernel counts the chunks first. Moving the rows is bound by
-// HBM: each kernel reads a token's vector once, in registers, for all of its choices, and writes each
-// row once.
+// distributed shared memory; above, a kernel counts the chunks first. Its time is latency: 16384
+// choices of 32 experts about 6 us, 160000 of 128 about 12.
+//
+// Moving the rows is bound by HBM: each kernel reads a token's vector once, in registers, for all of
+// its choices, and writes each row once. 20000 tokens x 8 choices of 2048 bf16: copies 124 us (5.9
+// TB/s of the 738 MB), sums 116 us (6.4 TB/s), gradients of the sums 227 us (6.1 TB/s); 6.56 TB/s is the
+// measured copy.
 #include "element.cuh"
 #include "qpucuda_fp8_internal.h"
 #include "qpucuda_internal.h"

@@ -8,9 +8,9 @@
 // expert's rows; the rows of the next expert that a tile's copy also brings in are computed and
 // not stored, the rows no expert owns are zeroed.
 //
-// Rows (tokens) are the narrow side here: the weight is the M = 128 operand and NT rows are the N
-// operand, so a few tokens cost a tile of NT = 16 and not 128. Tensor memory lane = output column,
-// tensor memory column = row.
+// Two kernels. A few rows per matrix are bound by the weight's bytes (narrow); many by the tensor
+// cores and, at one multiply-add per product of 128 columns beside them, by the board's power (wide).
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <type_traits>
@@ -109,6 +109,12 @@ __device__ __forceinline__ uint32_t owned_rows(const GemmParams &params) {
 
 // ---- the narrow kernel ------------------------------------------------------------------------
 
+// Few rows: the weight is the M = 128 operand and NT rows are the N operand, so they cost a tile of NT =
+// 16 or 32 and not 128. Tensor memory lane = output column, tensor memory column = row. Two CTAs an SM
+// keep 2 x 5 stages of 16 KB of weights under way. 4 x 28672 x 8192: 42 us back to back, 235 MB read
+// once (5.6 TB/s, 0.85 of the measured copy). NT = 64 and 128 were slower than the wide kernel or than
+// NT = 32 twice (64 x 11008 x 4096: 23 us at 64, 19 at 32).
+//
 // A few rows of a small matrix are quantized by the product itself: every CTA those of its K blocks,
 // at most kFusedBlocks, into shared memory, while its first weights arrive. One launch instead of two
 // (1 x 2048 x 2048 bf16: 14.4 -> 12.4 us a call, 5.3 -> 4.4 in a captured graph), as long as its four
@@ -533,6 +539,12 @@ cudaError_t launch_narrow_rows(const CUtensorMap &map_w, const CUtensorMap &map_
 // Many rows: 128 rows are the M operand, 256 output columns the N operand, so tensor memory lane =
 // row and the factor sx * sw is one number per thread and block (a row's scale; the two halves of
 // the columns are two rows of weight scales, one for each group of four epilogue warps).
+//
+// Per block of 128 columns a CTA's MMAs take 512 cycles in a pair (768 alone: both operands then come
+// from one SM's shared memory), its eight epilogue warps read 128 KB of tensor memory and form 32768
+// multiply-adds in registers meanwhile. 4096 x 28672 x 8192 bf16 in pairs: 920 us, 2.1 PFLOP/s (1.26 of
+// the measured bf16 burst), at the 1000 W power limit. Without the sums 845 us, without reading the
+// accumulators either 745, the MMAs alone 650: what is left is energy, not waiting.
 constexpr int kWideM = 128;
 constexpr int kWideN = 256;
 constexpr uint64_t kGroupBytes = 40ull << 20;  // rows of a group of tiles: part of the 126 MB L2
@@ -721,7 +733,7 @@ template <typename Out, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1)
     fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                          const __grid_constant__ CUtensorMap map_out,
-                         const GemmParams params, uint32_t n_tiles, uint32_t group_rows) {
+                         const GemmParams params, uint32_t n_tiles, uint32_t group_rows, uint32_t most_tiles) {
     using Shape = Wide<PAIR>;
     constexpr int kStages = Shape::kStages;
     using Ctl = Control<kStages, 2>;
@@ -742,7 +754,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const uint32_t slices = SPLIT ? cluster_size() : 1u;
     const uint32_t slice = SPLIT ? cluster_rank() : 0u;
     const uint32_t tile_first = PAIR ? blockIdx.x / 2 : blockIdx.x / slices;
-    const uint32_t tile_step = PAIR ? gridDim.x / 2 : gridDim.x / slices;
+    const uint32_t tile_step = PAIR ? gridDim.x / 2 : (SPLIT ? 0x80000000u : gridDim.x);
     const uint32_t kb_begin = SPLIT ? static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * slice / slices) : 0u;
     const uint32_t kb_end = SPLIT ? static_cast<uint32_t>(static_cast<uint64_t>(params.k_blocks) * (slice + 1) / slices) : params.k_blocks;
     if (threadIdx.x == 0) {
@@ -808,7 +820,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any arrival or copy of the other
     tc_fence_after();
     const uint32_t tmem_base = control->tmem_base;
-    const uint32_t total = params.experts != 0 ? first_tile[params.experts] : (params.rows + Shape::kRows - 1) / Shape::kRows * n_tiles;
+    // no more than ascending offsets can make
+    const uint32_t total = params.experts != 0 ? min(first_tile[params.experts], most_tiles) : most_tiles;
 
     if (warp == 0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
@@ -1164,7 +1177,7 @@ cudaError_t launch_wide(const CUtensorMap &map_w, const CUtensorMap &map_a, Gemm
                            ? 1u
                            : 0u;
     return cudaLaunchKernelEx(&config, fp8_gemm_wide_kernel<Out, PAIR, SPLIT>, map_w, map_a, map_out, params, launch.n_tiles,
-                              launch.group_rows);
+                              launch.group_rows, static_cast<uint32_t>(launch.tiles));
 }
 
 template <typename Out>
@@ -1259,7 +1272,8 @@ cudaError_t launch_gemm(const qpucuda_fp8_gemm_desc &desc, const qpucuda_fp8_qua
             return cudaErrorInvalidValue;
         }
         const uint64_t group = kGroupBytes / (static_cast<uint64_t>(wide.pair ? 2 * kWideM : kWideM) * desc.k);
-        wide.group_rows = static_cast<uint32_t>(group < kGroupRows ? kGroupRows : (group < 0x10000u ? group : 0x10000u));
+        const uint64_t row_blocks = wide.tiles / wide.n_tiles;
+        wide.group_rows = static_cast<uint32_t>(std::min(std::max(group, kGroupRows), row_blocks));
         switch (desc.out_type) {
             case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(map_w, map_a, params, wide, sm_count, stream);
             case QPUCUDA_DTYPE_BF16: return launch_wide_type<__nv_bfloat16>(map_w, map_a, params, wide, sm_count, stream);

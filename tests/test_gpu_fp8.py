@@ -333,6 +333,19 @@ def test_offsets_beyond_the_rows_are_clamped(cuda_device, rows) -> None:
         assert torch.equal(plan.forward(x, inside), plan.forward(x, beyond))
 
 
+@pytest.mark.parametrize("rows", [40, 900])
+def test_offsets_out_of_order_stay_inside_the_output(cuda_device, rows) -> None:
+    """Overlapping ranges leave rows unspecified; nothing outside the output is written and the call ends."""
+    weight = blocks(cuda_device, 200, 2048, experts=4)
+    x = draw((rows, 2048), seed=1)
+    wide = torch.full((rows + 2, 208), 7.0, device="cuda")
+    offsets = torch.tensor([0, rows, rows // 4, 2 * rows, 0], dtype=torch.int32, device="cuda")
+    with PreparedFP8Experts(cuda_device, weight) as plan:
+        plan.forward(x, offsets, out=wide[1:-1, 8:])
+        torch.cuda.synchronize()
+    assert (wide[[0, -1]] == 7.0).all() and (wide[:, :8] == 7.0).all()
+
+
 def test_experts_nan_rows_do_not_reach_a_neighbouring_expert(cuda_device) -> None:
     weight, x, offsets, exact, magnitude = expert_case(cuda_device, [5, 4, 6], 256, 256)
     x[5:9] = float("nan")
