@@ -170,11 +170,15 @@ __device__ __forceinline__ void fuse_rows(const FusedRows &rows, const GemmParam
         }
         float v[kVector<T>], amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kVector<T>; ++i) {
-            v[i] = to_float(raw[0].items[i]);
-            if (GATED) v[i] = silu_times(v[i], to_float(raw_up[0].items[i]));
-            amax = max_nan(amax, fabsf(v[i]));
+        for (int i = 0; i < kVector<T>; ++i) v[i] = to_float(raw[0].items[i]);
+        if constexpr (GATED) {
+            float up[kVector<T>];
+#pragma unroll
+            for (int i = 0; i < kVector<T>; ++i) up[i] = to_float(raw_up[0].items[i]);
+            silu_times(v, up);
         }
+#pragma unroll
+        for (int i = 0; i < kVector<T>; ++i) amax = max_nan(amax, fabsf(v[i]));
         const float scale = group_scale(group_max<kLanes>(amax));
         uint32_t packed[kVector<T> / 4];
         quantize_values(v, scale, packed);

@@ -31,7 +31,7 @@ struct RowsParams {
 // STEPS steps of one or two neighbouring groups of one row, at fixed distances from one address, and
 // loads them all before it uses the first (39 against 27 us). Each input is read once, each output
 // written once; what it has to keep below HBM's time is its instructions, 14 a value. 32768 x 8192
-// bf16: 142 us (5.7 TB/s), 4096 x 8192 fp32: 27 us (6.1 TB/s), gated bf16: 31 us (5.4 TB/s).
+// bf16: 142 us (5.7 TB/s), 4096 x 8192 fp32: 27 us (6.1 TB/s), gated bf16: 39 us (4.3 TB/s).
 constexpr int kRowsThreads = 128;
 
 template <typename T, bool GATED, bool VECTOR, int STEPS>
@@ -75,11 +75,15 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
         for (int u = 0; u < STEPS; ++u) {
             float v[kVector<T>], amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kVector<T>; ++i) {
-                v[i] = to_float(raw[u].items[i]);
-                if constexpr (GATED) v[i] = silu_times(v[i], to_float(raw_up[u].items[i]));
-                amax = max_nan(amax, fabsf(v[i]));
+            for (int i = 0; i < kVector<T>; ++i) v[i] = to_float(raw[u].items[i]);
+            if constexpr (GATED) {
+                float up[kVector<T>];
+#pragma unroll
+                for (int i = 0; i < kVector<T>; ++i) up[i] = to_float(raw_up[u].items[i]);
+                silu_times(v, up);
             }
+#pragma unroll
+            for (int i = 0; i < kVector<T>; ++i) amax = max_nan(amax, fabsf(v[i]));
             const float scale = group_scale(group_max<kLanes>(amax));
             uint32_t packed[kVector<T> / 4];
             quantize_values(v, scale, packed);

@@ -55,9 +55,43 @@ __device__ __forceinline__ void quantize_values(const float (&v)[N], float scale
     for (int i = 0; i < N / 4; ++i) packed[i] = pairs[2 * i] | (static_cast<uint32_t>(pairs[2 * i + 1]) << 16);
 }
 
-// silu(g) * u in fp32. exp(-g) overflows to infinity below g = -88.7, where the quotient is then -0
-// as it should be to fp32's range.
-__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// v = silu(v) * up = v / (1 + exp(-v)) * up in fp32, every step to the last bit: a value that the
+// quantizer then rounds to three bits should not land on the other side of a border for an
+// approximation's sake. The quotient is Markstein's: q0 = g y with y within 2^-23 of 1 / d, corrected
+// by its exact remainder, is within 2^-45 of g / d before it is rounded. Below -87 the denominator's
+// reciprocal is no normal number, and the hardware's division (-0 once exp overflows) takes over.
+// 4096 x 8192 bf16: 39 us, with a division per value 46, with the fast exp and quotient 31.
+template <int N>
+__device__ __forceinline__ void silu_times(float (&v)[N], const float (&up)[N]) {
+    using sm100::fma2;
+    using sm100::pack2;
+    float least = 0.0f, d[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        d[i] = __fadd_rn(1.0f, expf(-v[i]));
+        least = fminf(least, v[i]);
+    }
+    if (least < -87.0f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fmul_rn(__fdiv_rn(v[i], d[i]), up[i]);
+        return;
+    }
+    const uint64_t zero = pack2(-0.0f, -0.0f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t g = pack2(v[i], v[i + 1]), y = pack2(reciprocal(d[i]), reciprocal(d[i + 1]));
+        uint64_t q = fma2(g, y, zero);
+        q = fma2(fma2(q, pack2(-d[i], -d[i + 1]), g), y, q);
+        v[i] = __fmul_rn(sm100::low(q), up[i]);
+        v[i + 1] = __fmul_rn(sm100::high(q), up[i + 1]);
+    }
+}
 
 // kVector elements at x, zero from `remaining` of them on. Full vectors first and the ragged end of a
 // row in a pass of its own, so that nothing stands between the loads of several steps.

@@ -92,20 +92,31 @@ def test_row_quantizer_takes_strided_and_unaligned_rows(cuda_device, dtype) -> N
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows, cols", [(1, 1), (4, 128), (7, 333), (40, 5632)])
-def test_gated_rows(cuda_device, dtype, rows, cols) -> None:
-    """CUDA's bound on the fast exp is 2 + 1.173 |gate| steps of 2^-23 (8 for the |gate| < 6 drawn here),
-    on the fast quotient 2; the sum and the product round once each: below 2^-19 together, so the
-    scale is that close. The value is then within half an e4m3 step (2^-4 of it, or 2^-10 of the
-    scale below the normal range)."""
-    x = draw((rows, 2 * cols), dtype, seed=cols)
+@pytest.mark.parametrize("rows, cols, std", [(1, 1, 1.0), (4, 128, 1.0), (7, 333, 3.0), (40, 5632, 1.0), (50, 500, 40.0)])
+def test_gated_rows(cuda_device, dtype, rows, cols, std) -> None:
+    """exp is within 2 steps of 2^-23 (CUDA's bound), the sum and the product round once, the quotient is
+    the rounded one: below 5 steps (2^-20.6) together, so the scale is that close. The value is then
+    within half an e4m3 step (2^-4 of it, or 2^-10 of the scale below the normal range). Gates down to
+    -160 go through the overflow of exp."""
+    x = draw((rows, 2 * cols), dtype, seed=cols, std=std)
     rows_fp8 = quantize_rows_fp8(cuda_device, x, gated=True)
     exact = ref.silu_gate(x)
     _, scales = ref.quantize_rows(exact)
-    torch.testing.assert_close(rows_fp8.scales.double(), scales, rtol=2.0**-19, atol=0)
+    torch.testing.assert_close(rows_fp8.scales.double(), scales, rtol=2.0**-20, atol=0)
     wide = ref.spread(rows_fp8.scales.double(), rows, cols, 1)
-    bound = exact.abs() * (2.0**-4 + 2.0**-18) + wide * (2.0**-10 + 2.0**-18)
+    bound = exact.abs() * (2.0**-4 + 2.0**-19) + wide * (2.0**-10 + 2.0**-19)
     assert ((rows_fp8.dequantize().double() - exact).abs() <= bound).all()
+
+
+def test_gates_of_every_size(cuda_device) -> None:
+    """One gate per group, across the range of fp32's exp and past both of its ends."""
+    gates = torch.cat([torch.linspace(-110.0, 110.0, 400), torch.tensor([-1e30, -1e-30, 0.0, 1e-30, 1e30])])
+    x = torch.zeros((gates.numel(), 256), device="cuda")
+    x[:, 0], x[:, 128] = gates.cuda(), 3.0
+    exact = ref.silu_gate(x)[:, 0]
+    have = quantize_rows_fp8(cuda_device, x, gated=True).scales[:, 0].double() * 448.0
+    wanted = exact.abs().clamp_min(448.0 * 2.0**-60)
+    assert ((have - wanted).abs() <= 2.0**-20 * wanted).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
