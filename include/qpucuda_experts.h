@@ -7,6 +7,7 @@
  * Every token t makes `choices` choices; choice (t, j) has the flat index
  * t * choices + j. Rows are ordered by expert, then by flat index; an expert id
  * outside [0, experts) drops the choice.
+ * Outputs share no bytes with what a call reads.
  *
  *   offsets[e], offsets[e + 1]   the rows of expert e
  *   source[row]                  the flat index at that row, -1 from offsets[experts] on

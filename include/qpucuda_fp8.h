@@ -85,7 +85,7 @@ typedef struct qpucuda_fp8_gemm_desc {
      * offsets[experts] on become zero. At most QPUCUDA_MAX_EXPERTS. */
     uint32_t experts;
     const int32_t *offsets;
-    void *out;               /* [rows][n] */
+    void *out;               /* [rows][n]; shares no bytes with what the call reads */
     int out_type;            /* qpucuda_dtype */
     size_t out_stride;       /* elements */
     /* Nonzero: w, w_scales and offsets were complete before the kernel queued just before this one

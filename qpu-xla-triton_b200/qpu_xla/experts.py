@@ -25,6 +25,7 @@ from qpu_xla.fp8 import (
     MAX_EXPERTS,
     PreparedFP8Experts,
     QuantizedBlocksFP8,
+    check_apart,
     check_matrix,
     dtype_code,
     launch,
@@ -107,19 +108,13 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
 
 
 def _destination(out: Any, rows: int, width: int, read: Any, torch_device: Any, what: str) -> tuple[Any, int]:
-    """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride. It may not overlap
-    ``read``: the kernels read and write in no particular order."""
+    """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride."""
     if out is None:
         return new_matrix(rows, width, read.dtype, torch_device), max(width, 1)
     if out.dtype != read.dtype:
         raise ValueError(f"{what} must have the type of its source")
     stride = check_matrix(out, torch_device, what, rows, width)[2]
-    if out.numel() and read.numel():
-        (begin, end), (read_begin, read_end) = (
-            (t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()) for t in (out, read)
-        )
-        if begin < read_end and read_begin < end:
-            raise ValueError(f"{what} must not overlap its source")
+    check_apart(out, read, what)
     return out, stride
 
 

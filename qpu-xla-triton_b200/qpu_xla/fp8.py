@@ -80,6 +80,28 @@ def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = N
     return have_rows, have_cols, stride
 
 
+def check_apart(out: Any, read: Any, what: str) -> None:
+    """Refuse an ``out`` that shares bytes with the matrix the call reads: kernels read and write in no
+    particular order. Column ranges of one buffer do not meet."""
+    if _meet(*((t.data_ptr(), *t.shape, t.stride(0) * t.element_size(), t.element_size()) for t in (out, read))):
+        raise ValueError(f"{what} must not overlap its source")
+
+
+def _meet(one: tuple[int, ...], other: tuple[int, ...]) -> bool:
+    """Whether two row-major matrices (address, rows, columns, row stride in bytes, element size) share
+    bytes; of different row strides, whether their ranges of addresses do."""
+    (begin, rows, cols, stride, size), (other_begin, other_rows, other_cols, other_stride, other_size) = one, other
+    if 0 in (rows, cols, other_rows, other_cols):
+        return False
+    width, other_width = cols * size, other_cols * other_size
+    if begin >= other_begin + (other_rows - 1) * other_stride + other_width or other_begin >= begin + (rows - 1) * stride + width:
+        return False
+    if stride == other_stride and stride > 0:
+        gap = (begin - other_begin) % stride
+        return gap < other_width or gap + width > stride
+    return True
+
+
 def new_matrix(rows: int, cols: int, dtype: Any, torch_device: Any) -> Any:
     """An uninitialised row-major matrix (``empty_strided`` costs the host a third less than ``empty``)."""
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=torch_device)
@@ -232,6 +254,7 @@ class _PreparedFP8:
         self._scales_address = self._scales.data_ptr()
         self._bias_address = None if self._bias is None else self._bias.data_ptr()
         torch.cuda.current_stream(self._torch_device).synchronize()
+        self._pending: list[Event] = []  # executions on queues that may not have been launched yet
         self._closed = False
 
     def __enter__(self: Self) -> Self:
@@ -246,9 +269,14 @@ class _PreparedFP8:
             raise RuntimeError(f"{self._name} plan is closed")
 
     def close(self: Self) -> None:
-        """Wait for the device and release the weight."""
+        """Wait for queued executions and for the device, and release the weight."""
         if self._closed:
             return
+        for event in self._pending:
+            try:
+                event.wait()
+            except Exception:
+                pass
         torch.cuda.synchronize(self._torch_device)
         self._values = self._scales = self._bias = None
         self._closed = True
@@ -258,7 +286,7 @@ class _PreparedFP8:
         self._require_open()
         return sum(t.numel() * t.element_size() for t in (self._values, self._scales, self._bias) if t is not None)
 
-    def _output(self: Self, rows: int, out: Any, dtype: Any, default: Any) -> tuple[Any, int]:
+    def _output(self: Self, rows: int, out: Any, dtype: Any, read: Any, default: Any) -> tuple[Any, int]:
         if out is None:
             dtype = default if dtype is None else dtype
             dtype_code(dtype, f"{self._name} output")
@@ -266,7 +294,9 @@ class _PreparedFP8:
         if dtype is not None and out.dtype != dtype:
             raise ValueError(f"{self._name} out and dtype differ")
         dtype_code(out.dtype, f"{self._name} output")
-        return out, check_matrix(out, self._torch_device, f"{self._name} output", rows, self.output_count)[2]
+        stride = check_matrix(out, self._torch_device, f"{self._name} output", rows, self.output_count)[2]
+        check_apart(out, read, f"{self._name} output")
+        return out, stride
 
     def _gemm_desc(
         self: Self, a: int, a_stride: int, a_scales: int, scale_strides: tuple[int, int], rows: int, out_address: int, out_code: int,
@@ -325,10 +355,10 @@ class PreparedFP8Linear(_PreparedFP8):
 
     def forward(self: Self, source: Any, out: Any = None, *, dtype: Any = None) -> Any:
         """Rows ``[M, K]`` (float32, bfloat16 or float16) to ``[M, N]`` of ``dtype`` (default: the
-        source's type, or ``out``'s)."""
+        source's type, or ``out``'s). ``out`` may share a buffer with the source, but no bytes."""
         self._require_open()
         rows, stride, code = self._check_source(source)
-        out, out_stride = self._output(rows, out, dtype, source.dtype)
+        out, out_stride = self._output(rows, out, dtype, source, source.dtype)
         if rows:
             self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride)
         return out
@@ -338,7 +368,7 @@ class PreparedFP8Linear(_PreparedFP8):
         defaults to float32."""
         self._require_open()
         count, stride, scale_strides = self._check_rows(rows)
-        out, out_stride = self._output(count, out, dtype, torch.float32)
+        out, out_stride = self._output(count, out, dtype, rows.values, torch.float32)
         if count:
             gemm = self._gemm_desc(
                 rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride
@@ -357,6 +387,8 @@ class PreparedFP8Linear(_PreparedFP8):
             raise ValueError("prepared FP8 linear source and destination shapes do not align")
         if source.strides[1] != 4 or destination.strides[1] != 4:
             raise ValueError("prepared FP8 linear requires unit inner strides")
+        if _meet(*((t.address, *t.shape, t.strides[0], 4) for t in (destination, source))):
+            raise ValueError("prepared FP8 linear destination must not overlap its source")
         rows = int(source.shape[0])
 
         def executor(backend: Any, args: tuple[Any, ...], grid: tuple[int, int, int], stream: Any) -> None:
@@ -366,10 +398,13 @@ class PreparedFP8Linear(_PreparedFP8):
                     destination.row_stride_elements, stream=stream.cuda_stream,
                 )
 
-        return queue.submit(
+        event = queue.submit(
             Kernel("cuda.fp8_linear", executor), (), wait_for=wait_for,
             buffers=(source.access(AccessMode.READ), destination.access(AccessMode.WRITE)),
         )
+        self._pending = [pending for pending in self._pending if not pending.done]
+        self._pending.append(event)
+        return event
 
 
 class PreparedFP8Experts(_PreparedFP8):
@@ -397,7 +432,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._require_open()
         rows, stride, code = self._check_source(source)
         self._check_offsets(offsets)
-        out, out_stride = self._output(rows, out, dtype, source.dtype)
+        out, out_stride = self._output(rows, out, dtype, source, source.dtype)
         if rows:
             self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, offsets.data_ptr())
         return out
@@ -410,7 +445,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._check_offsets(order.offsets)
         order.check(self._torch_device, tokens=tokens_count)
         rows = order.rows
-        out, out_stride = self._output(rows, out, dtype, tokens.dtype)
+        out, out_stride = self._output(rows, out, dtype, tokens, tokens.dtype)
         if rows:
             self._linear(
                 tokens.data_ptr(), code, tokens_count, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, order.offsets.data_ptr(),

@@ -9,7 +9,15 @@ import torch
 
 from qpu_xla import Device, _native
 from qpu_xla.experts import ExpertOrder, FP8ExpertsFFN, gather_tokens, sort_tokens
-from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, QuantizedBlocksFP8, QuantizedRowsFP8, quantize_blocks_fp8, quantize_rows_fp8
+from qpu_xla.fp8 import (
+    PreparedFP8Experts,
+    PreparedFP8Linear,
+    QuantizedBlocksFP8,
+    QuantizedRowsFP8,
+    check_apart,
+    quantize_blocks_fp8,
+    quantize_rows_fp8,
+)
 
 E4M3 = torch.float8_e4m3fn
 
@@ -98,3 +106,37 @@ def test_sort_workspace_is_only_needed_past_one_cluster() -> None:
     assert size(4097, 8, 64) > 0 and size(4097, 8, 64) % (4 * 64) == 0
     assert size(0, 8, 64) == 0 and size(8, 0, 64) == 0 and size(8, 8, 1025) == 0
     assert size(2**31, 2, 4) == 0
+
+
+def meets_by_bytes(one: torch.Tensor, other: torch.Tensor) -> bool:
+    def touched(t: torch.Tensor) -> set[int]:
+        size = t.element_size()
+        return {
+            t.data_ptr() + r * t.stride(0) * size + c for r in range(t.shape[0]) for c in range(t.shape[1] * size)
+        }
+
+    return bool(touched(one) & touched(other))
+
+
+def test_outputs_may_share_a_buffer_with_the_source_but_no_bytes() -> None:
+    flat = torch.zeros(400)
+    for rows in (1, 2, 5):
+        for stride in (7, 12):
+            for begin in range(0, 90, 3):
+                for width in (1, 4, 7):
+                    one = flat.as_strided((rows, width), (stride, 1), begin)
+                    other = flat.as_strided((3, 5), (stride, 1), 30)
+                    if meets_by_bytes(one, other):
+                        with pytest.raises(ValueError, match="overlap"):
+                            check_apart(one, other, "out")
+                    else:
+                        check_apart(one, other, "out")
+    both = flat.as_strided((6, 12), (12, 1))
+    check_apart(both[:, 5:], both[:, :5], "out")
+    check_apart(both[:, :5], both[:, 5:], "out")
+    check_apart(both[1:3, 5:], both[:, :5], "out")
+    for out, source in ((both, both), (both[:, 4:], both[:, :5]), (both[:, :5], both[3:, 4:9]), (both.view(torch.bfloat16)[:, 8:], both[:, :5])):
+        with pytest.raises(ValueError, match="overlap"):
+            check_apart(out, source, "out")
+    check_apart(both.view(torch.bfloat16)[:, 10:], both[:, :5], "out")
+    check_apart(both[:0], both, "out")

@@ -3,6 +3,8 @@ the rounding bound of their fp32 sums."""
 
 from __future__ import annotations
 
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -409,6 +411,46 @@ def test_execute_on_a_queue(cuda_device) -> None:
         source.write(x)
         plan.execute(destination, source, queue=queue).wait()
         np.testing.assert_array_equal(destination.numpy(), plan.forward(torch.from_numpy(x).cuda()).cpu().numpy())
+
+
+def test_close_waits_for_queued_executions(cuda_device) -> None:
+    weight = blocks(cuda_device, 96, 160)
+    x = np.random.default_rng(1).standard_normal((5, 160), dtype=np.float32)
+    with PreparedFP8Linear(cuda_device, weight) as plan:
+        expected = plan.forward(torch.from_numpy(x).cuda()).cpu().numpy()
+    with cuda_device.queue() as queue:
+        source, destination = cuda_device.tensor((5, 160), np.float32), cuda_device.tensor((5, 96), np.float32)
+        source.write(x)
+        plan = PreparedFP8Linear(cuda_device, weight)
+        events = [queue.host_task(lambda: time.sleep(0.05)), *(plan.execute(destination, source, queue=queue) for _ in range(3))]
+        plan.close()
+        assert all(event.done for event in events)
+        np.testing.assert_array_equal(destination.numpy(), expected)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40, 600])
+def test_source_and_output_in_one_buffer(cuda_device, rows) -> None:
+    """Column ranges that do not meet give what separate tensors give; an output over its source is refused."""
+    n = k = 256
+    weight = blocks(cuda_device, n, k)
+    both = draw((rows, k + n), torch.bfloat16)
+    source = both[:, :k].clone()
+    with PreparedFP8Linear(cuda_device, weight) as plan:
+        expected = plan.forward(source)
+        with pytest.raises(ValueError, match="overlap"):
+            plan.forward(source, out=source)
+        plan.forward(both[:, :k], out=both[:, k:])
+        torch.testing.assert_close(both, torch.cat((source, expected), 1), rtol=0, atol=0)
+    with PreparedFP8Experts(cuda_device, blocks(cuda_device, n, k, experts=2)) as plan:
+        with pytest.raises(ValueError, match="overlap"):
+            plan.forward(source, torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda"), out=source)
+
+
+def test_execute_refuses_an_output_over_its_source(cuda_device) -> None:
+    with cuda_device.queue() as queue, PreparedFP8Linear(cuda_device, blocks(cuda_device, 64, 64)) as plan:
+        source = cuda_device.tensor((5, 64), np.float32)
+        with pytest.raises(ValueError, match="overlap"):
+            plan.execute(source, source, queue=queue)
 
 
 def test_results_repeat_bit_for_bit(cuda_device) -> None:
