@@ -3,6 +3,7 @@ the rounding bound of their fp32 sums."""
 
 from __future__ import annotations
 
+import threading
 import time
 
 import numpy as np
@@ -451,6 +452,93 @@ def test_execute_refuses_an_output_over_its_source(cuda_device) -> None:
         source = cuda_device.tensor((5, 64), np.float32)
         with pytest.raises(ValueError, match="overlap"):
             plan.execute(source, source, queue=queue)
+
+
+@pytest.mark.parametrize("n", [8192, 8191])
+def test_rows_beyond_32_bit_offsets(cuda_device, n) -> None:
+    """2.2e9 outputs, of the copy engine and of the warps: the last rows lie past 2^31 elements."""
+    rows, k = 270_000, 256
+    weight = blocks(cuda_device, n, k)
+    x = draw((rows, k), torch.bfloat16)
+    picked = torch.cat([torch.arange(150), torch.arange(131_000, 131_300), torch.arange(rows - 301, rows)]).cuda()
+    exact, magnitude = ref.product(*ref.quantize_rows(x[picked]), weight.values, weight.scales)
+    with PreparedFP8Linear(cuda_device, weight) as plan:
+        y = plan.forward(x)
+        check_product(y[picked], exact, magnitude, k)
+    del y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_row_quantizer_beyond_32_bit_offsets(cuda_device, gated) -> None:
+    rows, cols = 270_000, 8192
+    tile = draw((250, cols), torch.bfloat16, seed=4)
+    quantized = quantize_rows_fp8(cuda_device, tile.repeat(rows // 250, 1), gated=gated)
+    expected = quantize_rows_fp8(cuda_device, tile, gated=gated)
+    if not gated:
+        check_rows(expected, tile)
+    width = expected.shape[1]
+    assert torch.equal(quantized.values.view(torch.uint8).view(-1, 250, width), expected.values.view(torch.uint8).expand(rows // 250, -1, -1))
+    assert torch.equal(quantized.scales.view(-1, 250, width // 128), expected.scales.expand(rows // 250, -1, -1))
+    del quantized
+    torch.cuda.empty_cache()
+
+
+def test_weight_beyond_32_bit_offsets(cuda_device) -> None:
+    """4.6e9 bytes of weight, one matrix and one of three: both kernels, the last columns."""
+    for shape in ((70_000, 65_536), (3, 24_000, 65_536)):
+        tile = draw((250, 65_536), torch.bfloat16, seed=5, std=0.05)
+        full = tile.repeat(shape[-2] * (shape[0] if len(shape) == 3 else 1) // 250, 1).view(shape)
+        weight = quantize_blocks_fp8(cuda_device, full)
+        del full
+        last = slice(shape[-2] - 300 - shape[-2] % 128, shape[-2])
+        last = slice(last.start // 128 * 128, last.stop)
+        matrix, scales = (weight.values, weight.scales) if len(shape) == 2 else (weight.values[-1], weight.scales[-1])
+        for rows in (3, 100):
+            x = draw((rows, shape[-1]), torch.bfloat16, seed=rows)
+            exact, magnitude = ref.product(*ref.quantize_rows(x), matrix[last], scales[last.start // 128 :])
+            if len(shape) == 2:
+                with PreparedFP8Linear(cuda_device, weight) as plan:
+                    y = plan.forward(x)
+            else:
+                offsets = torch.tensor([0, 0, 0, rows], dtype=torch.int32, device="cuda")
+                with PreparedFP8Experts(cuda_device, weight) as plan:
+                    y = plan.forward(x, offsets)
+            check_product(y[:, last], exact, magnitude, shape[-1])
+        check_tile = ref.quantize_blocks(torch.cat([tile, tile, tile])[last.start % 250 :][:128])
+        assert torch.equal(matrix[last][:128].double(), check_tile[0])
+        del weight, matrix, scales, plan, y
+        torch.cuda.empty_cache()
+
+
+def test_one_plan_in_two_threads(cuda_device) -> None:
+    """Calls at once from threads with a stream each, beside executions on a queue."""
+    weight = blocks(cuda_device, 640, 1024)
+    inputs = [draw((rows, 1024), seed=rows) for rows in (3, 200)]
+    results: list[list[torch.Tensor]] = [[], []]
+    with PreparedFP8Linear(cuda_device, weight) as plan, cuda_device.queue() as queue:
+        expected = [plan.forward(x) for x in inputs]
+        torch.cuda.synchronize()
+
+        def call(i: int) -> None:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    results[i].append(plan.forward(inputs[i]))
+
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(2)]
+        source, destination = cuda_device.tensor((3, 1024), np.float32), cuda_device.tensor((3, 640), np.float32)
+        source.write(inputs[0].cpu().numpy())
+        for thread in threads:
+            thread.start()
+        for _ in range(20):
+            plan.execute(destination, source, queue=queue)
+        for thread in threads:
+            thread.join()
+        torch.cuda.synchronize()
+        queue.finish()
+        np.testing.assert_array_equal(destination.numpy(), expected[0].cpu().numpy())
+    for got, want in zip(results, expected):
+        assert len(got) == 50 and all(torch.equal(y, want) for y in got)
 
 
 def test_results_repeat_bit_for_bit(cuda_device) -> None:
