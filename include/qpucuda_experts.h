@@ -28,45 +28,45 @@ extern "C" {
 /* Scratch bytes of qpucuda_expert_sort (0 is possible). */
 size_t qpucuda_expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts);
 
-/* ids: [tokens][choices] int32, or int64 when ids_64 is nonzero. experts <= QPUCUDA_MAX_EXPERTS,
- * tokens * choices < 2^31. workspace: 4-byte aligned, used by this call alone until it has run. */
-qpucuda_status qpucuda_expert_sort(
-    qpucuda_context *context,
-    const void *ids, int ids_64,
-    uint32_t tokens, uint32_t choices, uint32_t experts,
-    int32_t *offsets, int32_t *source, int32_t *position,
-    void *workspace, size_t workspace_bytes);
+typedef struct qpucuda_expert_sort_desc {
+    const void *ids;         /* [tokens][choices] int32, or int64 when ids_64 is nonzero */
+    int ids_64;
+    uint32_t tokens, choices, experts; /* experts <= QPUCUDA_MAX_EXPERTS, tokens * choices < 2^31 */
+    int32_t *offsets, *source, *position;
+    void *workspace;         /* 4-byte aligned, used by this call alone until it has run */
+    size_t workspace_bytes;
+} qpucuda_expert_sort_desc;
 
-/* rows[position[t, j]] = x[t]; rows from offsets[experts] on (read from `offsets`) become zero.
- * x [tokens][width], rows [tokens * choices][width], both of `type` (qpucuda_dtype). */
-qpucuda_status qpucuda_expert_gather(
-    qpucuda_context *context,
-    const void *x, int type, size_t x_stride,
-    uint32_t tokens, uint32_t choices, uint32_t width,
-    const int32_t *position, const int32_t *offsets, uint32_t experts,
-    void *rows, size_t rows_stride);
+qpucuda_status qpucuda_expert_sort(qpucuda_context *context, const qpucuda_expert_sort_desc *desc);
 
-/* out[t] = sum_j weight[t, j] * rows[position[t, j]] in fp32, in the order of j, rounded once.
- * weights NULL: all one, which is the gradient of qpucuda_expert_gather. */
-qpucuda_status qpucuda_expert_combine(
-    qpucuda_context *context,
-    const void *rows, int type, size_t rows_stride,
-    uint32_t tokens, uint32_t choices, uint32_t width,
-    const int32_t *position, const float *weights,
-    void *out, size_t out_stride);
+/* One move of rows between the tokens' order, [tokens][width], and the experts', [tokens *
+ * choices][width]; strides in elements. */
+typedef struct qpucuda_expert_rows_desc {
+    int type;                /* qpucuda_dtype of source, grad and out */
+    uint32_t tokens, choices, width, experts;
+    const int32_t *position, *offsets; /* of the sort; combine reads no offsets */
+    const float *weights;    /* [tokens][choices]; gather has none */
+    const void *source;
+    size_t source_stride;
+    const void *grad;        /* combine_backward: the gradient of the tokens, and where the weights' goes */
+    size_t grad_stride;
+    float *grad_weights;
+    void *out;
+    size_t out_stride;
+} qpucuda_expert_rows_desc;
 
-/* The gradients of qpucuda_expert_combine: grad_rows[position[t, j]] = weight[t, j] * grad[t],
- * zero from offsets[experts] on; grad_weights[t, j] = <rows[position[t, j]], grad[t]> in fp32,
- * zero when dropped. */
-qpucuda_status qpucuda_expert_combine_backward(
-    qpucuda_context *context,
-    const void *rows, int type, size_t rows_stride,
-    const void *grad, size_t grad_stride,
-    uint32_t tokens, uint32_t choices, uint32_t width,
-    const int32_t *position, const int32_t *offsets, uint32_t experts,
-    const float *weights,
-    void *grad_rows, size_t grad_rows_stride,
-    float *grad_weights);
+/* Tokens to the experts' order: out[position[t, j]] = source[t]; rows from offsets[experts] on become
+ * zero. */
+qpucuda_status qpucuda_expert_gather(qpucuda_context *context, const qpucuda_expert_rows_desc *desc);
+
+/* And back: out[t] = sum_j weight[t, j] * source[position[t, j]] in fp32, in the order of j, rounded
+ * once. weights NULL: all one, which is the gradient of qpucuda_expert_gather. */
+qpucuda_status qpucuda_expert_combine(qpucuda_context *context, const qpucuda_expert_rows_desc *desc);
+
+/* The gradients of qpucuda_expert_combine, whose source is given again: out[position[t, j]] =
+ * weight[t, j] * grad[t], zero from offsets[experts] on; grad_weights[t, j] = <source[position[t, j]],
+ * grad[t]> in fp32, zero when dropped. */
+qpucuda_status qpucuda_expert_combine_backward(qpucuda_context *context, const qpucuda_expert_rows_desc *desc);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

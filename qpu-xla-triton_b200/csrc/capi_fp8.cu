@@ -35,6 +35,15 @@ bool routing_fits(uint32_t tokens, uint32_t choices, uint32_t experts) {
            static_cast<uint64_t>(tokens) * choices <= static_cast<uint64_t>(INT32_MAX);
 }
 
+bool present(const void *p) { return p != nullptr && aligned(p, 4); }
+
+// What every move of rows reads and writes.
+bool rows_fit(const qpucuda_expert_rows_desc &desc) {
+    return known_type(desc.type) && desc.width != 0 && present(desc.position) && desc.source != nullptr && desc.out != nullptr &&
+           desc.source_stride >= desc.width && desc.out_stride >= desc.width && aligned(desc.source, type_bytes(desc.type)) &&
+           aligned(desc.out, type_bytes(desc.type));
+}
+
 // Argument checks: QPUCUDA_OK, or the refusal with its message. `rows` is not zero.
 qpucuda_status check_quantize(qpucuda_context *context, const qpucuda_fp8_quantize_desc *desc) {
     const uint64_t width = static_cast<uint64_t>(desc->cols) * (desc->gated != 0 ? 2u : 1u);
@@ -132,77 +141,50 @@ size_t qpucuda_expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t
     return routing_fits(tokens, choices, experts) ? expert_sort_workspace(tokens, choices, experts) : 0;
 }
 
-qpucuda_status qpucuda_expert_sort(qpucuda_context *context, const void *ids, int ids_64, uint32_t tokens,
-                                   uint32_t choices, uint32_t experts, int32_t *offsets, int32_t *source,
-                                   int32_t *position, void *workspace, size_t workspace_bytes) {
-    if (context == nullptr) return QPUCUDA_INVALID_ARGUMENT;
-    if (!routing_fits(tokens, choices, experts) || offsets == nullptr || !aligned(offsets, 4) ||
-        (tokens != 0 && (ids == nullptr || source == nullptr || position == nullptr || !aligned(ids, ids_64 != 0 ? 8 : 4) ||
-                         !aligned(source, 4) || !aligned(position, 4)))) {
+qpucuda_status qpucuda_expert_sort(qpucuda_context *context, const qpucuda_expert_sort_desc *desc) {
+    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    const qpucuda_expert_sort_desc &d = *desc;
+    if (!routing_fits(d.tokens, d.choices, d.experts) || d.offsets == nullptr || !aligned(d.offsets, 4) ||
+        (d.tokens != 0 && (d.ids == nullptr || d.source == nullptr || d.position == nullptr ||
+                           !aligned(d.ids, d.ids_64 != 0 ? 8 : 4) || !aligned(d.source, 4) || !aligned(d.position, 4)))) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT,
                     "expert_sort: needs 1 to %u experts, at least one choice and fewer than 2^31 of them", QPUCUDA_MAX_EXPERTS);
     }
-    const size_t needed = expert_sort_workspace(tokens, choices, experts);
-    if (needed != 0 && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 4))) {
+    const size_t needed = expert_sort_workspace(d.tokens, d.choices, d.experts);
+    if (needed != 0 && (d.workspace == nullptr || d.workspace_bytes < needed || !aligned(d.workspace, 4))) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT, "expert_sort: the workspace is smaller than %zu bytes", needed);
     }
-    return submit(context, "expert_sort", [&] {
-        return launch_expert_sort(ids, ids_64 != 0, tokens, choices, experts, offsets, source, position, workspace,
-                                  context->sm_count, context->stream);
-    });
+    return submit(context, "expert_sort", [&] { return launch_expert_sort(d, context->stream); });
 }
 
-qpucuda_status qpucuda_expert_gather(qpucuda_context *context, const void *x, int type, size_t x_stride, uint32_t tokens,
-                                     uint32_t choices, uint32_t width, const int32_t *position, const int32_t *offsets,
-                                     uint32_t experts, void *rows, size_t rows_stride) {
-    if (context == nullptr) return QPUCUDA_INVALID_ARGUMENT;
-    if (tokens == 0) return QPUCUDA_OK;
-    if (!known_type(type) || !routing_fits(tokens, choices, experts) || width == 0 || x == nullptr || position == nullptr ||
-        offsets == nullptr || rows == nullptr || x_stride < width || rows_stride < width || !aligned(x, type_bytes(type)) ||
-        !aligned(rows, type_bytes(type)) || !aligned(position, 4) || !aligned(offsets, 4)) {
+qpucuda_status qpucuda_expert_gather(qpucuda_context *context, const qpucuda_expert_rows_desc *desc) {
+    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    if (desc->tokens == 0) return QPUCUDA_OK;
+    if (!routing_fits(desc->tokens, desc->choices, desc->experts) || !rows_fit(*desc) || !present(desc->offsets)) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT, "expert_gather: invalid pointers, types or extents");
     }
-    return submit(context, "expert_gather", [&] {
-        return launch_expert_gather(x, type, x_stride, tokens, choices, width, position, offsets, experts, rows, rows_stride,
-                                    context->sm_count, context->stream);
-    });
+    return submit(context, "expert_gather", [&] { return launch_expert_gather(*desc, context->sm_count, context->stream); });
 }
 
-qpucuda_status qpucuda_expert_combine(qpucuda_context *context, const void *rows, int type, size_t rows_stride,
-                                      uint32_t tokens, uint32_t choices, uint32_t width, const int32_t *position,
-                                      const float *weights, void *out, size_t out_stride) {
-    if (context == nullptr) return QPUCUDA_INVALID_ARGUMENT;
-    if (tokens == 0) return QPUCUDA_OK;
-    if (!known_type(type) || !routing_fits(tokens, choices, 1) || width == 0 || rows == nullptr || position == nullptr ||
-        out == nullptr || rows_stride < width || out_stride < width || !aligned(rows, type_bytes(type)) ||
-        !aligned(out, type_bytes(type)) || !aligned(position, 4) || !aligned(weights, 4)) {
+qpucuda_status qpucuda_expert_combine(qpucuda_context *context, const qpucuda_expert_rows_desc *desc) {
+    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    if (desc->tokens == 0) return QPUCUDA_OK;
+    if (!routing_fits(desc->tokens, desc->choices, 1) || !rows_fit(*desc) || !aligned(desc->weights, 4)) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT, "expert_combine: invalid pointers, types or extents");
     }
-    return submit(context, "expert_combine", [&] {
-        return launch_expert_combine(rows, type, rows_stride, tokens, choices, width, position, weights, out, out_stride,
-                                     context->sm_count, context->stream);
-    });
+    return submit(context, "expert_combine", [&] { return launch_expert_combine(*desc, context->sm_count, context->stream); });
 }
 
-qpucuda_status qpucuda_expert_combine_backward(qpucuda_context *context, const void *rows, int type, size_t rows_stride,
-                                               const void *grad, size_t grad_stride, uint32_t tokens, uint32_t choices,
-                                               uint32_t width, const int32_t *position, const int32_t *offsets,
-                                               uint32_t experts, const float *weights, void *grad_rows,
-                                               size_t grad_rows_stride, float *grad_weights) {
-    if (context == nullptr) return QPUCUDA_INVALID_ARGUMENT;
-    if (tokens == 0) return QPUCUDA_OK;
-    if (!known_type(type) || !routing_fits(tokens, choices, experts) || width == 0 || rows == nullptr || grad == nullptr ||
-        position == nullptr || offsets == nullptr || weights == nullptr || grad_rows == nullptr || grad_weights == nullptr ||
-        rows_stride < width || grad_stride < width || grad_rows_stride < width || !aligned(rows, type_bytes(type)) ||
-        !aligned(grad, type_bytes(type)) || !aligned(grad_rows, type_bytes(type)) || !aligned(position, 4) ||
-        !aligned(offsets, 4) || !aligned(weights, 4) || !aligned(grad_weights, 4)) {
+qpucuda_status qpucuda_expert_combine_backward(qpucuda_context *context, const qpucuda_expert_rows_desc *desc) {
+    if (context == nullptr || desc == nullptr) return QPUCUDA_INVALID_ARGUMENT;
+    if (desc->tokens == 0) return QPUCUDA_OK;
+    if (!routing_fits(desc->tokens, desc->choices, desc->experts) || !rows_fit(*desc) || !present(desc->offsets) ||
+        !present(desc->weights) || !present(desc->grad_weights) || desc->grad == nullptr || desc->grad_stride < desc->width ||
+        !aligned(desc->grad, type_bytes(desc->type))) {
         return fail(context, QPUCUDA_INVALID_ARGUMENT, "expert_combine_backward: invalid pointers, types or extents");
     }
-    return submit(context, "expert_combine_backward", [&] {
-        return launch_expert_combine_backward(rows, type, rows_stride, grad, grad_stride, tokens, choices, width, position,
-                                              offsets, experts, weights, grad_rows, grad_rows_stride, grad_weights,
-                                              context->sm_count, context->stream);
-    });
+    return submit(context, "expert_combine_backward",
+                  [&] { return launch_expert_combine_backward(*desc, context->sm_count, context->stream); });
 }
 
 }  // extern "C"

@@ -503,38 +503,32 @@ cudaError_t sort_typed(const Id *ids, uint32_t total, uint32_t experts, int32_t 
 }
 
 template <typename T, bool ALIGNED>
-cudaError_t gather_typed(const void *x, size_t x_stride, uint32_t tokens, uint32_t choices, uint32_t width,
-                         const int32_t *position, const int32_t *end, void *rows, size_t rows_stride, int sm_count,
-                         cudaStream_t stream) {
-    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
-    return launch(expert_gather_kernel<T, ALIGNED>, row_blocks(static_cast<uint64_t>(tokens) * packs, sm_count), kRowThreads,
-                  0, 1, stream, static_cast<const T *>(x), x_stride, tokens, choices, width, packs, position, end,
-                  static_cast<T *>(rows), rows_stride);
+cudaError_t gather_typed(const qpucuda_expert_rows_desc &d, int sm_count, cudaStream_t stream) {
+    const uint32_t packs = Columns<T, ALIGNED>::packs(d.width);
+    return launch(expert_gather_kernel<T, ALIGNED>, row_blocks(static_cast<uint64_t>(d.tokens) * packs, sm_count), kRowThreads,
+                  0, 1, stream, static_cast<const T *>(d.source), d.source_stride, d.tokens, d.choices, d.width, packs,
+                  d.position, d.offsets + d.experts, static_cast<T *>(d.out), d.out_stride);
 }
 
 template <typename T, bool ALIGNED>
-cudaError_t combine_typed(const void *rows, size_t rows_stride, uint32_t tokens, uint32_t choices, uint32_t width,
-                          const int32_t *position, const float *weights, void *out, size_t out_stride, int sm_count,
-                          cudaStream_t stream) {
-    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
-    const uint32_t blocks = row_blocks(static_cast<uint64_t>(tokens) * packs, sm_count);
-    auto kernel = weights != nullptr ? expert_combine_kernel<T, ALIGNED, true> : expert_combine_kernel<T, ALIGNED, false>;
-    return launch(kernel, blocks, kRowThreads, 0, 1, stream, static_cast<const T *>(rows), rows_stride, tokens, choices,
-                  width, packs, position, weights, static_cast<T *>(out), out_stride);
+cudaError_t combine_typed(const qpucuda_expert_rows_desc &d, int sm_count, cudaStream_t stream) {
+    const uint32_t packs = Columns<T, ALIGNED>::packs(d.width);
+    const uint32_t blocks = row_blocks(static_cast<uint64_t>(d.tokens) * packs, sm_count);
+    auto kernel = d.weights != nullptr ? expert_combine_kernel<T, ALIGNED, true> : expert_combine_kernel<T, ALIGNED, false>;
+    return launch(kernel, blocks, kRowThreads, 0, 1, stream, static_cast<const T *>(d.source), d.source_stride, d.tokens,
+                  d.choices, d.width, packs, d.position, d.weights, static_cast<T *>(d.out), d.out_stride);
 }
 
 template <typename T, bool ALIGNED>
-cudaError_t combine_backward_typed(const void *rows, size_t rows_stride, const void *grad, size_t grad_stride,
-                                   uint32_t tokens, uint32_t choices, uint32_t width, const int32_t *position,
-                                   const int32_t *end, const float *weights, void *grad_rows, size_t grad_rows_stride,
-                                   float *grad_weights, int sm_count, cudaStream_t stream) {
-    const uint32_t packs = Columns<T, ALIGNED>::packs(width);
+cudaError_t combine_backward_typed(const qpucuda_expert_rows_desc &d, int sm_count, cudaStream_t stream) {
+    const uint32_t packs = Columns<T, ALIGNED>::packs(d.width);
     uint32_t threads = 32;
     while (threads < kRowThreads && threads < packs) threads *= 2;
     const uint32_t most = static_cast<uint32_t>(sm_count) * 64u;
-    return launch(expert_combine_backward_kernel<T, ALIGNED>, tokens < most ? tokens : most, threads, 0, 1, stream,
-                  static_cast<const T *>(rows), rows_stride, static_cast<const T *>(grad), grad_stride, tokens, choices,
-                  width, packs, position, end, weights, static_cast<T *>(grad_rows), grad_rows_stride, grad_weights);
+    return launch(expert_combine_backward_kernel<T, ALIGNED>, d.tokens < most ? d.tokens : most, threads, 0, 1, stream,
+                  static_cast<const T *>(d.source), d.source_stride, static_cast<const T *>(d.grad), d.grad_stride, d.tokens,
+                  d.choices, d.width, packs, d.position, d.offsets + d.experts, d.weights, static_cast<T *>(d.out), d.out_stride,
+                  d.grad_weights);
 }
 
 // Calls f<T, ALIGNED>(...) for the element type.
@@ -549,6 +543,12 @@ cudaError_t combine_backward_typed(const void *rows, size_t rows_stride, const v
 
 size_t item_bytes(int type) { return type == QPUCUDA_DTYPE_F32 ? 4 : 2; }
 
+bool vector_moves(const qpucuda_expert_rows_desc &desc) {
+    const size_t item = item_bytes(desc.type);
+    return desc.width * item % 16u == 0 && vector_rows(desc.source, desc.source_stride, item) &&
+           vector_rows(desc.out, desc.out_stride, item);
+}
+
 }  // namespace
 
 size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts) {
@@ -559,45 +559,25 @@ size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts
     return static_cast<size_t>((total + chunk - 1) / chunk) * experts * sizeof(int32_t);
 }
 
-cudaError_t launch_expert_sort(const void *ids, bool ids_64, uint32_t tokens, uint32_t choices, uint32_t experts,
-                               int32_t *offsets, int32_t *source, int32_t *position, void *workspace, int sm_count,
-                               cudaStream_t stream) {
-    (void)sm_count;
-    const uint32_t total = tokens * choices;
-    int32_t *counts = static_cast<int32_t *>(workspace);
-    return ids_64 ? sort_typed(static_cast<const long long *>(ids), total, experts, offsets, source, position, counts, stream)
-                  : sort_typed(static_cast<const int32_t *>(ids), total, experts, offsets, source, position, counts, stream);
+cudaError_t launch_expert_sort(const qpucuda_expert_sort_desc &d, cudaStream_t stream) {
+    const uint32_t total = d.tokens * d.choices;
+    int32_t *counts = static_cast<int32_t *>(d.workspace);
+    return d.ids_64 != 0
+               ? sort_typed(static_cast<const long long *>(d.ids), total, d.experts, d.offsets, d.source, d.position, counts, stream)
+               : sort_typed(static_cast<const int32_t *>(d.ids), total, d.experts, d.offsets, d.source, d.position, counts, stream);
 }
 
-cudaError_t launch_expert_gather(const void *x, int type, size_t x_stride, uint32_t tokens, uint32_t choices,
-                                 uint32_t width, const int32_t *position, const int32_t *offsets, uint32_t experts,
-                                 void *rows, size_t rows_stride, int sm_count, cudaStream_t stream) {
-    const size_t item = item_bytes(type);
-    const bool aligned = width * item % 16u == 0 && vector_rows(x, x_stride, item) && vector_rows(rows, rows_stride, item);
-    QPUCUDA_ROWS_DISPATCH(gather_typed, type, aligned, x, x_stride, tokens, choices, width, position, offsets + experts,
-                          rows, rows_stride, sm_count, stream);
+cudaError_t launch_expert_gather(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream) {
+    QPUCUDA_ROWS_DISPATCH(gather_typed, desc.type, vector_moves(desc), desc, sm_count, stream);
 }
 
-cudaError_t launch_expert_combine(const void *rows, int type, size_t rows_stride, uint32_t tokens, uint32_t choices,
-                                  uint32_t width, const int32_t *position, const float *weights, void *out,
-                                  size_t out_stride, int sm_count, cudaStream_t stream) {
-    const size_t item = item_bytes(type);
-    const bool aligned = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) && vector_rows(out, out_stride, item);
-    QPUCUDA_ROWS_DISPATCH(combine_typed, type, aligned, rows, rows_stride, tokens, choices, width, position, weights, out,
-                          out_stride, sm_count, stream);
+cudaError_t launch_expert_combine(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream) {
+    QPUCUDA_ROWS_DISPATCH(combine_typed, desc.type, vector_moves(desc), desc, sm_count, stream);
 }
 
-cudaError_t launch_expert_combine_backward(const void *rows, int type, size_t rows_stride, const void *grad,
-                                           size_t grad_stride, uint32_t tokens, uint32_t choices, uint32_t width,
-                                           const int32_t *position, const int32_t *offsets, uint32_t experts,
-                                           const float *weights, void *grad_rows, size_t grad_rows_stride,
-                                           float *grad_weights, int sm_count, cudaStream_t stream) {
-    const size_t item = item_bytes(type);
-    const bool aligned = width * item % 16u == 0 && vector_rows(rows, rows_stride, item) &&
-                        vector_rows(grad, grad_stride, item) && vector_rows(grad_rows, grad_rows_stride, item);
-    QPUCUDA_ROWS_DISPATCH(combine_backward_typed, type, aligned, rows, rows_stride, grad, grad_stride, tokens, choices,
-                          width, position, offsets + experts, weights, grad_rows, grad_rows_stride, grad_weights,
-                          sm_count, stream);
+cudaError_t launch_expert_combine_backward(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream) {
+    const bool aligned = vector_moves(desc) && vector_rows(desc.grad, desc.grad_stride, item_bytes(desc.type));
+    QPUCUDA_ROWS_DISPATCH(combine_backward_typed, desc.type, aligned, desc, sm_count, stream);
 }
 
 }  // namespace qpucuda

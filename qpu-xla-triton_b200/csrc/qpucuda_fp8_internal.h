@@ -23,19 +23,9 @@ cudaError_t launch_fp8_linear(const qpucuda_fp8_quantize_desc &quantize, const q
                               int sm_count, cudaStream_t stream);
 
 size_t expert_sort_workspace(uint32_t tokens, uint32_t choices, uint32_t experts);
-cudaError_t launch_expert_sort(const void *ids, bool ids_64, uint32_t tokens, uint32_t choices, uint32_t experts,
-                               int32_t *offsets, int32_t *source, int32_t *position, void *workspace, int sm_count,
-                               cudaStream_t stream);
-cudaError_t launch_expert_gather(const void *x, int type, size_t x_stride, uint32_t tokens, uint32_t choices,
-                                 uint32_t width, const int32_t *position, const int32_t *offsets, uint32_t experts,
-                                 void *rows, size_t rows_stride, int sm_count, cudaStream_t stream);
-cudaError_t launch_expert_combine(const void *rows, int type, size_t rows_stride, uint32_t tokens, uint32_t choices,
-                                  uint32_t width, const int32_t *position, const float *weights, void *out,
-                                  size_t out_stride, int sm_count, cudaStream_t stream);
-cudaError_t launch_expert_combine_backward(const void *rows, int type, size_t rows_stride, const void *grad,
-                                           size_t grad_stride, uint32_t tokens, uint32_t choices, uint32_t width,
-                                           const int32_t *position, const int32_t *offsets, uint32_t experts,
-                                           const float *weights, void *grad_rows, size_t grad_rows_stride,
-                                           float *grad_weights, int sm_count, cudaStream_t stream);
+cudaError_t launch_expert_sort(const qpucuda_expert_sort_desc &desc, cudaStream_t stream);
+cudaError_t launch_expert_gather(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream);
+cudaError_t launch_expert_combine(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream);
+cudaError_t launch_expert_combine_backward(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream);
 
 }  // namespace qpucuda

@@ -149,11 +149,10 @@ class CudaBackend:
         if self._closed:
             raise DeviceClosedError("backend is closed")
         native = self.native
-        library, handle = native.library, native.handle
         with self.launch_lock:
-            status = library.qpucuda_context_set_stream(handle, stream or None)
-            if status == 0:
-                status = getattr(library, name)(handle, *args)
+            if native.stream != stream:
+                native.set_stream(stream)
+            status = getattr(native.library, name)(native.handle, *args)
             if status != 0:
                 native.check(status, name)
 

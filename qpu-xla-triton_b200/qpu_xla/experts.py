@@ -16,10 +16,12 @@ gradients are recorded (inside an ``autograd.Function`` they are not).
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Any, Self
 
 import torch
 
+from qpu_xla import _native
 from qpu_xla.device import Device
 from qpu_xla.fp8 import (
     MAX_EXPERTS,
@@ -33,6 +35,15 @@ from qpu_xla.fp8 import (
     new_matrix,
     require_cuda,
 )
+
+
+_pack_sort = _native.packer(_native.ExpertSortDesc)
+_pack_rows = _native.packer(_native.ExpertRowsDesc)
+
+
+@lru_cache(maxsize=256)
+def _sort_workspace(tokens: int, choices: int, experts: int) -> int:
+    return int(_native.load().qpucuda_expert_sort_workspace(tokens, choices, experts))
 
 
 @dataclass(frozen=True, slots=True)
@@ -98,12 +109,13 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     offsets, source, position = torch.empty(experts + 1 + 2 * total, dtype=torch.int32, device=torch_device).split_with_sizes(
         [experts + 1, total, total]
     )
-    needed = device.backend.native.library.qpucuda_expert_sort_workspace(tokens, choices, experts)  # type: ignore[attr-defined]
+    needed = _sort_workspace(tokens, choices, experts)
     workspace = torch.empty(needed, dtype=torch.uint8, device=torch_device) if needed else None
-    launch(
-        device, "qpucuda_expert_sort", ids.data_ptr(), ids.dtype == torch.int64, tokens, choices, experts, offsets.data_ptr(),
-        source.data_ptr(), position.data_ptr(), None if workspace is None else workspace.data_ptr(), needed,
+    desc = _pack_sort(
+        ids.data_ptr(), ids.dtype == torch.int64, tokens, choices, experts, offsets.data_ptr(), source.data_ptr(), position.data_ptr(),
+        0 if workspace is None else workspace.data_ptr(), needed,
     )
+    launch(device, "qpucuda_expert_sort", desc)
     return made(ExpertOrder, offsets=offsets, source=source, position=position.view(tokens, choices))
 
 
@@ -128,10 +140,11 @@ def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = No
     _, width, stride = check_matrix(source, torch_device, "gather_tokens source", tokens)
     out, out_stride = _destination(out, tokens * choices, width, source, torch_device, "gather_tokens out")
     if tokens and width:
-        launch(
-            device, "qpucuda_expert_gather", source.data_ptr(), code, stride, tokens, choices, width, order.position.data_ptr(),
-            order.offsets.data_ptr(), order.experts, out.data_ptr(), out_stride,
+        desc = _pack_rows(
+            code, tokens, choices, width, order.experts, order.position.data_ptr(), order.offsets.data_ptr(), 0, source.data_ptr(), stride,
+            0, 0, 0, out.data_ptr(), out_stride,
         )
+        launch(device, "qpucuda_expert_gather", desc)
     return out
 
 
@@ -142,10 +155,11 @@ def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: A
     _, width, stride = check_matrix(rows, torch_device, name, tokens * choices)
     out, out_stride = _destination(out, tokens, width, rows, torch_device, name)
     if tokens and width:
-        launch(
-            device, "qpucuda_expert_combine", rows.data_ptr(), code, stride, tokens, choices, width, order.position.data_ptr(),
-            None if weights is None else weights.data_ptr(), out.data_ptr(), out_stride,
+        desc = _pack_rows(
+            code, tokens, choices, width, order.experts, order.position.data_ptr(), 0, 0 if weights is None else weights.data_ptr(),
+            rows.data_ptr(), stride, 0, 0, 0, out.data_ptr(), out_stride,
         )
+        launch(device, "qpucuda_expert_combine", desc)
     return out
 
 
@@ -190,11 +204,11 @@ def combine_tokens_backward(device: Device, rows: Any, weights: Any, grad: Any, 
     grad_rows = new_matrix(tokens * choices, width, rows.dtype, torch_device)
     grad_weights = new_matrix(tokens, choices, torch.float32, torch_device)
     if tokens and width:
-        launch(
-            device, "qpucuda_expert_combine_backward", rows.data_ptr(), code, stride, grad.data_ptr(), grad_stride, tokens, choices, width,
-            order.position.data_ptr(), order.offsets.data_ptr(), order.experts, weights.data_ptr(), grad_rows.data_ptr(), width,
-            grad_weights.data_ptr(),
+        desc = _pack_rows(
+            code, tokens, choices, width, order.experts, order.position.data_ptr(), order.offsets.data_ptr(), weights.data_ptr(),
+            rows.data_ptr(), stride, grad.data_ptr(), grad_stride, grad_weights.data_ptr(), grad_rows.data_ptr(), width,
         )
+        launch(device, "qpucuda_expert_combine_backward", desc)
     else:
         grad_weights.zero_()
     return grad_rows, grad_weights

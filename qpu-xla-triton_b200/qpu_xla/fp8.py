@@ -18,7 +18,6 @@ source that requires grad is refused while gradients are recorded.
 
 from __future__ import annotations
 
-import ctypes
 from collections.abc import Iterable
 from dataclasses import dataclass
 from typing import Any, Self
@@ -37,6 +36,8 @@ FP8_GROUP = 128
 MAX_EXPERTS = 1024
 
 
+_pack_quantize = _native.packer(_native.Fp8QuantizeDesc)
+_pack_gemm = _native.packer(_native.Fp8GemmDesc)
 _DTYPE_CODES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 
 
@@ -70,6 +71,8 @@ def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = N
     if tensor.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires grad, and there is no autograd here: call under torch.no_grad() or from an autograd.Function")
     have_rows, have_cols = shape
+    if have_rows >= 2**31 or have_cols >= 2**31:
+        raise ValueError(f"{what} must have fewer than 2**31 rows and columns")
     stride, inner = tensor.stride()
     if inner != 1 and have_cols > 1:
         raise ValueError(f"{what} must be row-major (unit inner stride)")
@@ -193,16 +196,6 @@ def quantize_blocks_fp8(device: Device, weight: Any) -> QuantizedBlocksFP8:
     return QuantizedBlocksFP8(values, scales)
 
 
-def _quantize_desc(
-    source: Any, stride: int, cols: int, gated: bool, rows: int, q: int, q_stride: int, scales: int, scale_strides: tuple[int, int],
-    row_source: Any = None, row_divisor: int = 1,
-) -> Any:
-    return _native.Fp8QuantizeDesc(
-        source.data_ptr(), dtype_code(source.dtype, "quantizer source"), stride, rows, cols, int(gated),
-        None if row_source is None else row_source.data_ptr(), row_divisor, source.shape[0], q, q_stride, scales, *scale_strides,
-    )
-
-
 def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> QuantizedRowsFP8:
     """Quantize rows ``[M, K]`` (float32, bfloat16 or float16) with one scale per 128 columns.
 
@@ -210,7 +203,7 @@ def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> Qu
     computed in fp32. The values are a view of rows padded to 16 bytes.
     """
     torch_device = require_cuda(device, "quantize_rows_fp8")
-    dtype_code(source.dtype, "quantize_rows_fp8 source")
+    code = dtype_code(source.dtype, "quantize_rows_fp8 source")
     rows, cols, stride = check_matrix(source, torch_device, "quantize_rows_fp8 source")
     if cols == 0 or (gated and cols % 2):
         raise ValueError("quantize_rows_fp8 source must have columns, an even number of them when gated")
@@ -219,8 +212,11 @@ def quantize_rows_fp8(device: Device, source: Any, *, gated: bool = False) -> Qu
     values = new_matrix(rows, q_stride, torch.float8_e4m3fn, torch_device)
     scales = new_matrix(rows, groups_of(cols), torch.float32, torch_device)
     if rows:
-        desc = _quantize_desc(source, stride, cols, gated, rows, values.data_ptr(), q_stride, scales.data_ptr(), (groups_of(cols), 1))
-        launch(device, "qpucuda_fp8_quantize_rows", ctypes.byref(desc))
+        desc = _pack_quantize(
+            source.data_ptr(), code, stride, rows, cols, bool(gated), 0, 1, rows, values.data_ptr(), q_stride, scales.data_ptr(),
+            groups_of(cols), 1,
+        )
+        launch(device, "qpucuda_fp8_quantize_rows", desc)
     return made(QuantizedRowsFP8, values=values if q_stride == cols else values[:, :cols], scales=scales)
 
 
@@ -252,7 +248,7 @@ class _PreparedFP8:
             self._bias = bias.to(self._torch_device, torch.float32).clone(memory_format=torch.contiguous_format)
         self._values_address = self._values.data_ptr()
         self._scales_address = self._scales.data_ptr()
-        self._bias_address = None if self._bias is None else self._bias.data_ptr()
+        self._bias_address = 0 if self._bias is None else self._bias.data_ptr()
         torch.cuda.current_stream(self._torch_device).synchronize()
         self._pending: list[Event] = []  # executions on queues that may not have been launched yet
         self._closed = False
@@ -300,16 +296,16 @@ class _PreparedFP8:
 
     def _gemm_desc(
         self: Self, a: int, a_stride: int, a_scales: int, scale_strides: tuple[int, int], rows: int, out_address: int, out_code: int,
-        out_stride: int, offsets: int | None = None, settled: bool = False,
-    ) -> Any:
-        return _native.Fp8GemmDesc(
+        out_stride: int, offsets: int = 0, settled: bool = False,
+    ) -> bytes:
+        return _pack_gemm(
             a, a_stride, a_scales, *scale_strides, self._values_address, self._padded, self._scales_address, self._bias_address, rows,
             self.output_count, self.input_count, self.experts, offsets, out_address, out_code, out_stride, settled,
         )
 
     def _linear(
         self: Self, source: int, source_code: int, source_rows: int, stride: int, rows: int, out: int, out_code: int, out_stride: int,
-        offsets: int | None = None, row_source: int | None = None, row_divisor: int = 1, stream: int | None = None,
+        offsets: int = 0, row_source: int = 0, row_divisor: int = 1, stream: int | None = None,
     ) -> None:
         """Quantize and multiply. One scratch allocation, for this call alone: the quantized rows and,
         behind them, their scales, group-major (a warp of the product reads neighbouring rows' scales).
@@ -319,11 +315,11 @@ class _PreparedFP8:
         scratch = new_matrix(rows, padded + 4 * self._groups, torch.uint8, self._torch_device)
         values = scratch.data_ptr()
         scales = values + rows * padded
-        quantize = _native.Fp8QuantizeDesc(
+        quantize = _pack_quantize(
             source, source_code, stride, rows, self.input_count, self.gated, row_source, row_divisor, source_rows, values, padded, scales, 1, rows
         )
         gemm = self._gemm_desc(values, padded, scales, (1, rows), rows, out, out_code, out_stride, offsets, True)
-        launch(self.device, "qpucuda_fp8_linear", ctypes.byref(quantize), ctypes.byref(gemm), stream=stream)
+        launch(self.device, "qpucuda_fp8_linear", quantize, gemm, stream=stream)
 
     def _check_source(self: Self, source: Any) -> tuple[int, int, int]:
         """Rows, row stride and type code."""
@@ -373,7 +369,7 @@ class PreparedFP8Linear(_PreparedFP8):
             gemm = self._gemm_desc(
                 rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride
             )
-            launch(self.device, "qpucuda_fp8_gemm", ctypes.byref(gemm))
+            launch(self.device, "qpucuda_fp8_gemm", gemm)
         return out
 
     def execute(self: Self, destination: Tensor, source: Tensor, *, queue: Queue, wait_for: Iterable[Event] = ()) -> Event:

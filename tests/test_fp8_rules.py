@@ -15,6 +15,7 @@ from qpu_xla.fp8 import (
     QuantizedBlocksFP8,
     QuantizedRowsFP8,
     check_apart,
+    check_matrix,
     quantize_blocks_fp8,
     quantize_rows_fp8,
 )
@@ -94,10 +95,10 @@ def test_null_arguments_are_rejected_without_a_device() -> None:
     assert library.qpucuda_fp8_quantize_rows(None, ctypes.byref(_native.Fp8QuantizeDesc())) == _native.Status.INVALID_ARGUMENT
     assert library.qpucuda_fp8_gemm(None, ctypes.byref(_native.Fp8GemmDesc())) == _native.Status.INVALID_ARGUMENT
     assert library.qpucuda_fp8_quantize_blocks(None, None, 0, 0, 0, 0, 0, None, 0, None) == _native.Status.INVALID_ARGUMENT
-    assert library.qpucuda_expert_sort(None, None, 0, 0, 0, 0, None, None, None, None, 0) == _native.Status.INVALID_ARGUMENT
-    assert library.qpucuda_expert_gather(None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0) == _native.Status.INVALID_ARGUMENT
-    assert library.qpucuda_expert_combine(None, None, 0, 0, 0, 0, 0, None, None, None, 0) == _native.Status.INVALID_ARGUMENT
-    assert library.qpucuda_expert_combine_backward(None, None, 0, 0, None, 0, 0, 0, 0, None, None, 0, None, None, 0, None) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_sort(None, ctypes.byref(_native.ExpertSortDesc())) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_gather(None, ctypes.byref(_native.ExpertRowsDesc())) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_combine(None, ctypes.byref(_native.ExpertRowsDesc())) == _native.Status.INVALID_ARGUMENT
+    assert library.qpucuda_expert_combine_backward(None, ctypes.byref(_native.ExpertRowsDesc())) == _native.Status.INVALID_ARGUMENT
 
 
 def test_sort_workspace_is_only_needed_past_one_cluster() -> None:
@@ -106,6 +107,20 @@ def test_sort_workspace_is_only_needed_past_one_cluster() -> None:
     assert size(4097, 8, 64) > 0 and size(4097, 8, 64) % (4 * 64) == 0
     assert size(0, 8, 64) == 0 and size(8, 0, 64) == 0 and size(8, 8, 1025) == 0
     assert size(2**31, 2, 4) == 0
+
+
+@pytest.mark.parametrize("structure", [_native.Fp8QuantizeDesc, _native.Fp8GemmDesc, _native.ExpertSortDesc, _native.ExpertRowsDesc])
+def test_packed_descriptions_are_the_structures(structure) -> None:
+    values = [i + 1 for i in range(len(structure._fields_))]
+    assert _native.packer(structure)(*values) == bytes(structure(*values))
+
+
+def test_matrices_have_31_bit_extents() -> None:
+    meta = torch.device("meta")
+    for shape in ((2**31, 1), (1, 2**31)):
+        with pytest.raises(ValueError, match="2\\*\\*31"):
+            check_matrix(torch.empty(shape, device=meta), meta, "x")
+    assert check_matrix(torch.empty((2**31 - 1, 2), device=meta), meta, "x") == (2**31 - 1, 2, 2)
 
 
 def meets_by_bytes(one: torch.Tensor, other: torch.Tensor) -> bool:
