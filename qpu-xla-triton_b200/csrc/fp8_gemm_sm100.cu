@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t split = cluster_size();
+    const uint32_t split = cluster_size();  // a power of two
+    const uint32_t split_shift = __ffs(static_cast<int>(split)) - 1;
     const uint32_t rank = cluster_rank();
     const uint32_t n_block = blockIdx.x / split;
     const uint32_t n0 = n_block * kBlockN;
@@ -441,13 +442,18 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
         }
         const uint32_t column = quarter * 32u + lane;  // output column inside the block
         if (split > 1) {
-            // Every MMA of this CTA has completed, so its stages are free: partial[row][column].
-            float *partial = reinterpret_cast<float *>(smem);
+            // The tile's rows in turn over the ranks: each row's sums go to its rank's stages, which are
+            // free once the MMAs of the whole cluster have completed, as [rank][row / split][column].
+            __syncwarp();
+            cluster_sync();
+            const uint32_t rows = tile.row_end - tile.row0;
+            const uint32_t mine = smem_u32(smem) + ((rank * NT >> split_shift) * kBlockN + column) * 4u;
 #pragma unroll
-            for (int i = 0; i < kColumns / 2; ++i) {
-                partial[(2 * i) * kBlockN + column] = low(acc[i]);
-                partial[(2 * i + 1) * kBlockN + column] = high(acc[i]);
+            for (uint32_t i = 0; i < kColumns; ++i) {
+                const float v = (i & 1u) ? high(acc[i / 2]) : low(acc[i / 2]);
+                if (i < rows) store_cluster(map_to_rank(mine + (i >> split_shift) * (kBlockN * 4u), i & (split - 1u)), v);
             }
+            __syncwarp();
         } else if (ok && n0 + column < params.n) {
             const float bias = params.bias != nullptr ? __ldg(params.bias + n0 + column) : 0.0f;
             Out *out = static_cast<Out *>(params.out) + static_cast<size_t>(tile.row0) * params.out_stride + n0 + column;
@@ -461,18 +467,19 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     }
     if (split > 1) {
         __syncwarp();
-        cluster_sync();  // every CTA's partial sums are in place
+        if (warp < 2 || !tile.valid) cluster_sync();
+        cluster_sync();  // every rank's sums are in place; no CTA touches another's memory from here on
         if (tile.valid && warp >= 2) {
             const uint32_t rows = tile.row_end - tile.row0;
-            const float *partial = reinterpret_cast<const float *>(smem);
-            // the tile's rows in turn over the ranks, 128 columns across
-            const uint32_t column = threadIdx.x - 64u;
+            const float *sums = reinterpret_cast<const float *>(smem);
+            const uint32_t column = threadIdx.x - 64u;  // 128 across
             const bool inside = n0 + column < params.n;
             const float bias = params.bias != nullptr && inside ? __ldg(params.bias + n0 + column) : 0.0f;
             for (uint32_t row = rank; row < rows; row += split) {
-                const uint32_t address = smem_u32(partial + row * kBlockN + column);
                 float sum = 0.0f;
-                for (uint32_t r = 0; r < split; ++r) sum += load_cluster(map_to_rank(address, r));
+#pragma unroll
+                for (uint32_t r = 0; r < kMaxSplit; ++r)
+                    if (r < split) sum += sums[((r * NT >> split_shift) + (row >> split_shift)) * kBlockN + column];
                 if (inside)
                     static_cast<Out *>(params.out)[static_cast<size_t>(tile.row0 + row) * params.out_stride + n0 + column] =
                         from_float<Out>(sum + bias);
@@ -487,7 +494,6 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     }
     tc_fence_before();
     __syncthreads();
-    if (split > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Shape::kTmemColumns)
@@ -732,7 +738,9 @@ __device__ __forceinline__ void store_box(uint8_t *buffer, const float (&v)[128 
 //   warp 2   the experts' table of tiles, warp 3 nothing
 //   4 to 11  each block's accumulator into registers, scaled; at the tile's end the store
 // SPLIT: few tiles. The CTAs of a cluster share one tile's K blocks and add their sums, in slice
-// order, through distributed shared memory; each CTA has one tile.
+// order, through distributed shared memory; each CTA has one tile. The sums are pushed to the CTA that
+// adds them: 96 KB leave each of four CTAs in 2.9 us, 16 bytes a cycle, and take 5.6 to be read from
+// the other side.
 template <typename Out, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1)
     fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
@@ -876,7 +884,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         }
         __syncwarp();
-        if constexpr (SPLIT) cluster_sync();
+        if constexpr (SPLIT) {
+            cluster_sync();
+            cluster_sync();
+        }
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
         if (lane == 0 && rank == 0) {
@@ -928,10 +939,16 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         }
         __syncwarp();
-        if constexpr (SPLIT) cluster_sync();
+        if constexpr (SPLIT) {
+            cluster_sync();
+            cluster_sync();
+        }
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideFewRegisters));
-        if constexpr (SPLIT) cluster_sync();
+        if constexpr (SPLIT) {
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideManyRegisters));
         const uint32_t worker = warp - 4u;
@@ -944,6 +961,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         // released on the barrier of the CTA that issues the MMAs
         const uint32_t tmem_empty0 = PAIR ? map_to_rank(smem_u32(&control->tmem_empty[0]), 0) : smem_u32(&control->tmem_empty[0]);
         uint32_t buffer = 0, buffer_phase = 0;
+        const uint32_t part_shift = slices == 2 ? 4u : 3u;  // SPLIT: log2 of the float4 columns of a CTA's part of a half
+        bool summed = false;
         for (uint32_t t = tile_first; t < total; t += tile_step) {
             const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, t);
             const uint32_t n0 = tile.n0 + half * (kWideN / 2);
@@ -1022,12 +1041,23 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
             if (!ok) break;
             if constexpr (SPLIT) {
-                // The only tile of this CTA, and its MMAs are complete: the stages hold the partial
-                // sums, [column / 4][row] float4, which the cluster's CTAs add up below.
-                float4 *partial = reinterpret_cast<float4 *>(smem) + half * (kWideN / 8) * kWideM + quarter * 32u + lane;
+                // The only tile of this CTA. Each of the cluster's CTAs adds up its share of the columns, a
+                // part of both halves: the sums go to the stages of the CTA they belong to, free once the
+                // cluster's MMAs have completed, as [slice][half][column / 4][row] float4.
+                __syncwarp();
+                cluster_sync();
+                if (row0 < tile.row_end) {
+                    const uint32_t mine = smem_u32(smem) + ((((slice * 2u + half) << part_shift) * kWideM) + quarter * 32u + lane) * 16u;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    partial[i * kWideM] = make_float4(low(acc[2 * i]), high(acc[2 * i]), low(acc[2 * i + 1]), high(acc[2 * i + 1]));
+                    for (uint32_t i = 0; i < 32; ++i) {
+                        const uint32_t owner = i >> part_shift, place = i - (owner << part_shift);
+                        store_cluster4(map_to_rank(mine + place * (kWideM * 16u), owner),
+                                       make_float4(low(acc[2 * i]), high(acc[2 * i]), low(acc[2 * i + 1]), high(acc[2 * i + 1])));
+                    }
+                }
+                __syncwarp();
+                cluster_sync();
+                summed = true;
                 continue;
             }
             if (row0 >= tile.row_end || !block_inside) continue;
@@ -1054,32 +1084,32 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         }
         if constexpr (SPLIT) {
-            __syncwarp();
-            cluster_sync();  // every slice's partial sums are in place
-            if (tile_first < total) {
-                // This CTA's share of the columns, summed in slice order: 256 / slices of them, half to
-                // each four warps, a row to a thread.
+            if (!summed) {  // no tile, or given up
+                __syncwarp();
+                cluster_sync();
+                cluster_sync();
+            } else {
                 const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, tile_first);
-                constexpr int kChunk = 64 / static_cast<int>(sizeof(Out));
+                constexpr uint32_t kChunk = 64 / sizeof(Out);
                 const uint32_t row0 = tile.row0 + quarter * 32u;
-                const uint32_t columns = kWideN / slices / 2u;
-                const uint32_t column0 = slice * (kWideN / slices) + half * columns;
+                const uint32_t columns = 4u << part_shift;
+                const uint32_t n0 = tile.n0 + half * (kWideN / 2) + slice * columns;
                 if (row0 < tile.row_end) {
-                    for (uint32_t c = column0; c < column0 + columns && tile.n0 + c < params.n; c += kChunk) {
-                        const uint32_t address = smem_u32(smem) + ((c / 4u) * kWideM + quarter * 32u + lane) * 16u;
+                    for (uint32_t c = 0; c < columns && n0 + c < params.n; c += kChunk) {
+                        const float4 *part = reinterpret_cast<const float4 *>(smem) +
+                                             ((half << part_shift) + c / 4u) * kWideM + quarter * 32u + lane;
                         float v[kChunk] = {};
-                        for (uint32_t r = 0; r < slices; ++r) {
-                            const uint32_t remote = map_to_rank(address, r);
+                        for (uint32_t r = 0; r < slices; ++r, part += (2u << part_shift) * kWideM) {
 #pragma unroll
-                            for (int i = 0; i < kChunk / 4; ++i) {
-                                const float4 part = load_cluster4(remote + i * kWideM * 16u);
-                                v[4 * i] += part.x;
-                                v[4 * i + 1] += part.y;
-                                v[4 * i + 2] += part.z;
-                                v[4 * i + 3] += part.w;
+                            for (uint32_t i = 0; i < kChunk / 4; ++i) {
+                                const float4 term = part[i * kWideM];
+                                v[4 * i] += term.x;
+                                v[4 * i + 1] += term.y;
+                                v[4 * i + 2] += term.z;
+                                v[4 * i + 3] += term.w;
                             }
                         }
-                        const uint32_t n = tile.n0 + c;
+                        const uint32_t n = n0 + c;
                         add_bias(params, n, v);
                         store_chunk<Out>(reinterpret_cast<uint4 *>(buffer_out), v, static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n,
                                          params.out_stride, tile.row_end - row0, params.n - n, vector, lane);
@@ -1099,8 +1129,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    // No slice leaves while another reads its sums.
-    if constexpr (SPLIT) cluster_sync();
     // Neither CTA of a pair leaves while the other may still signal its barriers, read its shared
     // memory or write its tensor memory.
     if constexpr (PAIR) cluster_sync();
@@ -1196,16 +1224,6 @@ cudaError_t launch_wide_type(const CUtensorMap &map_w, const CUtensorMap &map_a,
 // rows each (4096 tokens, 4 of 32, 5632 x 2048) took 303 us in pairs and 292 alone, 1024 rows 525 and 534.
 constexpr uint64_t kPairShare = 1024;
 
-// Many rows per matrix, or weights that fill the SMs with wide tiles already: the wide kernel's deeper
-// copies then stream them at least as fast. One matrix of 11008 x 4096: 65 rows 17 us wide, 64 rows 19
-// us narrow, 24 rows 15 us narrow and 20 wide; of 2048 x 2048: 64 rows 9 us narrow, 65 rows 11 us wide.
-// 32 experts of 5632 x 2048 with 8 rows each: 70 us wide, 73 narrow; with 32 rows 77 against 104.
-bool use_wide(uint64_t share, uint64_t matrices, uint64_t n_tiles, uint64_t sms) {
-    if (share > 64) return true;
-    if (matrices > 1) return share > 4 && matrices * n_tiles * 4 >= sms * 3;
-    return share > 32 && n_tiles >= 16;
-}
-
 GemmParams gemm_params(const qpucuda_fp8_gemm_desc &desc, unsigned int *error_word) {
     GemmParams params{};
     params.rows = desc.rows;
@@ -1245,6 +1263,45 @@ NarrowLaunch plan_narrow(const qpucuda_fp8_gemm_desc &desc, const GemmParams &pa
     return launch;
 }
 
+WideLaunch plan_wide(const qpucuda_fp8_gemm_desc &desc, const GemmParams &params, uint64_t share, uint64_t filled, uint64_t sms) {
+    WideLaunch launch{};
+    launch.n_tiles = (desc.n + kWideN - 1) / kWideN;
+    // Pairs where tiles of 256 rows hold hardly more padding than tiles of 128.
+    const uint64_t single_tiles = most_tiles(desc, filled, kWideM), pair_tiles = most_tiles(desc, filled, 2 * kWideM);
+    launch.pair = sms >= 2 && (desc.experts != 0 ? share >= kPairShare : pair_tiles * 2 * 12 <= single_tiles * 13);
+    launch.split = 1;
+    if ((launch.pair ? pair_tiles : single_tiles) * launch.n_tiles * 2 <= sms) {
+        launch.pair = false;
+        while (launch.split < 4 && single_tiles * launch.n_tiles * launch.split * 2 <= sms && params.k_blocks >= 16) launch.split *= 2;
+    }
+    launch.tiles = (launch.pair ? pair_tiles : single_tiles) * launch.n_tiles;
+    const uint64_t group = kGroupBytes / (static_cast<uint64_t>(launch.pair ? 2 * kWideM : kWideM) * desc.k);
+    const uint64_t row_blocks = launch.tiles / launch.n_tiles;
+    launch.group_rows = static_cast<uint32_t>(std::min(std::max(group, kGroupRows), row_blocks));
+    return launch;
+}
+
+// Which kernel? Up to 64 rows per expert, wide tiles once they fill the SMs: the wide kernel's deeper
+// copies then stream the weights at least as fast (32 experts of 5632 x 2048 with 8 rows each: 70 us
+// wide, 73 narrow; with 32 rows 77 against 104). One matrix takes the narrow kernel up to 32 rows, its
+// tile. Beyond, the estimate of both in tenths of a microsecond: the blocks of K that a CTA walks
+// through, 0.3 us each with two narrow CTAs an SM and 0.4 us each with a wide one, over the rounds of
+// CTAs, what a further round of narrow CTAs costs (the wide ones stay), and what a split adds. Measured us, narrow and wide: one matrix of 2048 x 2048, 65 rows 7.5 and
+// 9.4, 512 rows 11.2 and 12.5; 2048 x 5632, 128 rows 11.3 and 13.9, 192 rows 16.4 and 14.3; 1024 x 8192,
+// 128 rows 9.9 and 16.2, 384 rows 20.7 and 16.7; 4096 x 4096, 64 rows 10.0 and 10.7, 65 rows 13.7 and
+// 11.7; 11008 x 4096, 33 rows 17.7 and 14.6.
+bool use_wide(const NarrowLaunch &narrow, const WideLaunch &wide, const GemmParams &params, uint64_t share, uint64_t filled, uint64_t sms) {
+    if (filled > 1 && share <= 64) return share > 4 && filled * wide.n_tiles * 4 >= sms * 3;
+    if (share <= 32) return false;
+    const uint64_t tiles = static_cast<uint64_t>(narrow.tiles) * params.n_blocks;
+    const uint64_t narrow_rounds = (tiles * narrow.split + 2 * sms - 1) / (2 * sms);
+    const uint64_t narrow_time =
+        (narrow.split > 1 ? 22 + 20 / narrow.split : 0) + 30 * (narrow_rounds - 1) + 3 * narrow_rounds * params.k_blocks / narrow.split;
+    const uint64_t wide_rounds = (wide.tiles * (wide.pair ? 2 : wide.split) + sms - 1) / sms;
+    const uint64_t wide_time = (wide.split > 1 ? 20 + 5 * wide.split : 15) + 4 * wide_rounds * params.k_blocks / wide.split;
+    return wide_time < narrow_time;
+}
+
 cudaError_t launch_gemm(const qpucuda_fp8_gemm_desc &desc, const qpucuda_fp8_quantize_desc *quantize, unsigned int *error_word,
                         int sm_count, cudaStream_t stream) {
     const GemmParams params = gemm_params(desc, error_word);
@@ -1253,31 +1310,18 @@ cudaError_t launch_gemm(const qpucuda_fp8_gemm_desc &desc, const qpucuda_fp8_qua
     const uint64_t share = (desc.rows + matrices - 1) / matrices;
     const uint64_t sms = static_cast<uint64_t>(sm_count);
     CUtensorMap map_w, map_a;
-    WideLaunch wide{};
-    wide.n_tiles = (desc.n + kWideN - 1) / kWideN;
-    if (use_wide(share, filled, wide.n_tiles, sms)) {
+    const WideLaunch wide = plan_wide(desc, params, share, filled, sms);
+    const NarrowLaunch narrow = plan_narrow(desc, params, share, filled, sms);
+    if (use_wide(narrow, wide, params, share, filled, sms)) {
         if (quantize != nullptr) {
             const cudaError_t error = launch_fp8_quantize_rows(*quantize, sm_count, stream);
             if (error != cudaSuccess) return error;
         }
-        // Pairs where tiles of 256 rows hold hardly more padding than tiles of 128.
-        const uint64_t single_tiles = most_tiles(desc, filled, kWideM), pair_tiles = most_tiles(desc, filled, 2 * kWideM);
-        wide.pair = sms >= 2 && (desc.experts != 0 ? share >= kPairShare : pair_tiles * 2 * 12 <= single_tiles * 13);
-        wide.split = 1;
-        if ((wide.pair ? pair_tiles : single_tiles) * wide.n_tiles * 2 <= sms) {
-            wide.pair = false;
-            while (wide.split < 4 && single_tiles * wide.n_tiles * wide.split * 2 <= sms && wide.split * 8 <= params.k_blocks)
-                wide.split *= 2;
-        }
-        wide.tiles = (wide.pair ? pair_tiles : single_tiles) * wide.n_tiles;
         if (wide.tiles > 0x3FFFFFFFull) return cudaErrorInvalidValue;
         if (!encode_tensor_map_2d_u8(&map_w, desc.w, desc.k, matrices * desc.n, desc.w_stride, kBlockK, kBlockN) ||
             !encode_tensor_map_2d_u8(&map_a, desc.a, desc.k, desc.rows, desc.a_stride, kBlockK, kWideM)) {
             return cudaErrorInvalidValue;
         }
-        const uint64_t group = kGroupBytes / (static_cast<uint64_t>(wide.pair ? 2 * kWideM : kWideM) * desc.k);
-        const uint64_t row_blocks = wide.tiles / wide.n_tiles;
-        wide.group_rows = static_cast<uint32_t>(std::min(std::max(group, kGroupRows), row_blocks));
         switch (desc.out_type) {
             case QPUCUDA_DTYPE_F32: return launch_wide_type<float>(map_w, map_a, params, wide, sm_count, stream);
             case QPUCUDA_DTYPE_BF16: return launch_wide_type<__nv_bfloat16>(map_w, map_a, params, wide, sm_count, stream);
@@ -1285,7 +1329,6 @@ cudaError_t launch_gemm(const qpucuda_fp8_gemm_desc &desc, const qpucuda_fp8_qua
         }
         return cudaErrorInvalidValue;
     }
-    const NarrowLaunch narrow = plan_narrow(desc, params, share, filled, sms);
     FusedRows fused{};
     bool fuse = false;
     if (quantize != nullptr) {

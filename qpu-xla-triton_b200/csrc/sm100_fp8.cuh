@@ -126,20 +126,16 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t address, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(mapped) : "r"(address), "r"(rank));
     return mapped;
 }
-__device__ __forceinline__ float load_cluster(uint32_t cluster_address) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address) : "memory");
-    return v;
+__device__ __forceinline__ void store_cluster(uint32_t cluster_address, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address), "f"(v) : "memory");
 }
 __device__ __forceinline__ int32_t load_cluster_s32(uint32_t cluster_address) {
     int32_t v;
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_address) : "memory");
     return v;
 }
-__device__ __forceinline__ float4 load_cluster4(uint32_t cluster_address) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_address) : "memory");
-    return v;
+__device__ __forceinline__ void store_cluster4(uint32_t cluster_address, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t rank;

@@ -160,7 +160,7 @@ def test_linear_shapes(cuda_device, rows, n, k) -> None:
 
 # One tile shape of the product each: a few rows, with and without a split K; few wide tiles whose K is
 # split in 4 and in 2; wide tiles alone and in pairs, more of them than SMs; a ragged last tile everywhere.
-KERNELS = [(5, 300, 4096), (30, 40000, 300), (200, 1000, 4096), (333, 5000, 2049), (640, 9000, 300), (1023, 5001, 384), (1023, 10000, 130)]
+KERNELS = [(5, 300, 4096), (300, 1000, 8192), (30, 40000, 300), (200, 1000, 4096), (333, 5000, 2049), (640, 9000, 300), (1023, 5001, 384), (1023, 10000, 130)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
