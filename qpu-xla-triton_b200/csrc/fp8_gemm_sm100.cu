@@ -136,8 +136,11 @@ struct Narrow {
     static constexpr int kBuffers = 4;  // tensor memory accumulators
     static constexpr int kTmemColumns = kBuffers * NT;      // a power of two
     static constexpr int kScaleFloats = 2 * NT;             // per warp: this block's and the next's
+    // Other CTAs' sums arrive in memory of their own, as long as they want, where there is room for it.
+    static constexpr bool kOwnSums = NT == 16;
+    static constexpr int kSumBytes = kOwnSums ? NT * kBlockN * 4 : 0;
     static constexpr size_t kSharedBytes =
-        static_cast<size_t>(kStages) * kStageBytes + kFusedBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
+        static_cast<size_t>(kStages) * kStageBytes + kFusedBytes + kSumBytes + kWarps * kScaleFloats * sizeof(float) + 1024 + 256;
     static_assert(kTmemColumns * kCtasPerSm <= 512, "tensor memory");
     static_assert(kSharedBytes * kCtasPerSm + 2048 <= 227 * 1024, "shared memory");
     static_assert(static_cast<size_t>(NT) * kBlockN * 4 <= static_cast<size_t>(kStages) * kStageBytes, "split sums");
@@ -223,7 +226,8 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     uint8_t *stage_w = smem;
     uint8_t *stage_x = smem + Shape::kStages * Shape::kWBytes;  // FUSED: one tile per K block of this CTA
     float *fused_scales = reinterpret_cast<float *>(stage_x + kFusedBlocks * Shape::kXBytes);
-    float *scale_rows = reinterpret_cast<float *>(smem + Shape::kStages * Shape::kStageBytes + Shape::kFusedBytes);
+    float *sums = reinterpret_cast<float *>(Shape::kOwnSums ? smem + Shape::kStages * Shape::kStageBytes + Shape::kFusedBytes : smem);
+    float *scale_rows = reinterpret_cast<float *>(smem + Shape::kStages * Shape::kStageBytes + Shape::kFusedBytes + Shape::kSumBytes);
     Ctl *control = reinterpret_cast<Ctl *>(scale_rows + Shape::kWarps * Shape::kScaleFloats);
     static_assert(sizeof(Ctl) <= 256, "control block");
 
@@ -258,6 +262,7 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (Shape::kOwnSums && split > 1) cluster_arrive();  // this CTA's memory may be written from now on
     const uint32_t tmem_base = control->tmem_base;
     const bool early = params.weights_settled != 0;
     // Weights and offsets that the previous kernel does not write are read before it has finished;
@@ -442,12 +447,13 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
         }
         const uint32_t column = quarter * 32u + lane;  // output column inside the block
         if (split > 1) {
-            // The tile's rows in turn over the ranks: each row's sums go to its rank's stages, which are
-            // free once the MMAs of the whole cluster have completed, as [rank][row / split][column].
+            // The tile's rows in turn over the ranks: each row's sums go to its rank, as [rank][row /
+            // split][column]; into its stages only once the MMAs of the whole cluster have completed.
             __syncwarp();
-            cluster_sync();
+            if (!Shape::kOwnSums) cluster_arrive();
+            cluster_wait();
             const uint32_t rows = tile.row_end - tile.row0;
-            const uint32_t mine = smem_u32(smem) + ((rank * NT >> split_shift) * kBlockN + column) * 4u;
+            const uint32_t mine = smem_u32(sums) + ((rank * NT >> split_shift) * kBlockN + column) * 4u;
 #pragma unroll
             for (uint32_t i = 0; i < kColumns; ++i) {
                 const float v = (i & 1u) ? high(acc[i / 2]) : low(acc[i / 2]);
@@ -467,11 +473,13 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     }
     if (split > 1) {
         __syncwarp();
-        if (warp < 2 || !tile.valid) cluster_sync();
+        if (warp < 2 || !tile.valid) {
+            if (!Shape::kOwnSums) cluster_arrive();
+            cluster_wait();
+        }
         cluster_sync();  // every rank's sums are in place; no CTA touches another's memory from here on
         if (tile.valid && warp >= 2) {
             const uint32_t rows = tile.row_end - tile.row0;
-            const float *sums = reinterpret_cast<const float *>(smem);
             const uint32_t column = threadIdx.x - 64u;  // 128 across
             const bool inside = n0 + column < params.n;
             const float bias = params.bias != nullptr && inside ? __ldg(params.bias + n0 + column) : 0.0f;

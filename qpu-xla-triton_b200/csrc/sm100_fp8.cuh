@@ -147,9 +147,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     return size;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 
 }  // namespace sm100
