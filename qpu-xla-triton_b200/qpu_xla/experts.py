@@ -119,14 +119,14 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     return made(ExpertOrder, offsets=offsets, source=source, position=position.view(tokens, choices))
 
 
-def _destination(out: Any, rows: int, width: int, read: Any, torch_device: Any, what: str) -> tuple[Any, int]:
+def _destination(out: Any, rows: int, width: int, read: Any, read_stride: int, torch_device: Any, what: str) -> tuple[Any, int]:
     """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride."""
     if out is None:
         return new_matrix(rows, width, read.dtype, torch_device), max(width, 1)
     if out.dtype != read.dtype:
         raise ValueError(f"{what} must have the type of its source")
     stride = check_matrix(out, torch_device, what, rows, width)[2]
-    check_apart(out, read, what)
+    check_apart(out, stride, read, read_stride, what)
     return out, stride
 
 
@@ -138,7 +138,7 @@ def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = No
     order.check(torch_device)
     tokens, choices = order.position.shape
     _, width, stride = check_matrix(source, torch_device, "gather_tokens source", tokens)
-    out, out_stride = _destination(out, tokens * choices, width, source, torch_device, "gather_tokens out")
+    out, out_stride = _destination(out, tokens * choices, width, source, stride, torch_device, "gather_tokens out")
     if tokens and width:
         desc = _pack_rows(
             code, tokens, choices, width, order.experts, order.position.data_ptr(), order.offsets.data_ptr(), 0, source.data_ptr(), stride,
@@ -153,7 +153,7 @@ def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: A
     order.check(torch_device)
     tokens, choices = order.position.shape
     _, width, stride = check_matrix(rows, torch_device, name, tokens * choices)
-    out, out_stride = _destination(out, tokens, width, rows, torch_device, name)
+    out, out_stride = _destination(out, tokens, width, rows, stride, torch_device, name)
     if tokens and width:
         desc = _pack_rows(
             code, tokens, choices, width, order.experts, order.position.data_ptr(), 0, 0 if weights is None else weights.data_ptr(),

@@ -83,10 +83,18 @@ def check_matrix(tensor: Any, torch_device: Any, what: str, rows: int | None = N
     return have_rows, have_cols, stride
 
 
-def check_apart(out: Any, read: Any, what: str) -> None:
-    """Refuse an ``out`` that shares bytes with the matrix the call reads: kernels read and write in no
-    particular order. Column ranges of one buffer do not meet."""
-    if _meet(*((t.data_ptr(), *t.shape, t.stride(0) * t.element_size(), t.element_size()) for t in (out, read))):
+def check_apart(out: Any, out_stride: int, read: Any, read_stride: int, what: str) -> None:
+    """Refuse an ``out`` that shares bytes with the matrix the call reads (both with the row strides of
+    :func:`check_matrix`): kernels read and write in no particular order. Column ranges of one buffer do
+    not meet."""
+    begin, read_begin = out.data_ptr(), read.data_ptr()
+    size, read_size = out.element_size(), read.element_size()
+    rows, cols = out.shape
+    read_rows, read_cols = read.shape
+    stride, read_stride = out_stride * size, read_stride * read_size
+    if begin >= read_begin + read_rows * read_stride or read_begin >= begin + rows * stride:
+        return
+    if _meet((begin, rows, cols, stride, size), (read_begin, read_rows, read_cols, read_stride, read_size)):
         raise ValueError(f"{what} must not overlap its source")
 
 
@@ -99,6 +107,10 @@ def _meet(one: tuple[int, ...], other: tuple[int, ...]) -> bool:
     width, other_width = cols * size, other_cols * other_size
     if begin >= other_begin + (other_rows - 1) * other_stride + other_width or other_begin >= begin + (rows - 1) * stride + width:
         return False
+    if rows == 1:
+        stride = other_stride
+    elif other_rows == 1:
+        other_stride = stride
     if stride == other_stride and stride > 0:
         gap = (begin - other_begin) % stride
         return gap < other_width or gap + width > stride
@@ -282,7 +294,7 @@ class _PreparedFP8:
         self._require_open()
         return sum(t.numel() * t.element_size() for t in (self._values, self._scales, self._bias) if t is not None)
 
-    def _output(self: Self, rows: int, out: Any, dtype: Any, read: Any, default: Any) -> tuple[Any, int]:
+    def _output(self: Self, rows: int, out: Any, dtype: Any, read: Any, read_stride: int, default: Any) -> tuple[Any, int]:
         if out is None:
             dtype = default if dtype is None else dtype
             dtype_code(dtype, f"{self._name} output")
@@ -291,7 +303,7 @@ class _PreparedFP8:
             raise ValueError(f"{self._name} out and dtype differ")
         dtype_code(out.dtype, f"{self._name} output")
         stride = check_matrix(out, self._torch_device, f"{self._name} output", rows, self.output_count)[2]
-        check_apart(out, read, f"{self._name} output")
+        check_apart(out, stride, read, read_stride, f"{self._name} output")
         return out, stride
 
     def _gemm_desc(
@@ -354,7 +366,7 @@ class PreparedFP8Linear(_PreparedFP8):
         source's type, or ``out``'s). ``out`` may share a buffer with the source, but no bytes."""
         self._require_open()
         rows, stride, code = self._check_source(source)
-        out, out_stride = self._output(rows, out, dtype, source, source.dtype)
+        out, out_stride = self._output(rows, out, dtype, source, stride, source.dtype)
         if rows:
             self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride)
         return out
@@ -364,7 +376,7 @@ class PreparedFP8Linear(_PreparedFP8):
         defaults to float32."""
         self._require_open()
         count, stride, scale_strides = self._check_rows(rows)
-        out, out_stride = self._output(count, out, dtype, rows.values, torch.float32)
+        out, out_stride = self._output(count, out, dtype, rows.values, stride, torch.float32)
         if count:
             gemm = self._gemm_desc(
                 rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride
@@ -428,7 +440,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._require_open()
         rows, stride, code = self._check_source(source)
         self._check_offsets(offsets)
-        out, out_stride = self._output(rows, out, dtype, source, source.dtype)
+        out, out_stride = self._output(rows, out, dtype, source, stride, source.dtype)
         if rows:
             self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, offsets.data_ptr())
         return out
@@ -441,7 +453,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._check_offsets(order.offsets)
         order.check(self._torch_device, tokens=tokens_count)
         rows = order.rows
-        out, out_stride = self._output(rows, out, dtype, tokens, tokens.dtype)
+        out, out_stride = self._output(rows, out, dtype, tokens, stride, tokens.dtype)
         if rows:
             self._linear(
                 tokens.data_ptr(), code, tokens_count, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, order.offsets.data_ptr(),

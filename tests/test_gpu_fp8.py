@@ -158,9 +158,10 @@ def test_linear_shapes(cuda_device, rows, n, k) -> None:
         check_product(plan.forward(x), exact, magnitude, k)
 
 
-# One tile shape of the product each: a few rows, with and without a split K; few wide tiles whose K is
-# split in 4 and in 2; wide tiles alone and in pairs, more of them than SMs; a ragged last tile everywhere.
-KERNELS = [(5, 300, 4096), (300, 1000, 8192), (30, 40000, 300), (200, 1000, 4096), (333, 5000, 2049), (640, 9000, 300), (1023, 5001, 384), (1023, 10000, 130)]
+# One tile shape of the product each: a few rows, with and without a split K, and several such tiles; few
+# wide tiles whose K is split in 4 and in 2; wide tiles alone and in pairs, more of them than SMs; a
+# ragged last tile everywhere.
+KERNELS = [(5, 300, 4096), (30, 40000, 300), (200, 1000, 4096), (300, 1000, 8192), (333, 5000, 2049), (640, 9000, 300), (1023, 5001, 384), (1023, 10000, 130)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -188,7 +189,7 @@ def test_every_kernel_and_output_layout(cuda_device, dtype, rows, n, k) -> None:
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize(
     "counts, trailing, n, k",
-    [([130, 0, 1, 255, 40], 9, 300, 4096), ([70, 90], 3, 1000, 2048), ([500, 0, 700, 129, 640], 40, 3000, 300), ([1100, 1500, 900, 1025], 17, 3001, 256), ([1100, 1500, 900, 1025], 17, 3200, 256)],
+    [([130, 0, 1, 255, 40], 9, 300, 4096), ([130, 0, 1, 255, 40], 9, 1000, 4096), ([130, 0, 1, 255, 40], 9, 1500, 4096), ([70, 90], 3, 1000, 2048), ([500, 0, 700, 129, 640], 40, 3000, 300), ([1100, 1500, 900, 1025], 17, 3001, 256), ([1100, 1500, 900, 1025], 17, 3200, 256)],
 )
 def test_every_kernel_with_experts(cuda_device, dtype, counts, trailing, n, k) -> None:
     weight, x, offsets, exact, magnitude = expert_case(cuda_device, counts, n, k, trailing)
