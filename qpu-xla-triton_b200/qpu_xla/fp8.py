@@ -410,8 +410,8 @@ class PreparedFP8Linear(_PreparedFP8):
             Kernel("cuda.fp8_linear", executor), (), wait_for=wait_for,
             buffers=(source.access(AccessMode.READ), destination.access(AccessMode.WRITE)),
         )
-        self._pending = [pending for pending in self._pending if not pending.done]
-        self._pending.append(event)
+        with self.device.backend.launch_lock:  # type: ignore[attr-defined]
+            self._pending = [*(pending for pending in self._pending if not pending.done), event]
         return event
 
 
