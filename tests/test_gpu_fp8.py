@@ -95,6 +95,20 @@ def test_row_quantizer_takes_strided_and_unaligned_rows(cuda_device, dtype) -> N
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", [(9, 300), (900, 4097)])
+def test_row_quantizer_at_every_alignment(cuda_device, dtype, rows, cols) -> None:
+    for stride in (cols + 7, cols + 8 + cols % 2, 2 * cols + 2):
+        base = draw((rows + 1, stride), dtype, seed=stride)
+        for start in range(8):
+            x = base.view(-1)[start : start + rows * stride].view(rows, stride)[:, :cols]
+            check_rows(quantize_rows_fp8(cuda_device, x), x)
+        x = base[1:, : 2 * (cols // 2)]
+        gated = quantize_rows_fp8(cuda_device, x, gated=True)
+        again = quantize_rows_fp8(cuda_device, x.clone(), gated=True)
+        assert torch.equal(gated.values.view(torch.uint8), again.values.view(torch.uint8)) and torch.equal(gated.scales, again.scales)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows, cols, std", [(1, 1, 1.0), (4, 128, 1.0), (7, 333, 3.0), (40, 5632, 1.0), (50, 500, 40.0)])
 def test_gated_rows(cuda_device, dtype, rows, cols, std) -> None:
     """exp is within 2 steps of 2^-23 (CUDA's bound), the sum and the product round once, the quotient is
