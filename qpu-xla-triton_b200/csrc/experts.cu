@@ -567,8 +567,20 @@ cudaError_t launch_expert_sort(const qpucuda_expert_sort_desc &d, cudaStream_t s
                : sort_typed(static_cast<const int32_t *>(d.ids), total, d.experts, d.offsets, d.source, d.position, counts, stream);
 }
 
-cudaError_t launch_expert_gather(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream) {
-    QPUCUDA_ROWS_DISPATCH(gather_typed, desc.type, vector_moves(desc), desc, sm_count, stream);
+cudaError_t launch_expert_gather(const qpucuda_expert_rows_desc &given, int sm_count, cudaStream_t stream) {
+    // A copy, whatever the elements: pairs of 16-bit ones move as one of 32 bits where they may (4096 x 4 of
+    // 2046 bf16, in a captured graph 11 us, 15 one by one).
+    qpucuda_expert_rows_desc desc = given;
+    if (desc.type != QPUCUDA_DTYPE_F32) {
+        const uint64_t either = reinterpret_cast<uintptr_t>(desc.source) / 2 | reinterpret_cast<uintptr_t>(desc.out) / 2 | desc.width |
+                                desc.source_stride | desc.out_stride;
+        if (either % 2 != 0) return gather_typed<__nv_bfloat16, false>(desc, sm_count, stream);
+        desc.type = QPUCUDA_DTYPE_F32;
+        desc.width /= 2;
+        desc.source_stride /= 2;
+        desc.out_stride /= 2;
+    }
+    return vector_moves(desc) ? gather_typed<float, true>(desc, sm_count, stream) : gather_typed<float, false>(desc, sm_count, stream);
 }
 
 cudaError_t launch_expert_combine(const qpucuda_expert_rows_desc &desc, int sm_count, cudaStream_t stream) {

@@ -132,7 +132,7 @@ def test_strided_and_unaligned_rows(cuda_device, dtype) -> None:
     tokens, choices, experts, width = 50, 3, 6, 64
     order = sort_tokens(cuda_device, draw_ids(tokens, choices, experts), experts)
     weights = torch.rand((tokens, choices), device="cuda")
-    for start in (0, 1, 8):
+    for start in (0, 1, 2, 8):
         x = draw((tokens, width + 24), dtype, seed=start)[:, start : start + width]
         wide = torch.full((tokens * choices + 2, width + 24), 5.0, dtype=dtype, device="cuda")
         out = wide[1:-1, start : start + width]
