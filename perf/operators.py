@@ -195,22 +195,22 @@ def _inputs(case: dict, seed: int) -> dict:
     return state
 
 
-_package: list = []  # the opened device and the two modules, once per process
+def _device():
+    root = Path(__file__).resolve().parents[1] / "qpu-xla-triton_b200"
+    if str(root) not in sys.path:
+        sys.path.insert(0, str(root))
+    from qpu_xla import Device
 
-
-def _framework():
-    if not _package:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "qpu-xla-triton_b200"))
-        from qpu_xla import Device, experts, fp8
-
-        _package.extend((Device.open(), experts, fp8))
-    return _package
+    if not hasattr(_device, "opened"):
+        _device.opened = Device.open()
+    return _device.opened
 
 
 def _plan(state: dict) -> None:
     """What a program makes once and keeps: the plan that owns the weight, the order of the forward pass."""
-    device, experts, fp8 = _framework()
-    op = state["case"]["op"]
+    device, op = _device(), state["case"]["op"]
+    from qpu_xla import experts, fp8
+
     if op == "linear":
         weight = fp8.QuantizedBlocksFP8(state["values"], state["scales"])
         state["plan"] = fp8.PreparedFP8Linear(device, weight, bias=state["bias"], gated=state["case"]["gated"])
@@ -236,8 +236,9 @@ def prepare(case: dict, seed: int) -> dict:
 def _run_own(state: dict):
     if "plan" not in state:
         _plan(state)
-    (device, experts, fp8), case = _framework(), state["case"]
-    op = case["op"]
+    device, case, op = _device(), state["case"], state["case"]["op"]
+    from qpu_xla import experts, fp8
+
     if op == "quantize":
         rows = fp8.quantize_rows_fp8(device, state["x"])
         return [rows.values, rows.scales]
