@@ -694,7 +694,9 @@ __device__ __forceinline__ void add_bias(const GemmParams &params, uint32_t n, f
 // One box of a warp's 32 rows (a row to a lane, 128 bytes each) on its way out. Staged in shared
 // memory in the 128-byte swizzle (16-byte slot c of row r at c ^ (r & 7): no bank conflicts) and copied
 // out from there: by the copy engine while the warp goes on, where the output's rows are aligned and
-// all 32 are the tile's (`map` then), else by the warp, eight lanes to a row.
+// all 32 are the tile's (`map` then), else by the warp, eight lanes to a row. A warp's boxes take its two
+// buffers in turn, over all of its tiles (a ragged last tile can have an odd number of boxes), and each
+// box is one group of copies, so a buffer is free once no more than the newest group is still being read.
 template <typename Out>
 __device__ __forceinline__ void store_box(uint8_t *buffer, const float (&v)[128 / sizeof(Out)], const CUtensorMap *map, Out *out,
                                           size_t out_stride, int row, uint32_t column, uint32_t rows, uint32_t columns, bool vector,
@@ -963,6 +965,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t quarter = warp & 3u;
         const uint32_t half = worker / 4u;
         uint8_t *buffer_out = store + worker * kWideStoreBytes;
+        uint32_t box = 0;  // the buffer of this warp's next box, in turn across its tiles
         const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + half * (kWideN / 2);
         const bool vector = (reinterpret_cast<uintptr_t>(params.out) & 15u) == 0 && params.out_stride * sizeof(Out) % 16 == 0;
         const uint32_t tmem_full0 = smem_u32(&control->tmem_full[0]);
@@ -1086,9 +1089,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     v[i + 1] = high(acc[(c + i) / 2]);
                 }
                 add_bias(params, n, v);
-                store_box<Out>(buffer_out + (c / kChunk & 1) * kWideBoxBytes, v, whole && n + kChunk <= params.n ? &map_out : nullptr,
+                store_box<Out>(buffer_out + box, v, whole && n + kChunk <= params.n ? &map_out : nullptr,
                                static_cast<Out *>(params.out) + static_cast<size_t>(row0) * params.out_stride + n, params.out_stride,
                                static_cast<int>(row0), n, rows, params.n - n, vector, lane);
+                box ^= kWideBoxBytes;
             }
         }
         if constexpr (SPLIT) {

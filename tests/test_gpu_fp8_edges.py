@@ -1,0 +1,54 @@
+"""Block-scaled FP8 on the GPU: output widths whose last tile has an odd number of boxes on their way out."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fp8_reference as ref
+from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear
+from test_gpu_fp8 import blocks, check_product, draw, expert_case
+
+pytestmark = pytest.mark.gpu
+
+# One box is 128 bytes of each of a warp's 32 rows and a tile's half has 128 columns, so widths that end in one
+# whole box (16-bit: 64, fp32: 32) or three (fp32: 96) give an odd number; the others are their neighbours.
+WIDTHS = [(torch.bfloat16, n) for n in (64, 192, 320, 576, 640)] + [(torch.float16, n) for n in (64, 192, 576)] + [
+    (torch.float32, n) for n in (32, 96, 160, 224, 352, 384)
+]
+
+
+@pytest.mark.parametrize("dtype, n", WIDTHS)
+@pytest.mark.parametrize("k", [128, 200])
+def test_many_short_tiles_of_every_width(cuda_device, dtype, n, k) -> None:
+    """65536 rows are 256 pairs' tiles per 256 columns, several to each pair of CTAs, and K of one or two blocks
+    leaves next to no time between a tile's store and the next one's. The copy engine's rows equal the warps'
+    (an output off its 16-byte boundary) bit for bit, and repeat."""
+    rows = 65536
+    weight = blocks(cuda_device, n, k)
+    x = draw((rows, k), torch.bfloat16, seed=n)
+    exact, magnitude = ref.product(*ref.quantize_rows(x), weight.values, weight.scales)
+    wide = torch.full((rows, n + 3), 7.0, dtype=dtype, device="cuda")
+    with PreparedFP8Linear(cuda_device, weight) as plan:
+        y = plan.forward(x, dtype=dtype)
+        check_product(y, exact, magnitude, k)
+        for _ in range(5):
+            assert torch.equal(plan.forward(x, dtype=dtype), y)
+        plan.forward(x, out=wide[:, 1 : 1 + n])
+        assert torch.equal(wide[:, 1 : 1 + n], y)
+
+
+@pytest.mark.parametrize("dtype, n", WIDTHS)
+@pytest.mark.parametrize("counts", [[700] * 16, [1100, 0, 900, 1300] * 4])
+def test_many_short_tiles_of_every_width_with_experts(cuda_device, dtype, n, counts) -> None:
+    """The same with a matrix per expert, in tiles of one CTA and of pairs: every expert has its own last tiles."""
+    k = 128
+    weight, x, offsets, exact, magnitude = expert_case(cuda_device, counts, n, k, trailing=5)
+    wide = torch.full((x.shape[0], n + 3), 7.0, dtype=dtype, device="cuda")
+    with PreparedFP8Experts(cuda_device, weight) as plan:
+        y = plan.forward(x, offsets, dtype=dtype)
+        check_product(y, exact, magnitude, k)
+        for _ in range(5):
+            assert torch.equal(plan.forward(x, offsets, dtype=dtype), y)
+        plan.forward(x, offsets, out=wide[:, 1 : 1 + n])
+        assert torch.equal(wide[:, 1 : 1 + n], y)
