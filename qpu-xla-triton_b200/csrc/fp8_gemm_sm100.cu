@@ -207,7 +207,34 @@ struct Control {
     uint64_t rows_ready;  // the product's own quantized rows are in place
     uint32_t tmem_base;
     volatile int abort_flag;
+    uint32_t copies;      // stages that warp 0's first thread has set under way
+    uint32_t multiplied;  // warp 1's has issued an MMA
 };
+
+// Parity of the phase that the last of `issued` copies into `stage` completes, the stages taken in turn.
+__host__ __device__ constexpr uint32_t last_phase(uint32_t issued, uint32_t stage, uint32_t stages) {
+    return ((issued - stage + stages - 1) / stages - 1) & 1u;
+}
+static_assert(last_phase(1, 0, 5) == 0 && last_phase(5, 4, 5) == 0 && last_phase(6, 0, 5) == 1 && last_phase(6, 1, 5) == 0 &&
+                  last_phase(10, 4, 5) == 1 && last_phase(11, 0, 5) == 0 && last_phase(11, 1, 5) == 1,
+              "stages 0 to issued - 1, each pass of the ring the other parity");
+
+// A wait of this CTA ran out, in whichever warp: no role takes another step, but the copies and the MMAs that
+// were issued must end before the CTA gives up its memory, also where the warp that issued them had nothing
+// left to wait for. Each by the thread that issued them; the waits are bounded.
+template <int STAGES>
+__device__ __forceinline__ void drain_copies(uint64_t *full, uint32_t issued) {
+    for (uint32_t s = 0; s < STAGES && s < issued; ++s) wait_drain(smem_u32(&full[s]), last_phase(issued, s, STAGES));
+}
+template <bool PAIR>
+__device__ __forceinline__ void drain_mmas(uint64_t *drain) {
+    if constexpr (PAIR) {
+        mma_commit_pair_local(smem_u32(drain));
+    } else {
+        mma_commit(smem_u32(drain));
+    }
+    wait_drain(smem_u32(drain), 0);
+}
 
 // Grid: x = column block * split + rank in the cluster, y = tile of rows. The CTAs of a cluster
 // share a tile and split its K blocks; their sums meet in distributed shared memory in rank order,
@@ -251,6 +278,7 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
         mbar_init(smem_u32(&control->drain), 1);
         mbar_init(smem_u32(&control->rows_ready), 1);
         control->abort_flag = 0;
+        control->copies = control->multiplied = 0;
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -297,28 +325,20 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
             if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             for (uint32_t s = 0; s < ahead; ++s) load_x(kb_begin + s, s);
-            uint32_t stage = 0, phase = 1, issued = ahead;
-            bool ok = true;
+            uint32_t stage = 0, phase = 1, copies = ahead;
             if (ahead == Shape::kStages) {
                 for (uint32_t i = ahead; i < count; ++i) {
-                    ok = wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word);
-                    if (!ok) break;
+                    if (!wait_bounded(smem_u32(&control->empty[stage]), phase ^ 1u, &control->abort_flag, params.error_word)) break;
                     load_w(kb_begin + i, stage);
                     load_x(kb_begin + i, stage);
-                    ++issued;
+                    ++copies;
                     if (++stage == Shape::kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (!ok) {
-                // Let every copy in flight land before the CTA exits: the last use of each stage.
-                for (uint32_t s = 0; s < ahead; ++s) {
-                    const uint32_t uses = (issued - s + Shape::kStages - 1) / Shape::kStages;
-                    wait_drain(smem_u32(&control->full[s]), (uses - 1) & 1u);
-                }
-            }
+            control->copies = copies;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -352,10 +372,7 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
                     buffer_phase ^= 1u;
                 }
             }
-            if (!ok && any) {
-                mma_commit(smem_u32(&control->drain));
-                wait_drain(smem_u32(&control->drain), 0);
-            }
+            control->multiplied = any ? 1u : 0u;
         }
         __syncwarp();
     } else {
@@ -502,6 +519,11 @@ __global__ void __launch_bounds__(Narrow<NT, FUSED>::kThreads, Narrow<NT, FUSED>
     }
     tc_fence_before();
     __syncthreads();
+    if (control->abort_flag != 0) {
+        if (threadIdx.x == 0) drain_copies<Shape::kStages>(control->full, control->copies);
+        if (threadIdx.x == 32 && control->multiplied != 0) drain_mmas<false>(&control->drain);
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Shape::kTmemColumns)
@@ -790,6 +812,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         }
         mbar_init(smem_u32(&control->drain), 1);
         control->abort_flag = 0;
+        control->copies = control->multiplied = 0;
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -850,7 +873,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         if (lane == 0) {
             prefetch_tensor_map(&map_w);
             prefetch_tensor_map(&map_a);
-            uint32_t stage = 0, phase = 0, issued_mask = 0, issued_phases = 0;
+            uint32_t stage = 0, phase = 0, copies = 0;
             bool ok = true;
             for (uint32_t t = tile_first; ok && t < total; t += tile_step) {
                 const WideTile tile = locate<Shape::kRows>(params, first_tile, first_row, n_tiles, group_rows, t);
@@ -872,26 +895,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes), &map_w, full, x, w_row);
                         tma_load_2d(smem_u32(stage_w + stage * Shape::kWBytes + Shape::kWBytes / 2), &map_w, full, x, w_row + kBlockN);
                     }
-                    issued_mask |= 1u << stage;
-                    issued_phases = (issued_phases & ~(1u << stage)) | (phase << stage);
+                    ++copies;
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (!ok) {
-                // Let every copy in flight land before the CTA exits. Only rank 0's barriers see a
-                // pair's copies; the other CTA gives its own a bounded 200 us instead.
-                if (rank == 0) {
-                    for (int s = 0; s < kStages; ++s)
-                        if ((issued_mask >> s) & 1u) wait_drain(smem_u32(&control->full[s]), (issued_phases >> s) & 1u);
-                } else {
-                    const uint64_t start = globaltimer();
-                    while (globaltimer() - start < 200000ull) {
-                    }
-                }
-            }
+            control->copies = copies;
         }
         __syncwarp();
         if constexpr (SPLIT) {
@@ -939,14 +950,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     }
                 }
             }
-            if (!ok && any) {
-                if constexpr (PAIR) {
-                    mma_commit_pair_local(smem_u32(&control->drain));
-                } else {
-                    mma_commit(smem_u32(&control->drain));
-                }
-                wait_drain(smem_u32(&control->drain), 0);
-            }
+            control->multiplied = any ? 1u : 0u;
         }
         __syncwarp();
         if constexpr (SPLIT) {
@@ -1141,6 +1145,20 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (control->abort_flag != 0) {
+        if (threadIdx.x == 0) {
+            // Only rank 0's barriers see a pair's copies; the other CTA gives its own a bounded 200 us.
+            if (!PAIR || cluster_rank() == 0) {
+                drain_copies<kStages>(control->full, control->copies);
+            } else {
+                const uint64_t start = globaltimer();
+                while (globaltimer() - start < 200000ull) {
+                }
+            }
+        }
+        if (threadIdx.x == 32 && control->multiplied != 0) drain_mmas<PAIR>(&control->drain);
+        __syncthreads();
+    }
     // Neither CTA of a pair leaves while the other may still signal its barriers, read its shared
     // memory or write its tensor memory.
     if constexpr (PAIR) cluster_sync();
