@@ -6,6 +6,8 @@ outside ``[0, experts)`` drops the choice (a padding token). No counterpart in
 the reference. The order and the sums never depend on timing: the sort counts
 integers, a token's choices are added in their order, there are no atomics on
 floating-point values.
+An output that the caller gives shares no bytes with what the call reads (rows,
+positions, offsets, weights); one that does is refused.
 
 The functions run on the current stream of their device. There is no autograd:
 each step's gradient is a function of its own (``gather_tokens_backward``,
@@ -28,6 +30,7 @@ from qpu_xla.fp8 import (
     PreparedFP8Experts,
     QuantizedBlocksFP8,
     check_apart,
+    check_apart_from,
     check_matrix,
     dtype_code,
     launch,
@@ -119,7 +122,9 @@ def sort_tokens(device: Device, expert_ids: Any, experts: int) -> ExpertOrder:
     return made(ExpertOrder, offsets=offsets, source=source, position=position.view(tokens, choices))
 
 
-def _destination(out: Any, rows: int, width: int, read: Any, read_stride: int, torch_device: Any, what: str) -> tuple[Any, int]:
+def _destination(
+    out: Any, rows: int, width: int, read: Any, read_stride: int, reads: tuple[Any, ...], torch_device: Any, what: str
+) -> tuple[Any, int]:
     """``out`` (or a new tensor) for rows of ``read``'s type, and its row stride."""
     if out is None:
         return new_matrix(rows, width, read.dtype, torch_device), max(width, 1)
@@ -127,6 +132,7 @@ def _destination(out: Any, rows: int, width: int, read: Any, read_stride: int, t
         raise ValueError(f"{what} must have the type of its source")
     stride = check_matrix(out, torch_device, what, rows, width)[2]
     check_apart(out, stride, read, read_stride, what)
+    check_apart_from(out, stride, reads, what)
     return out, stride
 
 
@@ -138,7 +144,8 @@ def gather_tokens(device: Device, source: Any, order: ExpertOrder, out: Any = No
     order.check(torch_device)
     tokens, choices = order.position.shape
     _, width, stride = check_matrix(source, torch_device, "gather_tokens source", tokens)
-    out, out_stride = _destination(out, tokens * choices, width, source, stride, torch_device, "gather_tokens out")
+    reads = (order.position, order.offsets)
+    out, out_stride = _destination(out, tokens * choices, width, source, stride, reads, torch_device, "gather_tokens out")
     if tokens and width:
         desc = _pack_rows(
             code, tokens, choices, width, order.experts, order.position.data_ptr(), order.offsets.data_ptr(), 0, source.data_ptr(), stride,
@@ -153,7 +160,8 @@ def _combine(device: Device, rows: Any, weights: Any, order: ExpertOrder, out: A
     order.check(torch_device)
     tokens, choices = order.position.shape
     _, width, stride = check_matrix(rows, torch_device, name, tokens * choices)
-    out, out_stride = _destination(out, tokens, width, rows, stride, torch_device, name)
+    reads = (order.position,) if weights is None else (order.position, weights)
+    out, out_stride = _destination(out, tokens, width, rows, stride, reads, torch_device, name)
     if tokens and width:
         desc = _pack_rows(
             code, tokens, choices, width, order.experts, order.position.data_ptr(), 0, 0 if weights is None else weights.data_ptr(),

@@ -10,6 +10,9 @@ Activation rows are quantized on the fly with one scale per 128 columns::
 summed in fp32 and rounded once to the output's type. A group of 128 columns
 that holds a NaN or an infinity dequantizes to NaN, and so do that row's outputs.
 
+An output that the caller gives may lie in a buffer with what the call reads (source, scales, offsets), but
+shares no bytes with it; such an output is refused.
+
 Everything here runs on the current stream of the plan's device, allocates its
 scratch from PyTorch per call (so calls on several streams, and several captured
 CUDA graphs, share no workspace) and has no CPU path. There is no autograd: a
@@ -96,6 +99,30 @@ def check_apart(out: Any, out_stride: int, read: Any, read_stride: int, what: st
         return
     if _meet((begin, rows, cols, stride, size), (read_begin, read_rows, read_cols, read_stride, read_size)):
         raise ValueError(f"{what} must not overlap its source")
+
+
+def check_apart_from(out: Any, out_stride: int, reads: Iterable[Any], what: str) -> None:
+    """Refuse an ``out`` that shares bytes with one of the other tensors the call reads (scales, offsets,
+    positions, weights; rank 1 or 2)."""
+    begin, size = out.data_ptr(), out.element_size()
+    rows, cols = out.shape
+    for read in reads:
+        if _meet((begin, rows, cols, out_stride * size, size), _layout(read)):
+            raise ValueError(f"{what} must not overlap what the call reads")
+
+
+def _layout(tensor: Any) -> tuple[int, ...]:
+    """A tensor as a row-major matrix for :func:`_meet`: its rows, its columns, or else the whole range of
+    addresses it spans."""
+    size, begin = tensor.element_size(), tensor.data_ptr()
+    if tensor.dim() == 2 and not tensor.is_contiguous():
+        (rows, cols), (stride, inner) = tensor.shape, tensor.stride()
+        if inner == 1:
+            return begin, rows, cols, stride * size, size
+        if stride == 1:
+            return begin, cols, rows, inner * size, size
+    span = 0 if tensor.numel() == 0 else 1 + sum((extent - 1) * step for extent, step in zip(tensor.shape, tensor.stride()))
+    return begin, 1, span, span * size, size
 
 
 def _meet(one: tuple[int, ...], other: tuple[int, ...]) -> bool:
@@ -294,7 +321,9 @@ class _PreparedFP8:
         self._require_open()
         return sum(t.numel() * t.element_size() for t in (self._values, self._scales, self._bias) if t is not None)
 
-    def _output(self: Self, rows: int, out: Any, dtype: Any, read: Any, read_stride: int, default: Any) -> tuple[Any, int]:
+    def _output(
+        self: Self, rows: int, out: Any, dtype: Any, read: Any, read_stride: int, default: Any, *reads: Any
+    ) -> tuple[Any, int]:
         if out is None:
             dtype = default if dtype is None else dtype
             dtype_code(dtype, f"{self._name} output")
@@ -304,6 +333,7 @@ class _PreparedFP8:
         dtype_code(out.dtype, f"{self._name} output")
         stride = check_matrix(out, self._torch_device, f"{self._name} output", rows, self.output_count)[2]
         check_apart(out, stride, read, read_stride, f"{self._name} output")
+        check_apart_from(out, stride, reads, f"{self._name} output")
         return out, stride
 
     def _gemm_desc(
@@ -376,7 +406,7 @@ class PreparedFP8Linear(_PreparedFP8):
         defaults to float32."""
         self._require_open()
         count, stride, scale_strides = self._check_rows(rows)
-        out, out_stride = self._output(count, out, dtype, rows.values, stride, torch.float32)
+        out, out_stride = self._output(count, out, dtype, rows.values, stride, torch.float32, rows.scales)
         if count:
             gemm = self._gemm_desc(
                 rows.values.data_ptr(), stride, rows.scales.data_ptr(), scale_strides, count, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride
@@ -440,7 +470,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._require_open()
         rows, stride, code = self._check_source(source)
         self._check_offsets(offsets)
-        out, out_stride = self._output(rows, out, dtype, source, stride, source.dtype)
+        out, out_stride = self._output(rows, out, dtype, source, stride, source.dtype, offsets)
         if rows:
             self._linear(source.data_ptr(), code, rows, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, offsets.data_ptr())
         return out
@@ -453,7 +483,7 @@ class PreparedFP8Experts(_PreparedFP8):
         self._check_offsets(order.offsets)
         order.check(self._torch_device, tokens=tokens_count)
         rows = order.rows
-        out, out_stride = self._output(rows, out, dtype, tokens, stride, tokens.dtype)
+        out, out_stride = self._output(rows, out, dtype, tokens, stride, tokens.dtype, order.offsets, order.source)
         if rows:
             self._linear(
                 tokens.data_ptr(), code, tokens_count, stride, rows, out.data_ptr(), _DTYPE_CODES[out.dtype], out_stride, order.offsets.data_ptr(),
