@@ -12,6 +12,9 @@
  * A group of rows with a NaN or an infinity dequantizes to NaN, and so do the
  * outputs of that row; no other row is affected. Every call allocates nothing
  * and may be captured into a CUDA graph.
+ * The product's waits inside a kernel are bounded. One that runs out leaves
+ * outputs unwritten or incomplete and ends without a CUDA error; the next
+ * qpucuda_context_synchronize returns QPUCUDA_TIMEOUT.
  */
 #ifndef QPUCUDA_FP8_H
 #define QPUCUDA_FP8_H

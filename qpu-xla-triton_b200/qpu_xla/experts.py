@@ -250,9 +250,16 @@ class FP8ExpertsFFN:
         rows = self.down.forward(hidden, order.offsets, dtype=source.dtype)
         return combine_tokens(self.device, rows, weights, order)
 
+    def synchronize(self: Self) -> None:
+        """Wait for the device's current stream and raise if a kernel's wait ran out (as a plan's ``synchronize``)."""
+        self.gate_up.synchronize()
+
     def close(self: Self) -> None:
-        self.gate_up.close()
-        self.down.close()
+        """Close both plans (which wait for the device and raise what ``synchronize`` would)."""
+        try:
+            self.gate_up.close()
+        finally:
+            self.down.close()
 
     def __enter__(self: Self) -> Self:
         return self

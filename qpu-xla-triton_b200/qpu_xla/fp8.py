@@ -10,13 +10,18 @@ Activation rows are quantized on the fly with one scale per 128 columns::
 summed in fp32 and rounded once to the output's type. A group of 128 columns
 that holds a NaN or an infinity dequantizes to NaN, and so do that row's outputs.
 
-An output that the caller gives may lie in a buffer with what the call reads (source, scales, offsets), but
-shares no bytes with it; such an output is refused.
+An output that the caller gives may lie in a buffer with what the call reads
+(source, scales, offsets), but one that shares bytes with it is refused.
 
 Everything here runs on the current stream of the plan's device, allocates its
 scratch from PyTorch per call (so calls on several streams, and several captured
 CUDA graphs, share no workspace) and has no CPU path. There is no autograd: a
 source that requires grad is refused while gradients are recorded.
+
+The product's waits inside a kernel are bounded: one that runs out leaves outputs
+unwritten or incomplete, records it on the device and ends without a CUDA error.
+A plan's ``synchronize`` and ``close`` raise then, as a queue's event does;
+results on a stream are certain once one of them has returned.
 """
 
 from __future__ import annotations
@@ -263,7 +268,7 @@ class _PreparedFP8:
     """A weight (one matrix, or one per expert) resident on one GPU in the layout the product reads:
     e4m3 rows padded to 16 bytes, block scales, optional bias. The plan owns copies; calls only
     read them, so any number may be in flight. Keep the plan open until their work has finished
-    (``close`` waits for the device)."""
+    (``close`` waits for the device, and raises what ``synchronize`` would)."""
 
     _name = "prepared FP8 linear"
 
@@ -303,8 +308,23 @@ class _PreparedFP8:
         if self._closed:
             raise RuntimeError(f"{self._name} plan is closed")
 
+    def synchronize(self: Self) -> None:
+        """Wait for the device's current stream (up to the device's timeout) and raise if a kernel's wait ran out,
+        in a call of any plan of the device: ``EventTimeoutError`` the first time, ``NativeError`` from then on."""
+        self._require_open()
+        with torch.cuda.device(self._torch_device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            raise RuntimeError(f"{self._name} calls cannot be waited for while a graph is captured")
+        self._raise_device_errors()
+
+    def _raise_device_errors(self: Self) -> None:
+        stream = torch.cuda.current_stream(self._torch_device)
+        self.device.backend.launch(stream, lambda native: native.synchronize())  # type: ignore[attr-defined]
+
     def close(self: Self) -> None:
-        """Wait for queued executions and for the device, and release the weight."""
+        """Wait for queued executions and for the device, release the weight, and raise if a kernel's wait
+        ran out (while the device is open; a closed one knows no more of it)."""
         if self._closed:
             return
         for event in self._pending:
@@ -315,6 +335,8 @@ class _PreparedFP8:
         torch.cuda.synchronize(self._torch_device)
         self._values = self._scales = self._bias = None
         self._closed = True
+        if not self.device.closed:
+            self._raise_device_errors()
 
     @property
     def resident_bytes(self: Self) -> int:

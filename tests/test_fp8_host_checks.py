@@ -4,13 +4,15 @@ its calls."""
 from __future__ import annotations
 
 import random
+from contextlib import nullcontext
 from types import SimpleNamespace
 from typing import Any
 
 import pytest
 import torch
 
-from qpu_xla.experts import ExpertOrder, combine_tokens, gather_tokens, gather_tokens_backward
+from qpu_xla.errors import EventTimeoutError, NativeError
+from qpu_xla.experts import ExpertOrder, FP8ExpertsFFN, combine_tokens, gather_tokens, gather_tokens_backward
 from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, QuantizedRowsFP8, check_apart_from
 
 E4M3 = torch.float8_e4m3fn
@@ -138,3 +140,86 @@ def test_positions_and_routing_weights_are_not_overwritten() -> None:
     combine_tokens(device, rows, weights, order, out=buffer[:32].view(4, 8))
     gather_tokens_backward(device, rows, order, out=buffer[40:72].view(4, 8))  # its offsets and source are not read
     assert device.calls == ["qpucuda_expert_gather", "qpucuda_expert_combine", "qpucuda_expert_combine"]
+
+
+class FakeNative:
+    """The library's context: its error word, read by ``synchronize``."""
+
+    def __init__(self) -> None:
+        self.expired = self.poisoned = False
+        self.waits: list[Any] = []
+
+    def synchronize(self) -> None:
+        if self.poisoned:
+            raise NativeError(5, "CUDA context is poisoned after a wait failure")
+        if self.expired:
+            self.poisoned = True
+            raise EventTimeoutError("a kernel barrier wait exceeded its bound")
+
+
+@pytest.fixture
+def waiting_device(monkeypatch: pytest.MonkeyPatch) -> RecordingDevice:
+    device, native = RecordingDevice(), FakeNative()
+
+    def launch(stream: Any, fn: Any) -> Any:
+        native.waits.append(stream)
+        return fn(native)
+
+    device.backend.native, device.backend.launch = native, launch
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: native.waits.append("device"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "current")
+    monkeypatch.setattr(torch.cuda, "device", lambda device: nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return device
+
+
+def test_an_expired_wait_of_a_stream_call_is_raised(waiting_device: RecordingDevice) -> None:
+    """The kernels end without a CUDA error, so the plan has to ask: on request, and when it closes."""
+    native = waiting_device.backend.native
+    with plan_of(PreparedFP8Linear, waiting_device, n=4, k=16) as plan:
+        plan.synchronize()
+        assert native.waits == ["current"]
+        native.expired = True
+        with pytest.raises(EventTimeoutError, match="exceeded its bound"):
+            plan.synchronize()
+        with pytest.raises(NativeError, match="poisoned"):
+            plan.close()
+    assert native.waits[-2:] == ["device", "current"]  # everything has ended before the error word is read
+    with pytest.raises(RuntimeError, match="closed"):
+        plan.synchronize()
+
+
+def test_close_reports_an_expired_wait_and_releases_the_weight(waiting_device: RecordingDevice) -> None:
+    waiting_device.backend.native.expired = True
+    plan = plan_of(PreparedFP8Linear, waiting_device, n=4, k=16)
+    plan._values = plan._scales = torch.zeros(1)
+    with pytest.raises(EventTimeoutError):
+        plan.close()
+    assert plan._closed and plan._values is None and plan._scales is None
+    plan.close()  # once
+
+
+def test_close_after_the_device_asks_it_nothing(waiting_device: RecordingDevice) -> None:
+    waiting_device.closed = True
+    waiting_device.backend.native.expired = True
+    plan_of(PreparedFP8Linear, waiting_device, n=4, k=16).close()
+
+
+def test_the_layer_closes_both_plans_and_raises(waiting_device: RecordingDevice) -> None:
+    layer = object.__new__(FP8ExpertsFFN)
+    layer.device = waiting_device
+    layer.gate_up, layer.down = (plan_of(PreparedFP8Experts, waiting_device, n=4, k=16, experts=2) for _ in range(2))
+    layer.synchronize()
+    waiting_device.backend.native.expired = True
+    with pytest.raises(EventTimeoutError):
+        layer.synchronize()
+    with pytest.raises(NativeError):
+        layer.close()
+    assert layer.gate_up._closed and layer.down._closed
+
+
+def test_no_wait_while_a_graph_is_captured(waiting_device: RecordingDevice, monkeypatch: pytest.MonkeyPatch) -> None:
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        plan_of(PreparedFP8Linear, waiting_device, n=4, k=16).synchronize()
+    assert waiting_device.backend.native.waits == []

@@ -1,4 +1,5 @@
-"""Block-scaled FP8 on the GPU: output widths whose last tile has an odd number of boxes on their way out."""
+"""Block-scaled FP8 on the GPU where it can go wrong: the widths of last tiles, signs and padding of quantized
+rows, waits that ran out."""
 
 from __future__ import annotations
 
@@ -6,6 +7,8 @@ import pytest
 import torch
 
 import fp8_reference as ref
+from qpu_xla import Device, _native
+from qpu_xla.errors import EventTimeoutError, NativeError
 from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear
 from test_gpu_fp8 import blocks, check_product, draw, expert_case
 
@@ -52,3 +55,33 @@ def test_many_short_tiles_of_every_width_with_experts(cuda_device, dtype, n, cou
             assert torch.equal(plan.forward(x, offsets, dtype=dtype), y)
         plan.forward(x, offsets, out=wide[:, 1 : 1 + n])
         assert torch.equal(wide[:, 1 : 1 + n], y)
+
+
+def test_an_expired_wait_reaches_the_caller_of_a_stream(cuda_device) -> None:
+    """``synchronize`` and ``close`` read the error word after the stream's work: with the library's injected wait
+    failure in place of a kernel's, on a context of its own."""
+    weight = blocks(cuda_device, 64, 128)
+    x = draw((4, 128))
+    with Device.open(device_ordinal=0) as device:
+        plan, other = PreparedFP8Linear(device, weight), PreparedFP8Linear(device, weight)
+        y = plan.forward(x)
+        plan.synchronize()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            again = plan.forward(x)
+            plan.synchronize()
+            assert torch.equal(again, y)
+        device.backend.native.set_failure_mask(int(_native.FailurePoint.WAIT))
+        plan.forward(x)
+        with pytest.raises(EventTimeoutError):
+            plan.synchronize()
+        device.backend.native.set_failure_mask(0)
+        with pytest.raises(NativeError, match="poisoned"):
+            other.forward(x)
+        for each in (plan, other):
+            with pytest.raises(NativeError, match="poisoned"):
+                each.close()
+            assert each._values is None
+    with PreparedFP8Linear(cuda_device, weight) as plan:  # other contexts of the device go on
+        assert torch.equal(plan.forward(x), y)
+        plan.synchronize()
