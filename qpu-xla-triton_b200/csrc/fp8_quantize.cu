@@ -30,8 +30,9 @@ struct RowsParams {
 // every lane moves 16 bytes and the maximum is a shuffle reduction inside those lanes. A warp takes
 // STEPS steps of one or two neighbouring groups of one row, at fixed distances from one address, and
 // loads them all before it uses the first (39 against 27 us). Each input is read once, each output
-// written once; what it has to keep below HBM's time is its instructions, 14 a value. 32768 x 8192
-// bf16: 142 us (5.7 TB/s), 4096 x 8192 fp32: 27 us (6.1 TB/s), gated bf16: 39 us (4.3 TB/s).
+// written once. 32768 x 8192 bf16: 145 us (5.6 TB/s), 4096 x 8192 fp32: 29 us (5.8 TB/s), bf16 21 us
+// (4.8), gated bf16: 40 us (4.2). At 4096 x 8192 bf16 neither the issue slots (57 %, about 14 instructions a
+// value) nor the warps (54 %) are full: a warp's loads, maximum and stores follow one another.
 constexpr int kRowsThreads = 128;
 
 template <typename T, bool GATED, bool VECTOR, int STEPS>

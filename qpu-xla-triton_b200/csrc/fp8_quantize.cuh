@@ -36,23 +36,28 @@ __device__ __forceinline__ float group_scale(float amax) {
 // an fma, and RN(q1 + (x - q1 s) y) is the rounded quotient (Markstein 1990). That needs remainders
 // above the smallest normal number: true for every quotient above 2^-10, the smallest border of e4m3,
 // as s is at least 2^-60; smaller quotients end as zero whatever their last bits.
+//
+// The steps run on n = -q: the last of them adds remainder * -y to n, which for x = -0 is -0 + (+0), the
+// negative of the wanted -0; on q itself the sum of -0 and +0 would lose the sign. The four signs of a word
+// are turned at the end, but for a group of NaNs, whose bytes stay 0x7F.
 template <int N>
 __device__ __forceinline__ void quantize_values(const float (&v)[N], float scale, uint32_t (&packed)[N / 4]) {
     using sm100::fma2;
     using sm100::pack2;
     const float inverse = __frcp_rn(scale);
-    const uint64_t y = pack2(inverse, inverse), minus_s = pack2(-scale, -scale), zero = pack2(-0.0f, -0.0f);
+    const uint64_t minus_y = pack2(-inverse, -inverse), s = pack2(scale, scale), zero = pack2(-0.0f, -0.0f);
+    const uint32_t signs = scale == scale ? 0x80808080u : 0u;
     uint16_t pairs[N / 2];
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         const uint64_t x = pack2(v[i], v[i + 1]);
-        uint64_t q = fma2(x, y, zero);
-        q = fma2(fma2(q, minus_s, x), y, q);
-        q = fma2(fma2(q, minus_s, x), y, q);
-        pairs[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(sm100::low(q), sm100::high(q)), __NV_SATFINITE, __NV_E4M3);
+        uint64_t n = fma2(x, minus_y, zero);
+        n = fma2(fma2(n, s, x), minus_y, n);
+        n = fma2(fma2(n, s, x), minus_y, n);
+        pairs[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(sm100::low(n), sm100::high(n)), __NV_SATFINITE, __NV_E4M3);
     }
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) packed[i] = pairs[2 * i] | (static_cast<uint32_t>(pairs[2 * i + 1]) << 16);
+    for (int i = 0; i < N / 4; ++i) packed[i] = (pairs[2 * i] | (static_cast<uint32_t>(pairs[2 * i + 1]) << 16)) ^ signs;
 }
 
 __device__ __forceinline__ float reciprocal(float x) {
@@ -64,9 +69,10 @@ __device__ __forceinline__ float reciprocal(float x) {
 // v = silu(v) * up = v / (1 + exp(-v)) * up in fp32, every step to the last bit: a value that the
 // quantizer then rounds to three bits should not land on the other side of a border for an
 // approximation's sake. The quotient is Markstein's: q0 = g y with y within 2^-23 of 1 / d, corrected
-// by its exact remainder, is within 2^-45 of g / d before it is rounded. Below -87 the denominator's
+// by its exact remainder, is within 2^-45 of g / d before it is rounded; as above its negative is
+// formed, and multiplied by -up. Below -87 the denominator's
 // reciprocal is no normal number, and the hardware's division (-0 once exp overflows) takes over.
-// 4096 x 8192 bf16: 39 us, with a division per value 46, with the fast exp and quotient 31.
+// 4096 x 8192 bf16: 40 us, with a division per value 46, with the fast exp and quotient 31.
 template <int N>
 __device__ __forceinline__ void silu_times(float (&v)[N], const float (&up)[N]) {
     using sm100::fma2;
@@ -85,11 +91,11 @@ __device__ __forceinline__ void silu_times(float (&v)[N], const float (&up)[N]) 
     const uint64_t zero = pack2(-0.0f, -0.0f);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const uint64_t g = pack2(v[i], v[i + 1]), y = pack2(reciprocal(d[i]), reciprocal(d[i + 1]));
-        uint64_t q = fma2(g, y, zero);
-        q = fma2(fma2(q, pack2(-d[i], -d[i + 1]), g), y, q);
-        v[i] = __fmul_rn(sm100::low(q), up[i]);
-        v[i + 1] = __fmul_rn(sm100::high(q), up[i + 1]);
+        const uint64_t g = pack2(v[i], v[i + 1]), minus_y = pack2(reciprocal(-d[i]), reciprocal(-d[i + 1]));
+        uint64_t n = fma2(g, minus_y, zero);
+        n = fma2(fma2(n, pack2(d[i], d[i + 1]), g), minus_y, n);
+        v[i] = __fmul_rn(sm100::low(n), -up[i]);
+        v[i + 1] = __fmul_rn(sm100::high(n), -up[i + 1]);
     }
 }
 

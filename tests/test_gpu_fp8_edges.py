@@ -9,8 +9,8 @@ import torch
 import fp8_reference as ref
 from qpu_xla import Device, _native
 from qpu_xla.errors import EventTimeoutError, NativeError
-from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear
-from test_gpu_fp8 import blocks, check_product, draw, expert_case
+from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, quantize_blocks_fp8, quantize_rows_fp8
+from test_gpu_fp8 import DTYPES, blocks, check_product, draw, expert_case
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,42 @@ def test_an_expired_wait_reaches_the_caller_of_a_stream(cuda_device) -> None:
     with PreparedFP8Linear(cuda_device, weight) as plan:  # other contexts of the device go on
         assert torch.equal(plan.forward(x), y)
         plan.synchronize()
+
+
+def signed(shape: tuple[int, int], dtype: torch.dtype, seed: int) -> torch.Tensor:
+    """Values a third of which are zeros of either sign or so small that they end as one."""
+    x = draw(shape, dtype, seed=seed)
+    kind = torch.randint(0, 9, shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    sign = torch.where(x < 0, -1.0, 1.0).to(dtype)
+    x[kind == 0] = 0.0
+    x[kind == 1] = -0.0
+    return torch.where(kind == 2, sign * torch.finfo(dtype).tiny, x)
+
+
+def as_bytes(values: torch.Tensor) -> torch.Tensor:
+    """The bytes of float64 e4m3 values; a zero has its sign."""
+    return values.float().to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", [(1, 1), (7, 129), (40, 1000), (1200, 1003)])
+def test_quantized_bytes_keep_the_sign_of_zero(cuda_device, dtype, rows, cols) -> None:
+    x = signed((rows, cols), dtype, seed=cols)
+    x[0, 0] = -0.0
+    assert torch.equal(quantize_rows_fp8(cuda_device, x).values.view(torch.uint8), as_bytes(ref.quantize_rows(x)[0]))
+    assert torch.equal(quantize_blocks_fp8(cuda_device, x).values.view(torch.uint8), as_bytes(ref.quantize_blocks(x)[0]))
+    wide = signed((rows, cols + 2), dtype, seed=cols)[:, 1 : cols + 1]
+    assert torch.equal(quantize_rows_fp8(cuda_device, wide).values.view(torch.uint8), as_bytes(ref.quantize_rows(wide)[0]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", [(3, 128), (40, 1003)])
+@pytest.mark.parametrize("far", [False, True])
+def test_gated_bytes_have_the_sign_of_their_product(cuda_device, dtype, rows, cols, far) -> None:
+    """silu(g) has g's sign at every size, zeros included; ``far``: beside gates below -87, which go another way."""
+    x = signed((rows, 2 * cols), dtype, seed=cols)
+    if far:
+        x[:, 3::8] = -100.0
+    sign = torch.signbit(x[:, :cols]) ^ torch.signbit(x[:, cols:])
+    values = quantize_rows_fp8(cuda_device, x, gated=True).values
+    assert torch.equal(values.view(torch.uint8) >= 0x80, sign)
