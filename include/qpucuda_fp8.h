@@ -54,7 +54,10 @@ typedef struct qpucuda_fp8_quantize_desc {
     uint32_t row_divisor;
     uint32_t source_rows;
     uint8_t *q;              /* [rows] rows of q_stride bytes, 16-byte aligned */
-    size_t q_stride;         /* a multiple of 16, at least cols; up to 7 bytes past cols are zeroed */
+    /* A multiple of 16, at least cols. The bytes past cols that a 16-byte vector of x reaches (up to 7,
+     * up to 3 of fp32) are written as the quantized zeros they stand for: zero, or NaN (0x7F) in a group
+     * whose scale is NaN. The others are left as they are. */
+    size_t q_stride;
     float *scales;           /* group g of row r at r * scale_row_stride + g * scale_group_stride */
     size_t scale_row_stride;
     size_t scale_group_stride;

@@ -9,7 +9,7 @@ import torch
 import fp8_reference as ref
 from qpu_xla import Device, _native
 from qpu_xla.errors import EventTimeoutError, NativeError
-from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, quantize_blocks_fp8, quantize_rows_fp8
+from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, dtype_code, quantize_blocks_fp8, quantize_rows_fp8
 from test_gpu_fp8 import DTYPES, blocks, check_product, draw, expert_case
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +124,27 @@ def test_gated_bytes_have_the_sign_of_their_product(cuda_device, dtype, rows, co
     sign = torch.signbit(x[:, :cols]) ^ torch.signbit(x[:, cols:])
     values = quantize_rows_fp8(cuda_device, x, gated=True).values
     assert torch.equal(values.view(torch.uint8) >= 0x80, sign)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", [(5, 1), (5, 13), (5, 130), (5, 255), (1300, 1003)])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_bytes_behind_the_columns(cuda_device, dtype, rows, cols, offset) -> None:
+    """Up to a vector's end (16 bytes of the source) they are quantized zeros, NaN in a last group that holds a NaN or
+    an infinity; what lies behind that stays as it was."""
+    x = draw((rows, cols + 8), dtype, seed=cols)[:, offset : cols + offset]
+    x[1, cols - 1] = float("nan")
+    x[2, (cols - 1) // 128 * 128] = -float("inf")
+    stride = -(-cols // 16) * 16 + 16
+    values = torch.full((rows, stride), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.empty((rows, -(-cols // 128)), device="cuda")
+    desc = _native.Fp8QuantizeDesc(
+        x.data_ptr(), dtype_code(dtype, "x"), x.stride(0), rows, cols, 0, None, 1, rows, values.data_ptr(), stride, scales.data_ptr(), scales.shape[1], 1
+    )
+    cuda_device.backend.call("qpucuda_fp8_quantize_rows", (bytes(desc),), cuda_device.backend.current_stream_handle)
+    end = cols + -cols % (16 // x.element_size())
+    assert (values[1:3, cols:end] == 0x7F).all() and (values[0, cols:end] == 0).all() and (values[3:, cols:end] == 0).all()
+    assert (values[:, end:] == 0x55).all()
+    quantized = quantize_rows_fp8(cuda_device, x)
+    assert torch.equal(values[:, :cols], quantized.values.view(torch.uint8))
+    assert quantized.values[1, cols - 1].isnan() and quantized.values[2, (cols - 1) // 128 * 128].isnan()
