@@ -229,8 +229,10 @@ def quantize_blocks_fp8(device: Device, weight: Any) -> QuantizedBlocksFP8:
         raise ValueError("quantize_blocks_fp8 requires a non-empty rank-2 or rank-3 weight")
     if weight.device != torch_device:
         raise ValueError(f"quantize_blocks_fp8 weight must be on {torch_device}")
-    weight = weight.contiguous()
     *batch, rows, cols = weight.shape
+    if rows > 65535 * FP8_GROUP or cols >= 2**31 or (batch and batch[0] > 65535):
+        raise ValueError(f"quantize_blocks_fp8 takes fewer than 65536 matrices of fewer than {65535 * FP8_GROUP + 1} rows and 2**31 columns")
+    weight = weight.contiguous()
     values = torch.empty(weight.shape, dtype=torch.float8_e4m3fn, device=torch_device)
     scales = torch.empty((*batch, groups_of(rows), groups_of(cols)), dtype=torch.float32, device=torch_device)
     launch(

@@ -13,7 +13,7 @@ import torch
 
 from qpu_xla.errors import EventTimeoutError, NativeError
 from qpu_xla.experts import ExpertOrder, FP8ExpertsFFN, combine_tokens, gather_tokens, gather_tokens_backward
-from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, QuantizedRowsFP8, check_apart_from
+from qpu_xla.fp8 import PreparedFP8Experts, PreparedFP8Linear, QuantizedRowsFP8, check_apart_from, quantize_blocks_fp8
 
 E4M3 = torch.float8_e4m3fn
 
@@ -223,3 +223,13 @@ def test_no_wait_while_a_graph_is_captured(waiting_device: RecordingDevice, monk
     with pytest.raises(RuntimeError, match="captured"):
         plan_of(PreparedFP8Linear, waiting_device, n=4, k=16).synchronize()
     assert waiting_device.backend.native.waits == []
+
+
+@pytest.mark.parametrize("shape", [(1, 2**32 + 1), (2**31, 1), (2, 2**31, 1), (2**16, 1, 1)])
+def test_weights_past_the_quantizers_extents_are_refused(shape: tuple[int, ...]) -> None:
+    """A C extent has 32 bits (2**32 + 1 columns would pass as one), a grid 65535 matrices."""
+    device = RecordingDevice()
+    device.backend.torch_device = torch.device("meta")
+    with pytest.raises(ValueError, match="fewer than"):
+        quantize_blocks_fp8(device, torch.empty(shape, dtype=torch.float16, device="meta"))
+    assert device.calls == []
