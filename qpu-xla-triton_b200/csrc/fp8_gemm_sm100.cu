@@ -582,9 +582,11 @@ cudaError_t launch_narrow_rows(const CUtensorMap &map_w, const CUtensorMap &map_
 //
 // Per block of 128 columns a CTA's MMAs take 512 cycles in a pair (768 alone: both operands then come
 // from one SM's shared memory), its eight epilogue warps read 128 KB of tensor memory and form 32768
-// multiply-adds in registers meanwhile. 4096 x 28672 x 8192 bf16 in pairs: 920 us, 2.1 PFLOP/s (1.26 of
-// the measured bf16 burst), at the 1000 W power limit. Without the sums 845 us, without reading the
-// accumulators either 745, the MMAs alone 650: what is left is energy, not waiting.
+// multiply-adds in registers meanwhile. 4096 x 28672 x 8192 bf16 in pairs: 900 us in a short run, 2.1
+// PFLOP/s (1.28 of the measured bf16 burst); 1040 us, 1.11, once the 1000 W limit holds the clock at 1.6 GHz.
+// By parts, in runs of one length: 920 us whole, without the sums 845, without reading the accumulators
+// either 745, the MMAs alone 650. Where power does not decide (4096 x 5632 x 8192, 170 us: tensor pipe 57 %
+// active, issue slots 38 %) the pipe waits for the accumulators' way through registers.
 constexpr int kWideM = 128;
 constexpr int kWideN = 256;
 constexpr uint64_t kGroupBytes = 40ull << 20;  // rows of a group of tiles: part of the 126 MB L2

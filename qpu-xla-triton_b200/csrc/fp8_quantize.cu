@@ -30,8 +30,8 @@ struct RowsParams {
 // every lane moves 16 bytes and the maximum is a shuffle reduction inside those lanes. A warp takes
 // STEPS steps of one or two neighbouring groups of one row, at fixed distances from one address, and
 // loads them all before it uses the first (39 against 27 us). Each input is read once, each output
-// written once. 32768 x 8192 bf16: 145 us (5.6 TB/s), 4096 x 8192 fp32: 29 us (5.8 TB/s), bf16 21 us
-// (4.8), gated bf16: 40 us (4.2). At 4096 x 8192 bf16 neither the issue slots (57 %, about 14 instructions a
+// written once. 32768 x 8192 bf16: 145 us (5.6 TB/s), 4096 x 8192 fp32: 29 us (5.8 TB/s), bf16 20 us
+// (5.1), gated bf16: 39 us (4.3). At 4096 x 8192 bf16 neither the issue slots (57 %, about 14 instructions a
 // value) nor the warps (54 %) are full: a warp's loads, maximum and stores follow one another.
 constexpr int kRowsThreads = 128;
 
@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kRowsThreads) quantize_rows_fp8_kernel(const R
 // One CTA per 128 x 128 block, held in registers between its maximum and its values: a warp's lanes
 // take four neighbouring columns each, its rows are 16 apart. WHOLE: rows of x and q allow vectors of
 // four; the ragged blocks of such a matrix go element by element all the same. Runs once per weight,
-// when it is prepared: 28672 x 8192 fp32 196 us (6.0 TB/s; 488 us with a second read in place of the
-// registers), bf16 330.
+// when it is prepared: 28672 x 8192 fp32 195 us (6.0 TB/s; 488 us with a second read in place of the
+// registers), bf16 343 (2.1 TB/s: a lane loads 8 bytes a row where fp32 loads 16).
 constexpr int kBlockThreads = 512;
 
 template <typename T>
