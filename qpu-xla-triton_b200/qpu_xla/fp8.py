@@ -311,13 +311,15 @@ class _PreparedFP8:
             raise RuntimeError(f"{self._name} plan is closed")
 
     def synchronize(self: Self) -> None:
-        """Wait for the device's current stream (up to the device's timeout) and raise if a kernel's wait ran out,
-        in a call of any plan of the device: ``EventTimeoutError`` the first time, ``NativeError`` from then on."""
+        """Wait for the device's current stream and raise if a kernel's wait ran out, in a call of any plan of the
+        device: ``EventTimeoutError`` the first time, ``NativeError`` from then on."""
         self._require_open()
         with torch.cuda.device(self._torch_device):
             capturing = torch.cuda.is_current_stream_capturing()
         if capturing:
             raise RuntimeError(f"{self._name} calls cannot be waited for while a graph is captured")
+        # without the launch lock, which other threads' calls need, and past the device's timeout if it takes that
+        torch.cuda.current_stream(self._torch_device).synchronize()
         self._raise_device_errors()
 
     def _raise_device_errors(self: Self) -> None:

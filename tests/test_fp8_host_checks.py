@@ -162,12 +162,13 @@ def waiting_device(monkeypatch: pytest.MonkeyPatch) -> RecordingDevice:
     device, native = RecordingDevice(), FakeNative()
 
     def launch(stream: Any, fn: Any) -> Any:
-        native.waits.append(stream)
+        native.waits.append("error word")
         return fn(native)
 
     device.backend.native, device.backend.launch = native, launch
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: native.waits.append("device"))
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "current")
+    current = SimpleNamespace(synchronize=lambda: native.waits.append("stream"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: current)
     monkeypatch.setattr(torch.cuda, "device", lambda device: nullcontext())
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return device
@@ -178,13 +179,13 @@ def test_an_expired_wait_of_a_stream_call_is_raised(waiting_device: RecordingDev
     native = waiting_device.backend.native
     with plan_of(PreparedFP8Linear, waiting_device, n=4, k=16) as plan:
         plan.synchronize()
-        assert native.waits == ["current"]
+        assert native.waits == ["stream", "error word"]
         native.expired = True
         with pytest.raises(EventTimeoutError, match="exceeded its bound"):
             plan.synchronize()
         with pytest.raises(NativeError, match="poisoned"):
             plan.close()
-    assert native.waits[-2:] == ["device", "current"]  # everything has ended before the error word is read
+    assert native.waits[-2:] == ["device", "error word"]  # everything has ended before the error word is read
     with pytest.raises(RuntimeError, match="closed"):
         plan.synchronize()
 
